@@ -36,11 +36,20 @@ enum {
     LL_ERR_BUSY = 8          /* a request is still outstanding */
 };
 
-/* ---- activations (include/ll/dense_warp.cuh:9-21 ActIdentity/ActRelu; GELU is new) ---- */
-enum { LL_ACT_IDENTITY = 0, LL_ACT_RELU = 1, LL_ACT_GELU = 2 };
+/* ---- activations (include/ll/dense_warp.cuh:9-21 ActIdentity/ActRelu; GELU and SiLU are new) ----
+ * LL_ACT_SILU, v / (1 + exp(-v)), is taken by the calls that run one layer at a time (ll_dense_*,
+ * ll_moe_forward, ll_mlp_forward_noalloc, the launch-per-layer chain); the resident engines and
+ * ll_batched_mlp refuse it. */
+enum { LL_ACT_IDENTITY = 0, LL_ACT_RELU = 1, LL_ACT_GELU = 2, LL_ACT_SILU = 3 };
 
-/* ---- weight storage types ---- */
-enum { LL_W_F32 = 0, LL_W_BF16 = 1, LL_W_I8 = 2 };
+/* ---- weight storage types ----
+ * LL_W_F8, e4m3 with one fp32 scale per block of 128 x 128, is a type of ll_moe_forward's experts and
+ * the one that ll_dense_fp8 reads; the engines, ll_batched_mlp and weight files refuse it. */
+enum { LL_W_F32 = 0, LL_W_BF16 = 1, LL_W_I8 = 2, LL_W_F8 = 3 };
+
+/* ---- element types of activations on the device (the operators that take more than fp32) ---- */
+enum { LL_T_F32 = 0, LL_T_BF16 = 1, LL_T_F16 = 2, LL_T_F8 = 3 /* e4m3 bytes, scales beside them */ };
+#define LL_F8_BLOCK 128 /* columns of a row, or rows and columns of a weight matrix, that share a scale */
 
 /* ---- initialisers for ll_init_params ---- */
 enum { LL_INIT_XAVIER_UNIFORM = 0, LL_INIT_NORMAL_FANIN = 1 };
@@ -412,6 +421,47 @@ int ll_batched_mlp_info(ll_batched_mlp *m, ll_batched_info *info);
  * for the MMA, 13 first stage re-issued, 14 that stage ready, 15 K step 0 converted (int8). */
 int ll_batched_mlp_set_trace(ll_batched_mlp *m, unsigned long long *d_trace, size_t n);
 int ll_batched_mlp_destroy(ll_batched_mlp *m);
+
+/*
+ * Dense layers in 8-bit floating point (no counterpart in the reference, which is fp32 only; the
+ * layer contract y = act(W x + b) is its own, include/ll/dense_warp.cuh:33-90).  Values are e4m3
+ * (largest 448); each value stands for itself times the fp32 scale of its block: activations have
+ * one scale per row and 128 columns, weights one per 128 rows x 128 columns (the last block of a
+ * row, column or matrix may be short).
+ *
+ * These calls keep nothing between them, allocate nothing and run on `stream` and the current
+ * device, whose memory every pointer must name (checked: LL_ERR_INVALID_ARG).  They can be
+ * captured into graphs and called from several threads and streams at once, on buffers of their
+ * own.  Make the first call of each per device before any capture.
+ *
+ * ll_quantize_fp8: x [rows x dim] (fp32, bf16 or fp16, row stride ldx elements) to e4m3 bytes q
+ * (row stride ldq bytes) and scales s [rows][ceil(dim / 128)]: s = max|x| / 448 of the group in
+ * fp32 (at least 2^-126; the power of two at or above that when pow2_scales = 1), q = e4m3 nearest
+ * to x / s, ties to even.  A group of zeros has scale 0.  NaN stays in its place; a group that
+ * holds an infinity gets an infinite scale and stands for NaN throughout.  Strides of 0 mean dim.
+ * Bytes of a row of q from dim on are left as they are.
+ */
+int ll_quantize_fp8(const void *d_x, int x_type, int rows, int dim, int64_t ldx, int pow2_scales, uint8_t *d_q,
+                    int64_t ldq, float *d_s, void *stream);
+/* The same for a weight matrix on the host, W [m x k] row-major: q [m x k], s [ceil(m/128)][ceil(k/128)],
+ * s = max|W| / 448 of the block (1 for a block of zeros), q nearest to W / s. */
+void ll_quantize_fp8_blocks(const float *W, int m, int k, uint8_t *q, float *s);
+/*
+ * ll_dense_fp8: y[r] = act(W x[r] + b) for `rows` rows on the tensor cores, W [M x K] e4m3 with
+ * scales sw [ceil(M/128)][ceil(K/128)], x [rows x K] e4m3 with scales sx [rows][ceil(K/128)], b fp32
+ * [M] or NULL.  Sums are fp32.  y_type: LL_T_F32, LL_T_BF16, LL_T_F16 (d_sy unused), or LL_T_F8: y as
+ * ll_quantize_fp8 would make it of the fp32 result (the next layer's input), its scales in
+ * d_sy [rows][ceil(M/128)].  ldw, ldx (bytes) and ldy (elements): row strides, 0 = dense; the rows
+ * of W and x start on 16 bytes, so ldw and ldx are multiples of 16.  What lies beyond column K of
+ * a row is not used.  rows = 0 does nothing.  Returns launch errors; ll_ops_check reports a device-side one.
+ */
+int ll_dense_fp8(const uint8_t *d_W, const float *d_sw, const float *d_b, const uint8_t *d_x, const float *d_sx,
+                 void *d_y, float *d_sy, int y_type, int rows, int M, int K, int64_t ldw, int64_t ldx, int64_t ldy,
+                 int act, void *stream);
+/* Synchronise `stream` and read the current device's status word of ll_dense_fp8 and ll_moe_forward:
+ * LL_OK, or LL_ERR_DEVICE_FAULT when a bounded device-side wait ran out since the last check (the
+ * outputs of the calls since then are not to be used; the word is cleared). */
+int ll_ops_check(void *stream);
 
 /* Host packing, include/ll/pack_weights.cuh:16-32. */
 void ll_pack_rm_to_kmajor_padded(const float *W_rm, size_t M, size_t K, float *W_cm, size_t Mpad);

@@ -30,8 +30,10 @@ LIB_PATH = os.path.join(_HERE, "_lib", "libll_b200.so")
 # ---- constants (include/ll_b200.h) ----
 LL_OK, LL_ERR_CUDA, LL_ERR_TIMEOUT, LL_ERR_BAD_DESC, LL_ERR_DEVICE_FAULT = 0, 1, 2, 3, 4
 LL_ERR_STOPPED, LL_ERR_INVALID_ARG, LL_ERR_UNSUPPORTED, LL_ERR_BUSY = 5, 6, 7, 8
-ACT_IDENTITY, ACT_RELU, ACT_GELU = 0, 1, 2
-W_F32, W_BF16, W_I8 = 0, 1, 2
+ACT_IDENTITY, ACT_RELU, ACT_GELU, ACT_SILU = 0, 1, 2, 3
+W_F32, W_BF16, W_I8, W_F8 = 0, 1, 2, 3
+T_F32, T_BF16, T_F16, T_F8 = 0, 1, 2, 3
+F8_BLOCK = 128
 INIT_XAVIER_UNIFORM, INIT_NORMAL_FANIN = 0, 1
 RUN_DIRECT_KERNEL, RUN_GRAPH_KERNEL, RUN_GRAPH_E2E, RUN_DIRECT_E2E, RUN_MAILBOX_TICK = 0, 1, 2, 3, 4
 STOP_SEQ = 0xFFFFFFFF
@@ -58,6 +60,7 @@ EXPORTED_SYMBOLS = [
     "ll_batched_mlp_set_trace", "ll_engine_serve_poisson",
     "ll_weights_save", "ll_weights_load", "ll_weights_net", "ll_weights_arrays", "ll_weights_free",
     "ll_submit_many", "ll_engine_bench_ring", "ll_engine_bench_ring_mt",
+    "ll_quantize_fp8", "ll_quantize_fp8_blocks", "ll_dense_fp8", "ll_ops_check",
 ]
 MAX_LAYERS = 24
 
@@ -222,6 +225,13 @@ def _sig(lib):
         "ll_engine_bench_ring": (ctypes.c_int, [_vp, _fp, ctypes.c_int, ctypes.c_int, ctypes.c_int, _fp, _dp, _dp]),
         "ll_engine_bench_ring_mt": (ctypes.c_int, [_vp, _fp, ctypes.c_int, ctypes.c_int, ctypes.c_int, _fp, _dp, _dp,
                                                     ctypes.c_int]),
+        "ll_quantize_fp8": (ctypes.c_int, [_vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int64, ctypes.c_int,
+                                           _vp, ctypes.c_int64, _vp, _vp]),
+        "ll_quantize_fp8_blocks": (None, [_fp, ctypes.c_int, ctypes.c_int, P(ctypes.c_uint8), _fp]),
+        "ll_dense_fp8": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int,
+                                        ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int,
+                                        _vp]),
+        "ll_ops_check": (ctypes.c_int, [_vp]),
     }
     for name, (res, args) in s.items():
         f = getattr(lib, name)
@@ -326,6 +336,16 @@ def quantize_int8_rows(W: np.ndarray):
     q = np.empty((m, k), np.int8)
     s = np.empty(m, np.float32)
     lib().ll_quantize_int8_rows(_f(W), m, k, q.ctypes.data_as(ctypes.POINTER(ctypes.c_int8)), _f(s))
+    return q, s
+
+
+def quantize_fp8_blocks(W: np.ndarray):
+    """e4m3 bytes and fp32 scales of W per block of 128 x 128 (ll_quantize_fp8_blocks, on the host)."""
+    W = np.ascontiguousarray(W, np.float32)
+    m, k = W.shape
+    q = np.empty((m, k), np.uint8)
+    s = np.empty((-(-m // F8_BLOCK), -(-k // F8_BLOCK)), np.float32)
+    lib().ll_quantize_fp8_blocks(_f(W), m, k, q.ctypes.data_as(ctypes.POINTER(ctypes.c_uint8)), _f(s))
     return q, s
 
 
@@ -635,6 +655,26 @@ def dense_warp_rm(W_ptr: int, b_ptr: int, x_ptr: int, y_ptr: int, M: int, K: int
 def dense_mbyv_packed(Wcm_ptr: int, bpad_ptr: int, x_ptr: int, y_ptr: int, M: int, K: int, act: int,
                       stream: int = 0):
     _check(lib().ll_dense_mbyv_packed(Wcm_ptr, bpad_ptr, x_ptr, y_ptr, M, K, act, stream or None))
+
+
+def quantize_fp8(x_ptr: int, x_type: int, rows: int, dim: int, q_ptr: int, s_ptr: int, ldx: int = 0, ldq: int = 0,
+                 pow2: bool = False, stream: int = 0):
+    """Rows of x (T_F32, T_BF16 or T_F16) to e4m3 bytes and one fp32 scale per row and 128 columns (ll_quantize_fp8)."""
+    _check(lib().ll_quantize_fp8(x_ptr or None, x_type, rows, dim, ldx, int(pow2), q_ptr or None, ldq, s_ptr or None,
+                                 stream or None))
+
+
+def dense_fp8(W_ptr: int, sw_ptr: int, b_ptr: int, x_ptr: int, sx_ptr: int, y_ptr: int, rows: int, M: int, K: int,
+              act: int = ACT_IDENTITY, y_type: int = T_F32, sy_ptr: int = 0, ldw: int = 0, ldx: int = 0, ldy: int = 0,
+              stream: int = 0):
+    """y = act(W x + b) on e4m3 operands with block scales (ll_dense_fp8); y_type T_F8 needs sy_ptr."""
+    _check(lib().ll_dense_fp8(W_ptr or None, sw_ptr or None, b_ptr or None, x_ptr or None, sx_ptr or None,
+                              y_ptr or None, sy_ptr or None, y_type, rows, M, K, ldw, ldx, ldy, act, stream or None))
+
+
+def ops_check(stream: int = 0):
+    """Raise if a device-side wait of dense_fp8 or moe_forward ran out since the last check (ll_ops_check)."""
+    _check(lib().ll_ops_check(stream or None))
 
 
 def plan_net(net: Net, W=None, b=None, scales=None, opts: Optional[EngineOpts] = None, want_images: bool = False):

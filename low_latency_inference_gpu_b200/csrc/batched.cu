@@ -5,11 +5,9 @@
 // between layers as bf16 row-major buffers padded to 128 rows.
 #include <cuda.h>
 #include <cuda_runtime.h>
-#include <cudaTypedefs.h>
 
 #include <algorithm>
 #include <cstring>
-#include <mutex>
 #include <vector>
 
 #include "common.h"
@@ -18,6 +16,7 @@
 #include "tc_layer.cuh"
 #include "tc_swap.cuh"
 #include "tc_swap2.cuh"
+#include "tmap.h"
 
 using namespace llk;
 
@@ -244,25 +243,11 @@ void fill_info(const ll_net_desc *net, const ll_batched_opts *o, ll_batched_info
     }
 }
 
-PFN_cuTensorMapEncodeTiled_v12000 encode_fn()
-{
-    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-    static std::once_flag once;
-    std::call_once(once, [] {
-        void *p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
-    });
-    return fn;
-}
-
 // 2-D row-major tensor map: inner dim `cols` elements, `rows` rows, box {64, box_rows}.
 bool make_map(CUtensorMap *m, CUtensorMapDataType t, int esize, const void *base, int cols, int rows, int box_rows,
               CUtensorMapSwizzle swizzle)
 {
-    auto fn = encode_fn();
+    auto fn = llh::encode_fn();
     if (!fn)
         return false;
     cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
@@ -279,7 +264,7 @@ bool make_map(CUtensorMap *m, CUtensorMapDataType t, int esize, const void *base
 bool make_map_grouped(CUtensorMap *m, CUtensorMapDataType t, int esize, const void *base, int cols, int rows,
                       int box_rows, int group, CUtensorMapSwizzle swizzle)
 {
-    auto fn = encode_fn();
+    auto fn = llh::encode_fn();
     if (!fn)
         return false;
     cuuint64_t dims[3] = {(cuuint64_t)kTcK, (cuuint64_t)rows, (cuuint64_t)(cols / kTcK)};
@@ -484,7 +469,7 @@ int ll_batched_mlp_create(const ll_net_desc *net, const void *const *W, const fl
             return LL_ERR_INVALID_ARG;
         }
     }
-    if (!encode_fn()) {
+    if (!llh::encode_fn()) {
         llh::set_error("cuTensorMapEncodeTiled is not available from the driver");
         return LL_ERR_CUDA;
     }

@@ -1,0 +1,473 @@
+// ll_dense_fp8: y = act(W x + b) on e4m3 operands (no counterpart in the reference, whose dense
+// layers are fp32: include/ll/dense_warp.cuh:33-90; the layer contract is the same).
+//
+//   y[r, m] = act( sum_kb sx[r, kb] sw[m / 128, kb] ( sum_{k in kb} x[r, k] W[m, k] ) + b[m] )
+//
+// with kb the 128-column blocks of K.  A block's products are summed by the tensor cores
+// (tcgen05.mma kind::f8f6f4, fp32 accumulator in TMEM), started afresh for every block; the
+// block's two scales multiply the sum on its way into a second accumulator in registers.
+#include <algorithm>
+#include <cstring>
+
+#include "ops_common.cuh"
+#include "tc_layer.cuh"
+#include "tmap.h"
+
+namespace llk {
+
+struct DenseF8Params {
+    CUtensorMap tm_w;   // e4m3 [M][K], box {128, 128}, 128-byte swizzle
+    CUtensorMap tm_x;   // e4m3 [rows][K], box {128, NT}, 128-byte swizzle
+    const float *sw;    // [ceil(M / 128)][nkb]
+    const float *sx;    // [rows][nkb]
+    const float *bias;  // [M] or nullptr
+    void *y;
+    float *sy;          // [rows][ceil(M / 128)] (e4m3 output)
+    long long ldy;
+    int rows, M, nkb, kb_split;  // kb_split: K blocks per CTA of the cluster
+    int act, y_type, y_vec;      // y_vec: 4 consecutive outputs may be stored at once
+    unsigned *status;
+    unsigned long long wait_ns;
+};
+
+// Instruction descriptor, kind::f8f6f4: A = B = e4m3, D = fp32, both K-major, M = 128, N = n.
+__host__ __device__ constexpr uint32_t tc_idesc_e4m3(int n)
+{
+    return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+
+__device__ __forceinline__ void tc_mma_f8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                          uint32_t accumulate)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// 32 lanes x 16 consecutive fp32 columns, waited for.
+__device__ __forceinline__ void tc_ld_16cols(uint32_t taddr, float (&v)[16])
+{
+    uint32_t r[16];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+        v[i] = __uint_as_float(r[i]);
+}
+
+__device__ __forceinline__ float4 ld_cluster_v4(uint32_t cluster_addr)
+{
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(cluster_addr)
+                 : "memory");
+    return v;
+}
+
+// Four consecutive outputs of row `row` from channel m on; a warp holds one row's 128 channels of
+// one tile (lane l: 4 l ..), so the e4m3 output's group maximum is a warp reduction.
+__device__ __forceinline__ void store_y4(const DenseF8Params &p, long long row, int m, float (&v)[4], int mtile)
+{
+    const int have = p.M - m;  // <= 0: past the last channel
+    if (p.y_type == LL_T_F8) {
+        float amax = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i < have)
+                amax = fmaxf(amax, fabsf(v[i]));
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1)
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
+        float s, inv;
+        e4m3_scale(amax, false, s, inv);
+        const uint32_t o = group_e4m3x4(v, false, s, inv);
+        uint8_t *q = static_cast<uint8_t *>(p.y) + row * p.ldy + m;
+        if (have >= 4 && p.y_vec) {
+            *reinterpret_cast<uint32_t *>(q) = o;
+        } else {
+            for (int i = 0; i < 4; ++i)
+                if (i < have)
+                    q[i] = (uint8_t)(o >> (8 * i));
+        }
+        if ((threadIdx.x & 31) == 0)
+            p.sy[row * ((p.M + kF8Block - 1) / kF8Block) + mtile] = s;
+    } else if (p.y_type == LL_T_F32) {
+        float *q = static_cast<float *>(p.y) + row * p.ldy + m;
+        if (have >= 4 && p.y_vec) {
+            *reinterpret_cast<float4 *>(q) = make_float4(v[0], v[1], v[2], v[3]);
+        } else {
+            for (int i = 0; i < 4; ++i)
+                if (i < have)
+                    q[i] = v[i];
+        }
+    } else {
+        uint16_t h[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            h[i] = p.y_type == LL_T_BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v[i]))
+                                         : __half_as_ushort(__float2half_rn(v[i]));
+        uint16_t *q = static_cast<uint16_t *>(p.y) + row * p.ldy + m;
+        if (have >= 4 && p.y_vec) {
+            *reinterpret_cast<uint2 *>(q) =
+                make_uint2((uint32_t)h[0] | ((uint32_t)h[1] << 16), (uint32_t)h[2] | ((uint32_t)h[3] << 16));
+        } else {
+            for (int i = 0; i < 4; ++i)
+                if (i < have)
+                    q[i] = h[i];
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Few rows: D[128 channels x NT rows] = W tile . X^T, so a weight tile is the MMA's A operand and
+// few rows are a narrow N.  The K blocks of a tile are split over the CTAs of one cluster (grid z),
+// which add their partial tiles through distributed shared memory in rank order.
+//   warp 0     TMA producer (W box 16 KB + X box NT * 128 B per K block)
+//   warp 1     TMEM allocation; one thread issues the MMAs (two accumulators in turn)
+//   warps 2-5  lane = channel: TMEM -> registers, times the block's scales
+//   all        sum of the cluster's partials of this CTA's rows, bias, activation, store
+constexpr int kDsThreads = 192;
+constexpr int kDsScaleKb = 8;  // K blocks whose scales are staged at once
+
+template <int NT>
+struct DsSmem {
+    static constexpr int WB = 128 * kF8Block;
+    static constexpr int XB = NT * kF8Block;
+    static constexpr int STAGE = WB + XB;
+    static constexpr int STAGES = NT <= 32 ? 8 : 6;
+    static constexpr int OFF_SC = STAGES * STAGE;  // sx * sw: [4 warps][kDsScaleKb][NT] fp32
+    static constexpr int OFF_BAR = OFF_SC + 4 * kDsScaleKb * NT * 4;  // full[S], empty[S], accfull[2], accempty[2], done
+    static constexpr int N_BAR = 2 * STAGES + 5;
+    static constexpr int OFF_MISC = OFF_BAR + 8 * N_BAR;          // tmem base, fail flag
+    static constexpr int ALLOC = OFF_MISC + 16 + 1024;
+    static constexpr int PART_LD = 128;                           // partial tile [NT][128] in the idle ring
+    static_assert(NT * PART_LD * 4 <= STAGES * STAGE, "the partial tile fits the ring");
+    static_assert(ALLOC <= 227 * 1024, "shared memory");
+    static constexpr uint32_t TMEM_COLS = 2 * NT < 32 ? 32 : 2 * NT;
+};
+
+template <int NT>
+__global__ void __launch_bounds__(kDsThreads, 1) ll_dense_fp8_kernel(const __grid_constant__ DenseF8Params p)
+{
+    using L = DsSmem<NT>;
+    constexpr int S = L::STAGES;
+    extern __shared__ uint8_t ds_smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(ds_smem_raw) + 1023) & ~uintptr_t(1023));
+    const uint32_t sbase = smem_u32(smem);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    uint32_t *misc = reinterpret_cast<uint32_t *>(smem + L::OFF_MISC);
+    volatile uint32_t *fail = misc + 1;
+    float *s_sc = reinterpret_cast<float *>(smem + L::OFF_SC);
+    float *s_part = reinterpret_cast<float *>(smem);
+    auto bar = [&](int i) { return sbase + (uint32_t)L::OFF_BAR + 8u * (uint32_t)i; };
+    auto b_full = [&](int s) { return bar(s); };
+    auto b_empty = [&](int s) { return bar(S + s); };
+    auto b_accf = [&](int b) { return bar(2 * S + b); };
+    auto b_acce = [&](int b) { return bar(2 * S + 2 + b); };
+    const uint32_t b_done = bar(2 * S + 4);
+
+    const int splits = (int)gridDim.z, rank = (int)blockIdx.z;  // the cluster is the z extent
+    const int mtile = blockIdx.x, m0 = mtile * 128;
+    const long long t0 = (long long)blockIdx.y * NT;
+    const int kb0 = rank * p.kb_split, nkb = max(0, min(p.kb_split, p.nkb - kb0));
+
+    if (tid == 0) {
+        for (int s = 0; s < S; ++s) {
+            mbar_init(b_full(s), 1);
+            mbar_init(b_empty(s), 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(b_accf(b), 1);
+            mbar_init(b_acce(b), 4);
+        }
+        mbar_init(b_done, 1);
+        misc[1] = 0;
+        fence_mbar_init_cluster();
+        prefetch_tmap(&p.tm_w);
+        prefetch_tmap(&p.tm_x);
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                         sbase + (uint32_t)L::OFF_MISC),
+                     "r"(L::TMEM_COLS)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = misc[0];
+
+    int issued = 0;  // producer: K blocks whose loads were started
+    if (warp == 0) {
+        if (lane == 0) {
+            for (int j = 0; j < nkb; ++j) {
+                const int s = j % S;
+                if (j >= S && !tc_wait(b_empty(s), ((j / S) - 1) & 1, p.wait_ns, fail, p.status, 1))
+                    break;
+                mbar_arrive_expect_tx(b_full(s), L::STAGE);
+                tma_load_2d(sbase + s * L::STAGE, &p.tm_w, (kb0 + j) * kF8Block, m0, b_full(s));
+                tma_load_2d(sbase + s * L::STAGE + L::WB, &p.tm_x, (kb0 + j) * kF8Block, (int)t0, b_full(s));
+                issued = j + 1;
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            constexpr uint32_t idesc = tc_idesc_e4m3(NT);
+            for (int j = 0; j < nkb; ++j) {
+                const int s = j % S, b = j & 1;
+                if (j >= 2 && !tc_wait(b_acce(b), ((j / 2) - 1) & 1, p.wait_ns, fail, p.status, 2))
+                    break;
+                if (!tc_wait(b_full(s), (j / S) & 1, p.wait_ns, fail, p.status, 3))
+                    break;
+                tc_fence_after();
+                const uint32_t a = sbase + s * L::STAGE, x = a + L::WB;
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk)
+                    tc_mma_f8(tmem + (uint32_t)(b * NT), sw128_kmajor_desc(a + kk * 32), sw128_kmajor_desc(x + kk * 32),
+                              idesc, kk != 0);
+                tc_commit(b_empty(s));
+                tc_commit(b_accf(b));
+            }
+            tc_commit(b_done);
+        }
+    } else {
+        const int quad = warp & 3, chan = 32 * quad + lane;
+        float *w_sc = s_sc + quad * (kDsScaleKb * NT);
+        const float *sw = p.sw + (size_t)mtile * p.nkb + kb0;
+        float acc[NT];
+#pragma unroll
+        for (int c = 0; c < NT; ++c)
+            acc[c] = 0.0f;
+        for (int j = 0; j < nkb; ++j) {
+            if (j % kDsScaleKb == 0) {  // the next blocks' scales, a copy per warp: no warp waits for another
+                const int n = min(kDsScaleKb, nkb - j);
+                __syncwarp();
+                for (int i = lane; i < n * NT; i += 32) {
+                    const int c = i / n, jj = i - c * n;  // consecutive lanes: consecutive blocks of a row
+                    const long long row = t0 + c;
+                    w_sc[jj * NT + c] =
+                        row < p.rows ? __ldg(p.sx + row * p.nkb + kb0 + j + jj) * __ldg(sw + j + jj) : 0.0f;
+                }
+                __syncwarp();
+            }
+            const int b = j & 1;
+            if (!tc_wait_warp(b_accf(b), (j / 2) & 1, p.wait_ns, fail, p.status, 4))
+                break;
+            tc_fence_after();
+            const float *sc = w_sc + (j % kDsScaleKb) * NT;
+#pragma unroll
+            for (int c0 = 0; c0 < NT; c0 += 16) {
+                float v[16];
+                tc_ld_16cols(tmem + ((uint32_t)(32 * quad) << 16) + (uint32_t)(b * NT + c0), v);
+#pragma unroll
+                for (int c = 0; c < 16; c += 4) {
+                    const float4 f = *reinterpret_cast<const float4 *>(sc + c0 + c);
+                    acc[c0 + c] = fmaf(v[c], f.x, acc[c0 + c]);
+                    acc[c0 + c + 1] = fmaf(v[c + 1], f.y, acc[c0 + c + 1]);
+                    acc[c0 + c + 2] = fmaf(v[c + 2], f.z, acc[c0 + c + 2]);
+                    acc[c0 + c + 3] = fmaf(v[c + 3], f.w, acc[c0 + c + 3]);
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0)
+                mbar_arrive_local(b_acce(b));
+        }
+        // every MMA has read the ring before the partial tile overwrites it
+        tc_wait_warp(b_done, 0, p.wait_ns, fail, p.status, 5);
+#pragma unroll
+        for (int c = 0; c < NT; ++c)
+            s_part[c * L::PART_LD + chan] = acc[c];
+    }
+    // A CTA that gave up leaves loads in flight: they land before its shared memory is given back.
+    if (warp == 0 && lane == 0 && *fail) {
+        for (int j = max(0, issued - S); j < issued; ++j) {
+            const uint64_t w0 = globaltimer();
+            while (!mbar_try_wait(b_full(j % S), (j / S) & 1) && globaltimer() - w0 < p.wait_ns) {
+            }
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        if (*fail && lane == 0) {
+            const uint64_t w0 = globaltimer();
+            while (!mbar_try_wait(b_done, 0) && globaltimer() - w0 < p.wait_ns) {
+            }
+        }
+        __syncwarp();
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(L::TMEM_COLS)
+                     : "memory");
+    }
+    if (splits > 1)
+        cluster_sync();  // every partial tile of the cluster is written
+
+    const uint32_t part = smem_u32(s_part);
+    if (*fail == 0) {
+        const int m = m0 + 4 * lane;
+        float bias[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            bias[i] = p.bias && m + i < p.M ? __ldg(p.bias + m + i) : 0.0f;
+        for (int c = rank + splits * warp; c < NT && t0 + c < p.rows; c += splits * (kDsThreads / 32)) {
+            const uint32_t at = part + (uint32_t)(c * L::PART_LD + 4 * lane) * 4u;
+            float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int r = 0; r < splits; ++r) {
+                const float4 q = ld_cluster_v4(mapa(at, (uint32_t)r));
+                v[0] += q.x, v[1] += q.y, v[2] += q.z, v[3] += q.w;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                v[i] = ops_act(v[i] + bias[i], p.act);
+            store_y4(p, t0 + c, m, v, mtile);
+        }
+    }
+    if (splits > 1)
+        cluster_sync();  // nobody leaves while a peer may still read its partial tile
+}
+
+}  // namespace llk
+
+namespace {
+
+using namespace llk;
+
+bool f8_map(CUtensorMap *m, const void *base, int k, long long rows, long long ld, int box_rows)
+{
+    auto fn = llh::encode_fn();
+    if (!fn)
+        return false;
+    cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)ld};
+    cuuint32_t box[2] = {(cuuint32_t)kF8Block, (cuuint32_t)box_rows};
+    cuuint32_t estr[2] = {1, 1};
+    return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, strides, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int NT>
+int launch_few(const DenseF8Params &p, int splits, int device, cudaStream_t st)
+{
+    static bool ready[kOpsMaxDevices];
+    const void *fn = reinterpret_cast<const void *>(&ll_dense_fp8_kernel<NT>);
+    if (!__atomic_load_n(&ready[device], __ATOMIC_ACQUIRE)) {
+        LL_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, DsSmem<NT>::ALLOC));
+        __atomic_store_n(&ready[device], true, __ATOMIC_RELEASE);
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((p.M + 127) / 128), (unsigned)((p.rows + NT - 1) / NT), (unsigned)splits);
+    cfg.blockDim = dim3(kDsThreads);
+    cfg.dynamicSmemBytes = (size_t)DsSmem<NT>::ALLOC;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = 1;
+    at[0].val.clusterDim.y = 1;
+    at[0].val.clusterDim.z = (unsigned)splits;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    void *args[] = {const_cast<DenseF8Params *>(&p)};
+    LL_CUDA_TRY(cudaLaunchKernelExC(&cfg, fn, args));
+    return LL_OK;
+}
+
+}  // namespace
+
+extern "C" int ll_dense_fp8(const uint8_t *d_W, const float *d_sw, const float *d_b, const uint8_t *d_x,
+                            const float *d_sx, void *d_y, float *d_sy, int y_type, int rows, int M, int K, int64_t ldw,
+                            int64_t ldx, int64_t ldy, int act, void *stream)
+{
+    static const char op[] = "ll_dense_fp8";
+    if (ldw == 0)
+        ldw = K;
+    if (ldx == 0)
+        ldx = K;
+    if (ldy == 0)
+        ldy = M;
+    if (rows < 0 || M < 1 || K < 1 || M > (1 << 24) || K > (1 << 24) || ldw < K || ldx < K || ldy < M ||
+        ldw % 16 != 0 || ldx % 16 != 0 || ldw >= (1ll << 40) || ldx >= (1ll << 40)) {
+        llh::set_error("%s: invalid sizes (rows=%d M=%d K=%d ldw=%lld ldx=%lld ldy=%lld; the rows of W and x start on "
+                       "16 bytes)",
+                       op, rows, M, K, (long long)ldw, (long long)ldx, (long long)ldy);
+        return LL_ERR_INVALID_ARG;
+    }
+    if (act < LL_ACT_IDENTITY || act > LL_ACT_SILU || y_type < LL_T_F32 || y_type > LL_T_F8) {
+        llh::set_error("%s: unknown activation %d or output type %d", op, act, y_type);
+        return LL_ERR_INVALID_ARG;
+    }
+    if (rows > 65535 * 128) {
+        llh::set_error("%s: at most %d rows in one call (rows=%d)", op, 65535 * 128, rows);
+        return LL_ERR_INVALID_ARG;
+    }
+    if (rows == 0)
+        return LL_OK;
+    if (!d_W || !d_sw || !d_x || !d_sx || !d_y || (y_type == LL_T_F8 && !d_sy)) {
+        llh::set_error("%s: null pointer (an e4m3 output needs its scales' address too)", op);
+        return LL_ERR_INVALID_ARG;
+    }
+    int dev = 0;
+    unsigned *status = nullptr;
+    LL_TRY(llh::ops_status_word(&dev, &status));
+    LL_TRY(llh::check_device_ptr(op, "W", d_W, dev, 16));
+    LL_TRY(llh::check_device_ptr(op, "the scales of W", d_sw, dev, 4));
+    LL_TRY(llh::check_device_ptr(op, "x", d_x, dev, 16));
+    LL_TRY(llh::check_device_ptr(op, "the scales of x", d_sx, dev, 4));
+    LL_TRY(llh::check_device_ptr(op, "y", d_y, dev, (size_t)type_bytes(y_type)));
+    if (d_b)
+        LL_TRY(llh::check_device_ptr(op, "b", d_b, dev, 4));
+    if (y_type == LL_T_F8)
+        LL_TRY(llh::check_device_ptr(op, "the scales of y", d_sy, dev, 4));
+
+    DenseF8Params p;
+    p.sw = d_sw;
+    p.sx = d_sx;
+    p.bias = d_b;
+    p.y = d_y;
+    p.sy = d_sy;
+    p.ldy = ldy;
+    p.rows = rows;
+    p.M = M;
+    p.nkb = (K + kF8Block - 1) / kF8Block;
+    p.act = act;
+    p.y_type = y_type;
+    const int v4 = 4 * type_bytes(y_type);  // bytes of four outputs
+    p.y_vec = (ldy % 4 == 0 && (reinterpret_cast<uintptr_t>(d_y) % v4) == 0) ? 1 : 0;
+    p.status = status;
+    p.wait_ns = kOpsWaitNs;
+    const int nt = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+    if (!f8_map(&p.tm_w, d_W, K, M, ldw, 128) || !f8_map(&p.tm_x, d_x, K, rows, ldx, nt)) {
+        llh::set_error("%s: the tensor maps could not be encoded", op);
+        return LL_ERR_CUDA;
+    }
+    // Splits: as many CTAs as SMs, each with two K blocks at least.
+    const long long tiles = (long long)((M + 127) / 128) * ((rows + nt - 1) / nt);
+    int splits = 1;
+    while (splits < 8 && tiles * splits * 2 <= 148 && p.nkb >= splits * 4)
+        splits *= 2;
+    p.kb_split = (p.nkb + splits - 1) / splits;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    switch (nt) {
+    case 16:
+        return launch_few<16>(p, splits, dev, st);
+    case 32:
+        return launch_few<32>(p, splits, dev, st);
+    case 64:
+        return launch_few<64>(p, splits, dev, st);
+    default:
+        return launch_few<128>(p, splits, dev, st);
+    }
+}

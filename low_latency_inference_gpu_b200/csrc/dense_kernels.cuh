@@ -12,6 +12,8 @@ __device__ __forceinline__ float dense_act(float v, int act)
         return v > 0.0f ? v : 0.0f;
     if (act == LL_ACT_GELU)
         return 0.5f * v * (1.0f + erff(v * 0.70710678118654752440f));
+    if (act == LL_ACT_SILU)
+        return v / (1.0f + expf(-v));
     return v;
 }
 

@@ -11,6 +11,28 @@
 
 #include "common.h"
 
+namespace {
+
+// e4m3 nearest to v, ties to even, beyond the largest (448) to the largest; NaN to 0x7f.
+uint8_t e4m3_bits(double v)
+{
+    if (std::isnan(v))
+        return 0x7f;
+    const uint8_t sign = std::signbit(v) ? 0x80 : 0;
+    const double a = std::fmin(std::fabs(v), 448.0);
+    int e = a > 0.0 ? std::ilogb(a) : -6;
+    e = e < -6 ? -6 : e;
+    // 8 steps per octave; below 2^-6 the steps of the lowest octave
+    long n = std::lrint(std::ldexp(a, 3 - e));  // 0 .. 16, ties to even
+    if (n == 16) {
+        n = 8;
+        ++e;
+    }
+    return (uint8_t)(sign | (n < 8 ? (int)n : ((e + 7) << 3) | ((int)n - 8)));
+}
+
+}  // namespace
+
 extern "C" {
 
 int ll_fill_normal(float *out, size_t n, float mean, float stddev, uint32_t seed)
@@ -98,6 +120,26 @@ void ll_quantize_int8_rows(const float *W, int m, int k, int8_t *q, float *s)
             float v = std::rint(row[j] / sc);
             v = std::fmin(127.0f, std::fmax(-127.0f, v));
             q[(size_t)i * k + j] = (int8_t)v;
+        }
+    }
+}
+
+void ll_quantize_fp8_blocks(const float *W, int m, int k, uint8_t *q, float *s)
+{
+    const int kb = (k + LL_F8_BLOCK - 1) / LL_F8_BLOCK;
+    for (int i0 = 0; i0 < m; i0 += LL_F8_BLOCK) {
+        const int i1 = std::min(m, i0 + LL_F8_BLOCK);
+        for (int b = 0; b < kb; ++b) {
+            const int j0 = b * LL_F8_BLOCK, j1 = std::min(k, j0 + LL_F8_BLOCK);
+            float amax = 0.0f;
+            for (int i = i0; i < i1; ++i)
+                for (int j = j0; j < j1; ++j)
+                    amax = std::fmax(amax, std::fabs(W[(size_t)i * k + j]));
+            const float sc = amax > 0.0f ? std::fmax(amax / 448.0f, 0x1p-126f) : 1.0f;
+            s[(size_t)(i0 / LL_F8_BLOCK) * kb + b] = sc;
+            for (int i = i0; i < i1; ++i)
+                for (int j = j0; j < j1; ++j)
+                    q[(size_t)i * k + j] = e4m3_bits((double)W[(size_t)i * k + j] / (double)sc);
         }
     }
 }

@@ -1,0 +1,122 @@
+// Shared by the stateless operators (fp8_quant.cu, dense_fp8.cu, moe.cu): element types,
+// the e4m3 rounding, checks of device pointers, and the device status word.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "common.h"
+
+namespace llk {
+
+constexpr int kF8Block = LL_F8_BLOCK;   // columns (and weight rows) that share one scale
+constexpr float kF8Max = 448.0f;        // largest e4m3 value
+constexpr int kOpsMaxDevices = 64;
+// Bound on every device-side wait of the stateless operators.
+constexpr unsigned long long kOpsWaitNs = 1000ull * 1000 * 1000;
+
+__host__ __device__ constexpr int type_bytes(int t)
+{
+    return t == LL_T_F32 ? 4 : t == LL_T_F8 ? 1 : 2;
+}
+
+__device__ __forceinline__ float ops_act(float v, int act)
+{
+    if (act == LL_ACT_RELU)
+        return v > 0.0f ? v : 0.0f;
+    if (act == LL_ACT_GELU)
+        return 0.5f * v * (1.0f + erff(v * 0.70710678118654752440f));
+    if (act == LL_ACT_SILU)
+        return v / (1.0f + expf(-v));
+    return v;
+}
+
+// ---- e4m3 ----
+
+// Two fp32 values to e4m3 (nearest, ties to even, beyond the largest to the largest), lo in bits 0..7.
+__device__ __forceinline__ uint32_t f32x2_to_e4m3(float lo, float hi)
+{
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+// e4m3 nearest to the exact quotient v / s (two of them).  The quotient of two 24-bit
+// significands that is not itself on the border of two e4m3 values (5 significant bits) is
+// at least 2^-30 (relative) away from it, so the 53-bit quotient lies on the right side;
+// rounding it to odd in fp32 keeps that side for the final rounding.
+static __device__ __noinline__ uint32_t quot_e4m3_exact(float v0, float v1, float s)
+{
+    float f[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const double d = (double)(i ? v1 : v0) / (double)s;
+        f[i] = __double2float_rz(d);
+        if ((double)f[i] != d && f[i] == f[i])
+            f[i] = __uint_as_float(__float_as_uint(f[i]) | 1u);
+    }
+    return f32x2_to_e4m3(f[0], f[1]);
+}
+
+// e4m3 of v0 / s and v1 / s given inv = 1 / s rounded.  v * inv is within 2^-23 (relative) of
+// the quotient; where both ends of an interval of +-2^-22 round to one e4m3 value that is the
+// answer, and else (about one pair in 2^17, or a tie) the exact quotient decides.
+__device__ __forceinline__ uint32_t quot_e4m3(float v0, float v1, float s, float inv)
+{
+    const float t0 = v0 * inv, t1 = v1 * inv;
+    constexpr float kUp = 1.0f + 0x1p-22f, kDown = 1.0f - 0x1p-22f;
+    const uint32_t a = f32x2_to_e4m3(t0 * kUp, t1 * kUp);
+    const uint32_t b = f32x2_to_e4m3(t0 * kDown, t1 * kDown);
+    return a == b ? a : quot_e4m3_exact(v0, v1, s);
+}
+
+// The scale of a group whose largest magnitude is amax: amax / 448, or the next power of two at
+// or above it; at least 2^-126 so that its reciprocal is finite; 0 for an all-zero group.
+__device__ __forceinline__ void e4m3_scale(float amax, bool pow2, float &s, float &inv)
+{
+    if (!(amax > 0.0f)) {
+        s = 0.0f;
+        inv = 0.0f;
+        return;
+    }
+    const float q = fmaxf(__fdiv_rn(amax, kF8Max), 0x1p-126f);
+    if (pow2) {
+        const uint32_t u = __float_as_uint(q);
+        const uint32_t e = (u >> 23) + ((u & 0x7fffffu) != 0u);
+        s = __uint_as_float(e << 23);
+        inv = e >= 254u ? 0.0f : __uint_as_float((254u - e) << 23);
+    } else {
+        s = q;
+        inv = __frcp_rn(q);
+    }
+}
+
+// Four fp32 values of one group as four e4m3 bytes.
+__device__ __forceinline__ uint32_t group_e4m3x4(const float *v, bool pow2, float s, float inv)
+{
+    if (pow2 || s == 0.0f)  // the product is the quotient (a power of two; zeros and NaN)
+        return f32x2_to_e4m3(v[0] * inv, v[1] * inv) | (f32x2_to_e4m3(v[2] * inv, v[3] * inv) << 16);
+    return quot_e4m3(v[0], v[1], s, inv) | (quot_e4m3(v[2], v[3], s, inv) << 16);
+}
+
+}  // namespace llk
+
+namespace llh {
+
+// Device word that a stateless operator's kernel sets when a bounded wait runs out (one per GPU,
+// read and cleared by ll_ops_check).  Looked up once per device.
+int ops_status_word(int *device, unsigned **word);
+
+// LL_OK when p is memory of the current device (managed memory included), aligned to `align` bytes.
+int check_device_ptr(const char *op, const char *what, const void *p, int device, size_t align);
+
+}  // namespace llh
+
+#define LL_TRY(call)         \
+    do {                     \
+        int _rc = (call);    \
+        if (_rc != LL_OK)    \
+            return _rc;      \
+    } while (0)
