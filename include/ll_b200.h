@@ -463,6 +463,52 @@ int ll_dense_fp8(const uint8_t *d_W, const float *d_sw, const float *d_b, const 
  * outputs of the calls since then are not to be used; the word is cleared). */
 int ll_ops_check(void *stream);
 
+/*
+ * Mixture-of-experts layer for a few rows, in two kernels (no counterpart in the reference, whose
+ * net is one dense chain):
+ *   logits = Wr x; the top_k experts of a row by logit (a tie goes to the lower index), with weights
+ *   softmax(logits) of all experts at the picked ones, divided by their sum when renormalize = 1;
+ *   y = sum over the picked experts of weight * Wd (act(Wg x) * (Wu x))      (gated = 1)
+ *                                     weight * Wd act(Wg x)                 (gated = 0).
+ * Matrices are row-major on the device, expert after expert: router [n_experts x hidden] (bf16 or
+ * fp32), gate and up [n_experts][inter x hidden], down [n_experts][hidden x inter], in wtype:
+ * LL_W_BF16; LL_W_I8 with scales per output channel (gate_scale / up_scale [n_experts][inter],
+ * down_scale [n_experts][hidden], as ll_quantize_int8_rows makes them); LL_W_F8 with scales per
+ * 128 x 128 block of each expert's matrix (as ll_quantize_fp8_blocks makes them).  x and y are
+ * [rows x hidden] in x_type (fp32, bf16, fp16), row strides ldx / ldy elements (0 = hidden);
+ * rows <= LL_MOE_MAX_ROWS, 0 does nothing.  All sums are fp32; the weights are used exactly, x exactly,
+ * the activations with 16 bits or more (24 when x is fp32).  d_ids / d_probs [rows][top_k]
+ * (NULL to skip) receive the picked experts, largest logit first, and their weights.  A NaN logit
+ * ranks below every number.
+ * d_work: work_bytes >= ll_moe_workspace_bytes(desc, rows), 256-byte aligned device memory that no
+ * other call may use at the same time (calls one after another on a stream may share it); it needs
+ * no initialisation.  Keeps nothing, allocates nothing, can be captured; as for ll_dense_fp8 every
+ * pointer names memory of the current device, and the first call per device and description comes
+ * before any capture.  Results repeat bit for bit.  ll_ops_check reports a device-side failure.
+ */
+#define LL_MOE_MAX_ROWS 32
+#define LL_MOE_MAX_EXPERTS 256
+#define LL_MOE_MAX_TOPK 16
+#define LL_MOE_MAX_DIM 65536
+typedef struct ll_moe_desc {
+    int32_t hidden, inter, n_experts, top_k;
+    int32_t act;         /* LL_ACT_* */
+    int32_t gated;       /* 1 = act(gate) * up */
+    int32_t wtype;       /* LL_W_BF16, LL_W_I8 or LL_W_F8 */
+    int32_t x_type;      /* LL_T_F32, LL_T_BF16 or LL_T_F16 */
+    int32_t router_type; /* LL_T_F32 or LL_T_BF16 */
+    int32_t renormalize; /* 1 = the picked experts' weights add up to 1 */
+    int32_t reserved[2];
+} ll_moe_desc;
+typedef struct ll_moe_weights { /* device pointers */
+    const void *router, *gate, *up, *down;               /* up: NULL when not gated */
+    const float *gate_scale, *up_scale, *down_scale;     /* NULL for bf16 */
+} ll_moe_weights;
+int ll_moe_workspace_bytes(const ll_moe_desc *desc, int rows, size_t *bytes);
+int ll_moe_forward(const ll_moe_desc *desc, const ll_moe_weights *w, const void *d_x, int64_t ldx, void *d_y,
+                   int64_t ldy, int rows, int32_t *d_ids, float *d_probs, void *d_work, size_t work_bytes,
+                   void *stream);
+
 /* Host packing, include/ll/pack_weights.cuh:16-32. */
 void ll_pack_rm_to_kmajor_padded(const float *W_rm, size_t M, size_t K, float *W_cm, size_t Mpad);
 void ll_pack_bias_padded(const float *b, size_t M, float *b_pad, size_t Mpad);

@@ -61,6 +61,7 @@ EXPORTED_SYMBOLS = [
     "ll_weights_save", "ll_weights_load", "ll_weights_net", "ll_weights_arrays", "ll_weights_free",
     "ll_submit_many", "ll_engine_bench_ring", "ll_engine_bench_ring_mt",
     "ll_quantize_fp8", "ll_quantize_fp8_blocks", "ll_dense_fp8", "ll_ops_check",
+    "ll_moe_workspace_bytes", "ll_moe_forward",
 ]
 MAX_LAYERS = 24
 
@@ -139,6 +140,17 @@ class BatchedInfo(ctypes.Structure):
     _fields_ = [("n_layers", ctypes.c_int32), ("rows_pad", ctypes.c_int32), ("bn", ctypes.c_int32 * 24),
                 ("splits", ctypes.c_int32 * 24), ("ctas", ctypes.c_int32 * 24), ("smem_bytes", ctypes.c_int32 * 24),
                 ("kind", ctypes.c_int32 * 24)]
+
+
+class MoEDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("hidden", "inter", "n_experts", "top_k", "act", "gated", "wtype",
+                                               "x_type", "router_type", "renormalize")] + \
+               [("reserved", ctypes.c_int32 * 2)]
+
+
+class MoEWeightsStruct(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("router", "gate", "up", "down", "gate_scale", "up_scale",
+                                                "down_scale")]
 
 
 LAYER_MODE_NAMES = {0: "replicated", 1: "rowsplit_allgather", 2: "rowsplit_local", 3: "ksplit_gather",
@@ -232,6 +244,9 @@ def _sig(lib):
                                         ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int,
                                         _vp]),
         "ll_ops_check": (ctypes.c_int, [_vp]),
+        "ll_moe_workspace_bytes": (ctypes.c_int, [P(MoEDesc), ctypes.c_int, P(ctypes.c_size_t)]),
+        "ll_moe_forward": (ctypes.c_int, [P(MoEDesc), P(MoEWeightsStruct), _vp, ctypes.c_int64, _vp, ctypes.c_int64,
+                                          ctypes.c_int, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
     }
     for name, (res, args) in s.items():
         f = getattr(lib, name)
@@ -675,6 +690,60 @@ def dense_fp8(W_ptr: int, sw_ptr: int, b_ptr: int, x_ptr: int, sx_ptr: int, y_pt
 def ops_check(stream: int = 0):
     """Raise if a device-side wait of dense_fp8 or moe_forward ran out since the last check (ll_ops_check)."""
     _check(lib().ll_ops_check(stream or None))
+
+
+# ---- mixture-of-experts layer ----
+MOE_MAX_ROWS, MOE_MAX_EXPERTS, MOE_MAX_TOPK, MOE_MAX_DIM = 32, 256, 16, 65536
+
+
+@dataclass
+class MoE:
+    """Description of a mixture-of-experts layer (ll_moe_desc)."""
+    hidden: int
+    inter: int
+    n_experts: int
+    top_k: int
+    act: int = ACT_SILU
+    gated: bool = True
+    wtype: int = W_BF16
+    x_type: int = T_BF16
+    router_type: int = T_BF16
+    renormalize: bool = True
+
+    def desc(self) -> MoEDesc:
+        return MoEDesc(self.hidden, self.inter, self.n_experts, self.top_k, self.act, int(self.gated), self.wtype,
+                       self.x_type, self.router_type, int(self.renormalize))
+
+
+@dataclass
+class MoEWeights:
+    """Device pointers of a layer's matrices and scales (ll_moe_weights); 0 where there is none."""
+    router: int
+    gate: int
+    up: int
+    down: int
+    gate_scale: int = 0
+    up_scale: int = 0
+    down_scale: int = 0
+
+    def struct(self) -> MoEWeightsStruct:
+        return MoEWeightsStruct(self.router or None, self.gate or None, self.up or None, self.down or None,
+                                self.gate_scale or None, self.up_scale or None, self.down_scale or None)
+
+
+def moe_workspace_bytes(moe: MoE, rows: int) -> int:
+    """Bytes of device memory that moe_forward needs beside its operands for up to `rows` rows."""
+    n = ctypes.c_size_t()
+    _check(lib().ll_moe_workspace_bytes(ctypes.byref(moe.desc()), rows, ctypes.byref(n)))
+    return n.value
+
+
+def moe_forward(moe: MoE, weights: MoEWeights, x_ptr: int, y_ptr: int, rows: int, work_ptr: int, work_bytes: int,
+                ids_ptr: int = 0, probs_ptr: int = 0, ldx: int = 0, ldy: int = 0, stream: int = 0):
+    """One mixture-of-experts layer for up to MOE_MAX_ROWS rows (ll_moe_forward), device pointers."""
+    _check(lib().ll_moe_forward(ctypes.byref(moe.desc()), ctypes.byref(weights.struct()), x_ptr or None, ldx,
+                                y_ptr or None, ldy, rows, ids_ptr or None, probs_ptr or None, work_ptr or None,
+                                work_bytes, stream or None))
 
 
 def plan_net(net: Net, W=None, b=None, scales=None, opts: Optional[EngineOpts] = None, want_images: bool = False):

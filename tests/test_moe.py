@@ -1,0 +1,323 @@
+"""ll_moe_forward, a mixture-of-experts layer for a few rows, against numpy in 64 bits (B200).
+
+Tolerances, per output, from the sums of magnitudes (A_v = sum |a| |b| of each product v):
+  * every weight and every bf16 term of x is exact in the tensor instruction, whose fp32 sums are
+    off by at most 2^-23 of a partial sum (<= A) per addition; a product over K columns makes
+    NS K additions (NS = 1, 2, 3 bf16 terms for bf16, fp16, fp32 x) and at most 40 more (warps,
+    blocks' scales, splits): |v - exact| <= A (NS K + 40) 2^-23.
+  * the router (bf16 or 3 terms, so NS is 3 NS): logits off by t_l; a softmax weight is off by a
+    factor within exp(+-2 t_l), and 2^-19 for exp and the sum of up to 256 terms.
+  * act has slope <= 1.13 and is evaluated to 2^-20 of |v|; the product with up adds 2^-23; the
+    activation is kept with 16 bits (2^-16) for 16-bit x, 23 (2^-22) for fp32.
+  * the result is rounded by half a step: 2^-8 bf16, 2^-11 fp16.
+The picked experts must be a top_k up to t_l: any expert left out has a logit at most 2 t_l above
+one that was picked; the reference continues with the device's choice.
+"""
+import numpy as np
+import pytest
+
+import low_latency_inference_gpu_b200 as ll
+from test_fp8 import F8, act64, decode, dequant_blocks, dequant_rows, dev, quantize_rows, t_dtype, up
+
+U = 2.0 ** -23
+ROUND = {ll.T_F32: 2.0 ** -23, ll.T_BF16: 2.0 ** -8, ll.T_F16: 2.0 ** -11}
+
+
+def desc(**kw):
+    d = dict(hidden=64, inter=32, n_experts=4, top_k=2)
+    d.update(kw)
+    return ll.MoE(**d)
+
+
+# ---------------------------------------------------------------- refusals (host)
+def refused(fn, code, *a, **kw):
+    with pytest.raises(ll.LLError) as e:
+        fn(*a, **kw)
+    assert e.value.code == code
+    return str(e.value)
+
+
+@pytest.mark.parametrize("bad", [
+    dict(hidden=0), dict(inter=0), dict(hidden=65537), dict(n_experts=0), dict(n_experts=257), dict(top_k=0),
+    dict(top_k=5), dict(n_experts=64, top_k=17), dict(act=4), dict(act=-1), dict(wtype=ll.W_F32), dict(wtype=4),
+    dict(x_type=ll.T_F8), dict(router_type=ll.T_F16), dict(router_type=ll.T_F8)])
+def test_refuses_descriptions(bad):
+    refused(ll.moe_workspace_bytes, ll.LL_ERR_BAD_DESC, desc(**bad), 1)
+    w = ll.MoEWeights(16, 16, 16, 16, 16, 16, 16)
+    refused(ll.moe_forward, ll.LL_ERR_BAD_DESC, desc(**bad), w, 16, 16, 1, 256, 1 << 20)
+
+
+def test_refuses_arguments():
+    m, big = desc(), 1 << 20
+    w = ll.MoEWeights(16, 16, 16, 16)
+    bad = ll.LL_ERR_INVALID_ARG
+    for rows in (-1, ll.MOE_MAX_ROWS + 1):
+        refused(ll.moe_workspace_bytes, bad, m, rows)
+        refused(ll.moe_forward, bad, m, w, 16, 16, rows, 256, big)
+    refused(ll.moe_forward, bad, m, w, 0, 16, 1, 256, big)
+    refused(ll.moe_forward, bad, m, w, 16, 0, 1, 256, big)
+    refused(ll.moe_forward, bad, m, w, 16, 16, 1, 0, big)
+    refused(ll.moe_forward, bad, m, w, 16, 16, 1, 256, big, ldx=63)
+    refused(ll.moe_forward, bad, m, w, 16, 16, 1, 256, big, ldy=63)
+    assert "workspace" in refused(ll.moe_forward, bad, m, w, 16, 16, 1, 256, ll.moe_workspace_bytes(m, 1) - 1)
+    for name in ("router", "gate", "up", "down"):
+        refused(ll.moe_forward, bad, m, ll.MoEWeights(**{**w.__dict__, name: 0}), 16, 16, 1, 256, big)
+    for t in (ll.W_I8, ll.W_F8):
+        refused(ll.moe_forward, bad, desc(wtype=t), w, 16, 16, 1, 256, big)
+    ll.moe_forward(m, w, 0, 0, 0, 0, 0)  # no rows: nothing to do
+
+
+def test_workspace_grows_with_rows_and_covers_every_pair():
+    for x_type, planes in ((ll.T_BF16, 2), (ll.T_F16, 2), (ll.T_F32, 3)):
+        m = desc(inter=333, top_k=3, x_type=x_type)
+        sizes = [ll.moe_workspace_bytes(m, r) for r in range(ll.MOE_MAX_ROWS + 1)]
+        assert all(a <= b for a, b in zip(sizes, sizes[1:]))
+        assert sizes[-1] >= 32 * 3 * (333 * 2 * planes + 8)
+
+
+# ---------------------------------------------------------------- device
+class Layer:
+    def __init__(self, m: ll.MoE, rows, seed=1, router_scale=2.0, pad_x=0, pad_y=0, shift=0):
+        import torch
+
+        self.m, self.rows, self.torch = m, rows, torch
+        e, h, f = m.n_experts, m.hidden, m.inter
+        self.ldx, self.ldy = h + pad_x, h + pad_y
+        x = ll.fill_normal(rows * h, 0.0, 1.0, seed).reshape(rows, h)
+        xb = torch.full((shift + rows * self.ldx,), 5.0, device="cuda", dtype=t_dtype(m.x_type))
+        self.xv = xb[shift:].view(rows, self.ldx)
+        self.xv[:, :h] = dev(x).to(t_dtype(m.x_type))
+        self.x = self.xv[:, :h].double().cpu().numpy()
+        r = ll.fill_normal(e * h, 0.0, router_scale * h ** -0.5, seed + 1).reshape(e, h)
+        self.d = {"router": dev(r).to(t_dtype(m.router_type))}
+        self.r = self.d["router"].double().cpu().numpy()
+        self.w = {}
+        for i, (name, a, b) in enumerate((("gate", f, h), ("up", f, h), ("down", h, f))):
+            if name == "up" and not m.gated:
+                continue
+            mats = [ll.fill_normal(a * b, 0.0, b ** -0.5, seed + 10 + 3 * j + i).reshape(a, b) for j in range(e)]
+            if m.wtype == ll.W_BF16:
+                t = dev(np.stack(mats)).to(torch.bfloat16)
+                self.d[name], self.w[name] = t, t.double().cpu().numpy()
+            elif m.wtype == ll.W_I8:
+                q, s = zip(*[ll.quantize_int8_rows(v) for v in mats])
+                self.d[name], self.d[name + "_scale"] = dev(np.stack(q)), dev(np.stack(s))
+                self.w[name] = np.stack(q).astype(np.float64) * np.stack(s).astype(np.float64)[:, :, None]
+            else:
+                q, s = zip(*[ll.quantize_fp8_blocks(v) for v in mats])
+                self.d[name], self.d[name + "_scale"] = dev(np.stack(q)), dev(np.stack(s))
+                self.w[name] = np.stack([dequant_blocks(*v) for v in zip(q, s)])
+        self.weights = ll.MoEWeights(**{n: self.d[n].data_ptr() if n in self.d else 0
+                                        for n in ("router", "gate", "up", "down", "gate_scale", "up_scale",
+                                                  "down_scale")})
+        self.buffers()
+
+    def buffers(self):
+        t = self.torch
+        n = ll.moe_workspace_bytes(self.m, self.rows)
+        self.work = t.full((n,), 0xFF, dtype=t.uint8, device="cuda")  # NaN wherever it is read unwritten
+        self.y = t.full((self.rows + 1, self.ldy), 99.0, device="cuda", dtype=t_dtype(self.m.x_type))
+        self.ids = t.full((self.rows, self.m.top_k), -1, dtype=t.int32, device="cuda")
+        self.probs = t.full((self.rows, self.m.top_k), -1.0, device="cuda")
+
+    def run(self, stream=None):
+        st = (stream or self.torch.cuda.current_stream()).cuda_stream
+        ll.moe_forward(self.m, self.weights, self.xv.data_ptr(), self.y.data_ptr(), self.rows, self.work.data_ptr(),
+                       self.work.numel(), ids_ptr=self.ids.data_ptr(), probs_ptr=self.probs.data_ptr(), ldx=self.ldx,
+                       ldy=self.ldy, stream=st)
+
+    def check(self):
+        m, x = self.m, self.x
+        ns = {ll.T_BF16: 1, ll.T_F16: 2, ll.T_F32: 3}[m.x_type]
+        ids, probs = self.ids.cpu().numpy(), self.probs.double().cpu().numpy()
+        h, f, k = m.hidden, m.inter, m.top_k
+        got = self.y.double().cpu().numpy()
+        assert np.all(got[self.rows:] == 99) and np.all(got[:, h:] == 99)
+        logits = x @ self.r.T
+        tl = (np.abs(x) @ np.abs(self.r).T) * (3 * ns * h + 40) * U
+        for i in range(self.rows):
+            order = ids[i]
+            assert len(set(order)) == k and order.min() >= 0 and order.max() < m.n_experts
+            t = 2 * tl[i].max()
+            l = logits[i]
+            rest = np.delete(l, order)
+            assert np.all(np.diff(l[order]) <= t) and (rest.size == 0 or rest.max() <= l[order].min() + t)
+            p = np.exp(l - l.max())
+            p /= p.sum()
+            w = p[order] / (p[order].sum() if m.renormalize else 1.0)
+            assert np.all(np.abs(probs[i] - w) <= w * (np.expm1(2 * t) + 2.0 ** -19))
+            y, tol = np.zeros(h), np.zeros(h)
+            for j, e in enumerate(order):
+                g = x[i] @ self.w["gate"][e].T
+                tg = (np.abs(x[i]) @ np.abs(self.w["gate"][e]).T) * (ns * h + 40) * U
+                a = act64(g, m.act)
+                ta = 1.13 * tg + 2.0 ** -20 * np.abs(g)
+                if m.gated:
+                    u = x[i] @ self.w["up"][e].T
+                    tu = (np.abs(x[i]) @ np.abs(self.w["up"][e]).T) * (ns * h + 40) * U
+                    ta = ta * (np.abs(u) + tu) + np.abs(a) * tu
+                    a = a * u
+                    ta = ta + np.abs(a) * U
+                ta = ta + np.abs(a) * (2.0 ** -22 if m.x_type == ll.T_F32 else 2.0 ** -16)
+                d = np.abs(self.w["down"][e])
+                nsh = 3 if m.x_type == ll.T_F32 else 2
+                y += w[j] * (self.w["down"][e] @ a)
+                tol += w[j] * (d @ ta + (d @ (np.abs(a) + ta)) * ((nsh * f + 40) * U + np.expm1(2 * t) + 2.0 ** -19))
+            tol = tol * 1.01 + np.abs(y) * ROUND[m.x_type] + 2.0 ** -25
+            worst = np.max(np.abs(got[i, :h] - y) - tol)
+            assert worst <= 0, (i, worst)
+
+
+CASES = [
+    # rows, hidden, inter, experts, top_k, gated, renorm, act, router_type, pads
+    (1, 64, 64, 1, 1, True, True, ll.ACT_SILU, ll.T_BF16, 0),
+    (1, 256, 128, 8, 2, True, True, ll.ACT_SILU, ll.T_BF16, 0),
+    (1, 2048, 512, 16, 8, True, False, ll.ACT_SILU, ll.T_F32, 0),
+    (2, 100, 36, 5, 3, False, False, ll.ACT_GELU, ll.T_BF16, 4),
+    (3, 129, 65, 7, 7, True, True, ll.ACT_RELU, ll.T_F32, 1),
+    (7, 1000, 344, 10, 3, False, True, ll.ACT_GELU, ll.T_BF16, 0),
+    (8, 640, 1032, 20, 4, True, True, ll.ACT_SILU, ll.T_BF16, 8),
+    (9, 512, 256, 2, 1, True, True, ll.ACT_IDENTITY, ll.T_BF16, 0),
+    (16, 257, 129, 33, 16, False, False, ll.ACT_SILU, ll.T_BF16, 3),
+    (32, 384, 200, 40, 8, True, True, ll.ACT_SILU, ll.T_F32, 0),
+    (32, 64, 16, 256, 2, True, True, ll.ACT_SILU, ll.T_BF16, 0),
+    (31, 1040, 528, 3, 3, True, True, ll.ACT_GELU, ll.T_BF16, 0),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.timeout(300)
+@pytest.mark.parametrize("wtype", [ll.W_BF16, ll.W_I8, ll.W_F8])
+@pytest.mark.parametrize("x_type", [ll.T_BF16, ll.T_F16, ll.T_F32])
+@pytest.mark.parametrize("case", range(len(CASES)))
+def test_moe(wtype, x_type, case):
+    rows, h, f, e, k, gated, renorm, act, rt, pad = CASES[case]
+    m = ll.MoE(h, f, e, k, act, gated, wtype, x_type, rt, renorm)
+    layer = Layer(m, rows, seed=case + 1, pad_x=pad, pad_y=2 * pad, shift=pad % 2)
+    layer.run()
+    ll.ops_check()
+    layer.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.timeout(300)
+def test_ties_go_to_the_lower_index():
+    m = ll.MoE(128, 64, 12, 5)
+    layer = Layer(m, 4)
+    layer.d["router"][:] = layer.d["router"][0]
+    layer.d["router"][9] += layer.d["router"][0]  # twice the others' logit: first or last
+    layer.run()
+    ids = layer.ids.cpu().numpy()
+    l = layer.x @ layer.r[0]
+    for i in range(4):
+        assert ids[i].tolist() == ([9, 0, 1, 2, 3] if l[i] > 0 else [0, 1, 2, 3, 4])
+    assert np.all(np.isfinite(layer.y.float().cpu().numpy()))
+
+
+@pytest.mark.gpu
+@pytest.mark.timeout(300)
+@pytest.mark.parametrize("wtype", [ll.W_BF16, ll.W_F8])
+def test_special_values_stay_in_their_rows(wtype):
+    m = ll.MoE(256, 128, 8, 2, wtype=wtype)
+    clean, layer = Layer(m, 6), Layer(m, 6)
+    clean.run()
+    layer.xv[2, 7] = float("nan")
+    layer.xv[4, 9] = float("inf")
+    layer.run()
+    ll.ops_check()
+    y, want = layer.y.float().cpu().numpy()[:6], clean.y.float().cpu().numpy()[:6]
+    assert np.isnan(y[2]).all() and not np.isfinite(y[4]).any()
+    keep = [0, 1, 3, 5]
+    assert np.array_equal(y[keep], want[keep])  # and the others do not move by a bit
+    ids = layer.ids.cpu().numpy()
+    assert ids.min() >= 0 and ids.max() < 8 and all(len(set(r)) == 2 for r in ids)
+
+
+@pytest.mark.gpu
+@pytest.mark.timeout(300)
+@pytest.mark.parametrize("rows", [1, 20])
+def test_repeats_bit_for_bit_on_streams_and_in_graphs(rows):
+    import torch
+
+    m = ll.MoE(512, 320, 16, 4, wtype=ll.W_F8)
+    a, b = Layer(m, rows, seed=2), Layer(m, rows, seed=50)
+    a.run(), b.run()
+    torch.cuda.synchronize()
+    ya, yb = a.y.clone(), b.y.clone()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(10):  # two calls at once, each with its own workspace
+        a.run(s1), b.run(s2)
+    torch.cuda.synchronize()
+    assert torch.equal(a.y, ya) and torch.equal(b.y, yb)
+    for _ in range(10):  # one after another through one workspace
+        b.work = a.work
+        a.run(), b.run()
+    assert torch.equal(a.y, ya) and torch.equal(b.y, yb)
+    b.buffers()
+    ga, gb = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(ga):
+        a.run()
+    with torch.cuda.graph(gb):
+        b.run()
+        b.run()
+    for _ in range(5):
+        a.y.zero_(), b.y.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s1):
+            ga.replay()
+        with torch.cuda.stream(s2):
+            gb.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(a.y[:rows], ya[:rows]) and torch.equal(b.y[:rows], yb[:rows])
+    a.xv.copy_(b.xv)  # a replay reads x anew: other experts
+    ga.replay()
+    torch.cuda.synchronize()
+    a.x = b.x
+    a.y[rows:] = 99
+    a.check()
+    ll.ops_check()
+
+
+@pytest.mark.gpu
+@pytest.mark.timeout(300)
+def test_refuses_memory_of_the_host():
+    import torch
+
+    layer = Layer(ll.MoE(64, 32, 4, 2), 2)
+    host = torch.zeros(2, 64, dtype=torch.bfloat16)
+    a = (layer.m, layer.weights, layer.xv.data_ptr(), layer.y.data_ptr(), 2, layer.work.data_ptr(), layer.work.numel())
+    for i in (2, 3, 5):
+        args = list(a)
+        args[i] = host.data_ptr() // 256 * 256
+        assert "current device" in refused(ll.moe_forward, ll.LL_ERR_INVALID_ARG, *args)
+    args = list(a)
+    args[5] += 16
+    assert "aligned" in refused(ll.moe_forward, ll.LL_ERR_INVALID_ARG, *args)
+
+
+@pytest.mark.gpu
+@pytest.mark.timeout(300)
+@pytest.mark.parametrize("rows", [1, 6, 32])
+def test_a_layer_of_experts_and_an_output_layer(rows):
+    """moe (e4m3 experts) -> quantise -> dense (e4m3): each step against 64 bits on the device's own input."""
+    import torch
+
+    m = ll.MoE(384, 256, 12, 3, wtype=ll.W_F8, x_type=ll.T_BF16)
+    layer = Layer(m, rows, seed=5)
+    W = ll.fill_normal(96 * 384, 0.0, 384 ** -0.5, 77).reshape(96, 384)
+    wq, sw = ll.quantize_fp8_blocks(W)
+    dw, dsw = dev(wq), dev(sw)
+    q = torch.zeros(rows, 384, dtype=torch.uint8, device="cuda")
+    s = torch.zeros(rows, 3, device="cuda")
+    out = torch.zeros(rows, 96, device="cuda")
+    st = torch.cuda.current_stream().cuda_stream
+    layer.run()
+    ll.quantize_fp8(layer.y.data_ptr(), ll.T_BF16, rows, 384, q.data_ptr(), s.data_ptr(), ldx=layer.ldy, stream=st)
+    ll.dense_fp8(dw.data_ptr(), dsw.data_ptr(), 0, q.data_ptr(), s.data_ptr(), out.data_ptr(), rows, 96, 384, stream=st)
+    ll.ops_check(st)
+    layer.check()
+    qn, sn = quantize_rows(layer.y[:rows].float().cpu().numpy())
+    assert np.array_equal(decode(q.cpu().numpy()), decode(qn)) and np.array_equal(s.cpu().numpy(), sn)
+    x, w = dequant_rows(qn, sn), dequant_blocks(wq, sw)
+    tol = (np.abs(x) @ np.abs(w).T) * (128 + 3 + 11) * U
+    assert np.all(np.abs(out.cpu().numpy() - x @ w.T) <= tol)
