@@ -262,7 +262,7 @@ __global__ void __launch_bounds__(kDsThreads, 1) ll_dense_fp8_kernel(const __gri
                 __syncwarp();
             }
             const int b = j & 1;
-            if (!tc_wait_warp(b_accf(b), (j / 2) & 1, p.wait_ns, fail, p.status, 4))
+            if (!ops_wait_warp(b_accf(b), (j / 2) & 1, p.wait_ns, fail, p.status, 4))
                 break;
             tc_fence_after();
             const float *sc = w_sc + (j % kDsScaleKb) * NT;
@@ -285,7 +285,7 @@ __global__ void __launch_bounds__(kDsThreads, 1) ll_dense_fp8_kernel(const __gri
                 mbar_arrive_local(b_acce(b));
         }
         // every MMA has read the ring before the partial tile overwrites it
-        tc_wait_warp(b_done, 0, p.wait_ns, fail, p.status, 5);
+        ops_wait_warp(b_done, 0, p.wait_ns, fail, p.status, 5);
 #pragma unroll
         for (int c = 0; c < NT; ++c)
             s_part[c * L::PART_LD + chan] = acc[c];

@@ -53,7 +53,7 @@ WorkLayout work_layout(const ll_moe_desc *d, int rows)
     const size_t n = (size_t)rows * d->top_k;
     w.probs = llh::round_up(4 * n, 256);
     w.hid = w.probs + llh::round_up(4 * n, 256);
-    w.ld = (int)llh::round_up((size_t)d->inter, 16);
+    w.ld = moe_cols(d->inter, d->wtype == LL_W_BF16 ? 2 : 1);
     w.plane = (long long)(n * (size_t)w.ld);
     w.bytes = w.hid + (size_t)w.plane * 2 * (d->x_type == LL_T_F32 ? 3 : 2);
     return w;
@@ -104,8 +104,11 @@ int ll_moe_forward(const ll_moe_desc *d, const ll_moe_weights *w, const void *d_
         return LL_ERR_INVALID_ARG;
     }
     int dev = 0;
-    unsigned *status = nullptr;
-    LL_TRY(llh::ops_status_word(&dev, &status));
+    LL_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= kOpsMaxDevices) {
+        llh::set_error("%s: device index %d out of range", op, dev);
+        return LL_ERR_INVALID_ARG;
+    }
     const size_t xa = (size_t)type_bytes(d->x_type), wa = d->wtype == LL_W_BF16 ? 2 : 1;
     LL_TRY(llh::check_device_ptr(op, "x", d_x, dev, xa));
     LL_TRY(llh::check_device_ptr(op, "y", d_y, dev, xa));
@@ -153,8 +156,11 @@ int ll_moe_forward(const ll_moe_desc *d, const ll_moe_weights *w, const void *d_
     p.sg = w->gate_scale;
     p.su = w->up_scale;
     p.sd = w->down_scale;
-    p.up_ring = on16(p.wg, (long long)d->hidden * (long long)wa) && (!d->gated || on16(p.wu, 0));
-    p.down_ring = on16(p.wd, (long long)d->inter * (long long)wa);
+    // The widest copy that every weight row allows.
+    auto grain = [](uintptr_t bits) { return (int)std::min<uintptr_t>(16, bits & (~bits + 1)); };
+    p.up_grain = grain(reinterpret_cast<uintptr_t>(p.wg) | (d->gated ? reinterpret_cast<uintptr_t>(p.wu) : 0) |
+                       (uintptr_t)d->hidden * wa);
+    p.down_grain = grain(reinterpret_cast<uintptr_t>(p.wd) | (uintptr_t)d->inter * wa);
     uint8_t *work = static_cast<uint8_t *>(d_work);
     p.ids = reinterpret_cast<int *>(work);
     p.probs = reinterpret_cast<float *>(work + wl.probs);
@@ -163,8 +169,6 @@ int ll_moe_forward(const ll_moe_desc *d, const ll_moe_weights *w, const void *d_
     p.hid_ld = wl.ld;
     p.user_ids = d_ids;
     p.user_probs = d_probs;
-    p.status = status;
-    p.wait_ns = kOpsWaitNs;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     return d->wtype == LL_W_BF16 ? launch_moe_bf16(p, dev, st)
            : d->wtype == LL_W_I8 ? launch_moe_i8(p, dev, st)

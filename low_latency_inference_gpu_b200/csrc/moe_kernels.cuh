@@ -6,19 +6,23 @@
 //   y_r     = sum_j w[r, j] Wd_e a[r, j]
 //
 // With few rows the layer reads the picked experts' weights once and does little else, so both
-// kernels stream weight rows from memory through a ring in shared memory (bulk copies, 1 KB of
-// each of 16 rows per stage; one warp copies, eight compute) and multiply them on the warp-level
-// bf16 tensor instruction with 16 weight rows as M and 8 of the expert's rows of x as N.  A
-// tcgen05 tile (M = 128) would need each expert's rows padded to a full tile and int8 / e4m3
-// weights widened in tensor memory; at these widths the memory is the bound and the warp-level
-// instruction is at a few per cent of its rate.
+// kernels stream weight rows from memory and multiply them on the warp-level bf16 tensor
+// instruction with 16 weight rows as M and 8 of the expert's rows of x as N.  A tcgen05 tile
+// (M = 128) would need each expert's rows padded to a full tile and int8 / e4m3 weights widened in
+// tensor memory; at these widths the memory is the bound and the warp-level instruction is at a
+// few per cent of its rate.
+// Every warp works alone: it takes whole tiles (up to 16 weight rows, all columns), copies their
+// rows into a ring of its own (asynchronous copies, kMoeStages stages of 4 KB, refilled as soon as
+// a stage is read) and keeps the tile's sums in registers.  Nothing is handed from warp to warp on
+// the way, so the warps drift apart and cover each other's latencies, and nothing is waited for
+// that could fail to come.
 //
 // Precision: weights are exact in bf16 (int8 and e4m3 too; their scales multiply fp32 sums).  x
 // and the activations a are split into bf16 terms that add up to the value: x in bf16 one, fp16
 // two (exact), fp32 three (exact); a two (16 bits, below the rounding of a 16-bit y) or three
 // for an fp32 layer.  All sums are fp32.
 //
-// Kernel 1 (clusters of 8 CTAs): every cluster computes all logits, each CTA over an eighth of the
+// Kernel 1 (clusters of 4 CTAs): every cluster computes all logits, each CTA over a quarter of the
 // columns, exchanged through distributed shared memory; then each CTA picks the experts and takes
 // its share of the (expert, channels) tiles: 8 gate rows and the 8 up rows of the same channels
 // (so the product of the two is taken in the thread that holds both).
@@ -26,18 +30,19 @@
 // them; every warp keeps its own partial outputs, added in warp order at the end.
 // No atomics on floating-point values: results repeat bit for bit.
 #pragma once
+#include <type_traits>
+
 #include "ops_common.cuh"
 #include "tc_layer.cuh"
 
 namespace llk {
 
-constexpr int kMoeThreads = 288;        // warps 0..7 compute, warp 8 copies
 constexpr int kMoeWarps = 8;
-constexpr int kMoeCluster = 8;          // kernel 1
-constexpr int kMoeSegment = 1024;       // bytes of a weight row per stage: 128 per computing warp
-constexpr int kMoePitch = kMoeSegment + 64;  // 64 mod 128: the 8 rows that a quarter warp reads do not collide
-constexpr int kMoeStage = 16 * kMoePitch;
-constexpr int kMoeMaxStages = 12;
+constexpr int kMoeThreads = 32 * kMoeWarps;
+constexpr int kMoeCluster = 4;          // kernel 1
+constexpr int kMoeStage = 5120;         // bytes of a ring stage: 16 rows of 256 + 64, or fewer longer ones
+constexpr int kMoeStages = 4;           // stages of a warp's ring
+constexpr int kMoeRing = kMoeWarps * kMoeStages * kMoeStage;
 constexpr int kMoeMaxPairs = LL_MOE_MAX_ROWS * LL_MOE_MAX_TOPK;
 
 struct MoeParams {
@@ -50,7 +55,7 @@ struct MoeParams {
     int router_f32, router_vec, x_vec;  // *_vec: rows start on 16 bytes
     const uint8_t *wg, *wu, *wd;
     const float *sg, *su, *sd;
-    int up_ring, down_ring;             // weight rows start on 16 bytes and are multiples of 16 bytes long
+    int up_grain, down_grain;           // weight rows start on and are multiples of so many bytes (1 .. 16)
     int *ids;                           // workspace [rows][top_k]
     float *probs;
     int *user_ids;                      // or nullptr
@@ -58,14 +63,12 @@ struct MoeParams {
     __nv_bfloat16 *hid;                 // workspace: planes [rows * top_k][hid_ld]
     long long hid_plane;
     int hid_ld;
-    int stages;                         // of the ring
-    unsigned *status;
-    unsigned long long wait_ns;
 };
 
-// ---- shared memory after the ring (byte offsets; the ring is at 0) ----
+// ---- shared memory (byte offsets) ----
+// The warps' rings from 0; kernel 1's logits lie in the same place, read before the rings fill.
 struct MoeSmem {
-    int bars, pairs, ids, probs, mask, act_e, act_off, misc, logits, part, red, total;
+    int pairs, ids, probs, mask, act_e, act_off, misc, logits, part, x, total;
 };
 
 __host__ __device__ inline int moe_up16(int v)
@@ -73,32 +76,27 @@ __host__ __device__ inline int moe_up16(int v)
     return (v + 15) & ~15;
 }
 
-__host__ __device__ inline MoeSmem moe_smem(const MoeParams &p, bool up, int nt)
+__host__ __device__ inline MoeSmem moe_smem(const MoeParams &p, bool up)
 {
     MoeSmem s;
-    int o = p.stages * kMoeStage;
-    const int n = p.rows * p.top_k;
-    s.bars = o, o += moe_up16(16 * kMoeMaxStages);
-    s.misc = o, o += 16;  // fail flag, number of picked experts
+    const int n = p.rows * p.top_k, picked = p.experts < n ? p.experts : n;
+    int o = kMoeRing;
+    s.misc = o, o += 16;  // number of picked experts
     s.pairs = o, o += moe_up16(2 * n);
     s.ids = o, o += moe_up16(4 * n);
     s.probs = o, o += moe_up16(4 * n);
     s.mask = o, o += moe_up16(4 * p.experts);
-    s.act_e = o, o += moe_up16(2 * (p.experts < n ? p.experts : n));
-    s.act_off = o, o += moe_up16(2 * ((p.experts < n ? p.experts : n) + 1));
-    s.logits = s.part = 0;
-    if (up) {
-        const int mt = (p.experts + 15) / 16, ksub = mt >= kMoeWarps ? 1 : kMoeWarps / mt;
-        const int tp = (p.rows + 7) / 8 * 8;
-        s.logits = o, o += moe_up16(4 * p.rows * p.experts);
-        s.part = o, o += 4 * ksub * mt * 16 * tp;
-        s.red = o, o += 2 * kMoeWarps * nt * 32 * 16;
-    } else {
-        s.red = o, o += kMoeWarps * p.rows * 16 * 4;
-    }
+    s.act_e = o, o += moe_up16(2 * picked);
+    s.act_off = o, o += moe_up16(2 * (picked + 1));
+    s.logits = 0;
+    s.part = moe_up16(4 * p.rows * p.experts);  // kernel 1: at most 32 + 64 KB with the logits
+    s.x = o;  // kernel 1: the rows of x, where they are staged
+    if (!up)
+        s.part = o, o += kMoeWarps * p.rows * 16 * 4;
     s.total = o;
     return s;
 }
+static_assert(4 * LL_MOE_MAX_ROWS * LL_MOE_MAX_EXPERTS * 2 <= kMoeRing, "logits and their parts fit the rings' place");
 
 // ---- bf16 terms ----
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi)
@@ -137,13 +135,17 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Weight types: EP values in 16 bytes; widen() gives them as EP / 2 packed bf16 pairs, exact.
+// Weight types: EP values in 16 bytes; widen() gives them as EP / 2 packed bf16 pairs times UNIT
+// (exact).  PERM: of every four values the pairs are (0, 2) and (1, 3), and x follows.
+constexpr float kMoeF8Up = 0x1p40f, kMoeF8Back = 0x1p80f;
+
 template <int WT>
 struct MoeW;
 
 template <>
 struct MoeW<LL_W_BF16> {
     static constexpr int BYTES = 2, EP = 8;
+    static constexpr bool PERM = false;
     static __device__ __forceinline__ void widen(const uint4 &v, uint32_t (&o)[4])
     {
         o[0] = v.x, o[1] = v.y, o[2] = v.z, o[3] = v.w;
@@ -153,115 +155,212 @@ struct MoeW<LL_W_BF16> {
 template <>
 struct MoeW<LL_W_I8> {
     static constexpr int BYTES = 1, EP = 16;
-    static __device__ __forceinline__ void widen(const uint4 &v, uint32_t (&o)[8])
+    static constexpr bool PERM = false;
+    // A byte b = m - 128 s (s its sign bit, m the rest): bf16 0x43mm is 128 + m and 0x4300 | 128 s is
+    // 128 + 128 s, so their difference, exact, is b.
+    static __device__ __forceinline__ uint32_t pair(uint32_t w, uint32_t sel)
     {
-        i8x4_to_bf16x4(v.x, o[0], o[1]);
-        i8x4_to_bf16x4(v.y, o[2], o[3]);
-        i8x4_to_bf16x4(v.z, o[4], o[5]);
-        i8x4_to_bf16x4(v.w, o[6], o[7]);
-    }
-};
-
-template <>
-struct MoeW<LL_W_F8> {
-    static constexpr int BYTES = 1, EP = 16;
-    static __device__ __forceinline__ uint32_t pair(uint32_t two)
-    {
-        uint32_t h;
-        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)two));
-        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h));
-        return pack_bf16(f.x, f.y);
+        const uint32_t p = prmt(w, 0x43434343u, sel);
+        return bf16x2_sub(p & 0xff7fff7fu, p & 0xff80ff80u);
     }
     static __device__ __forceinline__ void widen(const uint4 &v, uint32_t (&o)[8])
     {
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            o[2 * i] = pair(w[i] & 0xffffu);
-            o[2 * i + 1] = pair(w[i] >> 16);
+            o[2 * i] = pair(w[i], 0x4140u);
+            o[2 * i + 1] = pair(w[i], 0x4342u);
         }
     }
 };
 
-// The first n values of 16 bytes at p (n <= 0: none), the others zero; any alignment.
-template <int BYTES>
-__device__ __forceinline__ uint4 load_some(const uint8_t *p, int n)
-{
-    uint32_t w[4] = {0, 0, 0, 0};
+template <>
+struct MoeW<LL_W_F8> {
+    static constexpr int BYTES = 1, EP = 16;
+    static constexpr bool PERM = true;
+    // Sign, exponent and significand moved to their bf16 places are the value times 2^-120 (the
+    // exponents' biases differ by 120; e4m3's subnormals become bf16's).  x is multiplied by
+    // kMoeF8Up = 2^40 beforehand, so the sums carry 2^-80, far above fp32's underflow, and are
+    // multiplied by kMoeF8Back at the end: 7 operations for 4 values, where the conversion
+    // instructions run at a fraction of the rate.  NaN (0x7f) would read as 480: looked for.
+    static __device__ __noinline__ uint32_t nan_in(uint32_t w, uint32_t o)  // bytes 0 and 2 of w
+    {
+        const uint32_t b0 = w & 0x7fu, b1 = (w >> 16) & 0x7fu;
+        return (b0 == 0x7fu ? 0x7fffu : o & 0xffffu) | (b1 == 0x7fu ? 0x7fff0000u : o & 0xffff0000u);
+    }
+    static __device__ __forceinline__ void widen(const uint4 &v, uint32_t (&o)[8])
+    {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < 16 / BYTES; ++i)
-        if (i < n) {
-            const uint32_t v = BYTES == 1 ? (uint32_t)p[i] : (uint32_t) reinterpret_cast<const uint16_t *>(p)[i];
-            w[i * BYTES / 4] |= v << (8 * (i * BYTES % 4));
+        for (int i = 0; i < 4; ++i) {
+            o[2 * i] = ((w[i] << 8) & 0x80008000u) | ((w[i] << 4) & 0x07f007f0u);  // bytes 0 and 2
+            o[2 * i + 1] = (w[i] & 0x80008000u) | ((w[i] >> 4) & 0x07f007f0u);     // bytes 1 and 3
+            top |= (w[i] & 0x7f7f7f7fu) + 0x01010101u;  // bit 7 of a byte: it was 0x7f
         }
-    return make_uint4(w[0], w[1], w[2], w[3]);
+        if (top & 0x80808080u) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                o[i] = nan_in(w[i >> 1] >> (8 * (i & 1)), o[i]);
+        }
+    }
+};
+
+// (v0, v1), (v2, v3) -> (v0, v2), (v1, v3)
+__device__ __forceinline__ void moe_permute(uint32_t &a, uint32_t &b)
+{
+    const uint32_t lo = prmt(a, b, 0x5410u), hi = prmt(a, b, 0x7632u);
+    a = lo;
+    b = hi;
 }
 
-// EP consecutive values of a row of x as NS packed bf16 terms: n of them exist (n <= 0: none).
+constexpr int moe_terms(int x_type)
+{
+    return x_type == LL_T_BF16 ? 1 : x_type == LL_T_F16 ? 2 : 3;
+}
+
+// Rows of x in global memory: EP consecutive values as RAW 16-byte words, and those as NS packed
+// bf16 terms.
 template <int XT>
 struct MoeX {
-    static constexpr int NS = XT == LL_T_BF16 ? 1 : XT == LL_T_F16 ? 2 : 3;
+    static constexpr int NS = moe_terms(XT);
     static constexpr int BYTES = XT == LL_T_F32 ? 4 : 2;
-
+    static constexpr bool GLOBAL = true;
     template <int EP>
-    static __device__ __forceinline__ void load(const uint8_t *row, int k, int n, bool vec, uint32_t (&w)[NS][EP / 2])
+    static constexpr int RAW = EP * BYTES / 16;
+
+    const uint8_t *base;
+    size_t row_bytes;
+    int cols;
+    bool vec;  // rows start on 16 bytes
+
+    // Values k .. k + EP - 1 of a row, zero from column `cols` on.
+    template <int EP>
+    __device__ __forceinline__ void load(uint32_t row, int k, uint4 (&v)[RAW<EP>]) const
     {
-        const uint8_t *p = row + (size_t)k * BYTES;
+        const uint8_t *p = base + row * row_bytes + (size_t)k * BYTES;
+        const int n = cols - k;
         if (vec && n >= EP) {
 #pragma unroll
-            for (int i = 0; i < EP * BYTES / 16; ++i) {
-                const uint4 v = __ldg(reinterpret_cast<const uint4 *>(p) + i);
-                take<EP>(v, i, w);
-            }
+            for (int i = 0; i < RAW<EP>; ++i)
+                v[i] = __ldg(reinterpret_cast<const uint4 *>(p) + i);
         } else {
+#pragma unroll 1
+            for (int i = 0; i < RAW<EP>; ++i) {
+                uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
-            for (int i = 0; i < EP * BYTES / 16; ++i) {
-                const int have = n - i * (16 / BYTES);
-                uint4 v;
-                if constexpr (BYTES == 4) {
-                    const uint32_t *q = reinterpret_cast<const uint32_t *>(p) + 4 * i;
-                    v.x = have > 0 ? __ldg(q) : 0u;
-                    v.y = have > 1 ? __ldg(q + 1) : 0u;
-                    v.z = have > 2 ? __ldg(q + 2) : 0u;
-                    v.w = have > 3 ? __ldg(q + 3) : 0u;
-                } else {
-                    v = load_some<2>(p + 16 * i, have);
-                }
-                take<EP>(v, i, w);
+                for (int j = 0; j < 16 / BYTES; ++j)
+                    if (i * (16 / BYTES) + j < n) {
+                        const uint32_t one = BYTES == 4
+                                                 ? __ldg(reinterpret_cast<const uint32_t *>(p) + 4 * i + j)
+                                                 : (uint32_t)__ldg(reinterpret_cast<const uint16_t *>(p) + 8 * i + j);
+                        w[j * BYTES / 4] |= one << (8 * (j * BYTES % 4));
+                    }
+                const uint4 t = make_uint4(w[0], w[1], w[2], w[3]);
+#pragma unroll
+                for (int j = 0; j < RAW<EP>; ++j)  // v is kept in registers: no index that is not known
+                    if (j == i)
+                        v[j] = t;
             }
         }
     }
 
-    // The i-th 16 bytes of the values into their places.
-    template <int EP>
-    static __device__ __forceinline__ void take(const uint4 &v, int i, uint32_t (&w)[NS][EP / 2])
+    template <int EP, bool PERM>
+    static __device__ __forceinline__ void terms(const uint4 (&v)[RAW<EP>], uint32_t (&w)[NS][EP / 2])
     {
-        if constexpr (XT == LL_T_BF16) {
-            w[0][4 * i] = v.x, w[0][4 * i + 1] = v.y, w[0][4 * i + 2] = v.z, w[0][4 * i + 3] = v.w;
-        } else if constexpr (XT == LL_T_F16) {
-            const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+        const float up = PERM ? kMoeF8Up : 1.0f;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&u[j]));
-                uint32_t t[NS];
-                split_pair<NS>(f.x, f.y, t);
+        for (int i = 0; i < RAW<EP>; ++i) {
+            const uint32_t u[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+            if constexpr (BYTES == 4) {
 #pragma unroll
-                for (int s = 0; s < NS; ++s)
-                    w[s][4 * i + j] = t[s];
+                for (int j = 0; j < 2; ++j) {
+                    uint32_t t[NS];
+                    split_pair<NS>(__uint_as_float(u[2 * j]) * up, __uint_as_float(u[2 * j + 1]) * up, t);
+#pragma unroll
+                    for (int s = 0; s < NS; ++s)
+                        w[s][2 * i + j] = t[s];
+                }
+            } else if constexpr (XT == LL_T_BF16) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    w[0][4 * i + j] = u[j];
+                    if constexpr (PERM)  // 0x5380: 2^40
+                        asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(w[0][4 * i + j]) : "r"(0x53805380u));
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&u[j]));
+                    uint32_t t[NS];
+                    split_pair<NS>(f.x * up, f.y * up, t);
+#pragma unroll
+                    for (int s = 0; s < NS; ++s)
+                        w[s][4 * i + j] = t[s];
+                }
             }
-        } else {
-            uint32_t t[NS];
-            split_pair<NS>(__uint_as_float(v.x), __uint_as_float(v.y), t);
-#pragma unroll
-            for (int s = 0; s < NS; ++s)
-                w[s][2 * i] = t[s];
-            split_pair<NS>(__uint_as_float(v.z), __uint_as_float(v.w), t);
-#pragma unroll
-            for (int s = 0; s < NS; ++s)
-                w[s][2 * i + 1] = t[s];
         }
+        if constexpr (PERM)
+#pragma unroll
+            for (int s = 0; s < NS; ++s)
+#pragma unroll
+                for (int j = 0; j < EP / 2; j += 2)
+                    moe_permute(w[s][j], w[s][j + 1]);
     }
 };
+
+// Rows of bf16 terms, ready for the tensor instruction: planes of rows, zero behind the last column.
+// SMEM: x staged in shared memory by kernel 1; else the activations in the workspace, written by
+// kernel 1 while kernel 2 may already be resident, so read past L1.
+template <int NSP, bool SMEM>
+struct MoeTerms {
+    static constexpr int NS = NSP;
+    static constexpr bool GLOBAL = !SMEM;
+    template <int EP>
+    static constexpr int RAW = NSP * EP / 8;
+
+    const uint8_t *base;
+    size_t plane;  // bytes
+    uint32_t pitch;
+
+    template <int EP>
+    __device__ __forceinline__ void load(uint32_t row, int k, uint4 (&v)[RAW<EP>]) const
+    {
+        const uint8_t *p = base + (size_t)row * pitch + (size_t)k * 2;
+#pragma unroll
+        for (int s = 0; s < NSP; ++s)
+#pragma unroll
+            for (int i = 0; i < EP / 8; ++i) {
+                const uint4 *q = reinterpret_cast<const uint4 *>(p + s * plane) + i;
+                v[s * (EP / 8) + i] = SMEM ? *q : __ldcg(q);
+            }
+    }
+
+    template <int EP, bool PERM>
+    static __device__ __forceinline__ void terms(const uint4 (&v)[RAW<EP>], uint32_t (&w)[NSP][EP / 2])
+    {
+#pragma unroll
+        for (int s = 0; s < NSP; ++s)
+#pragma unroll
+            for (int i = 0; i < EP / 8; ++i) {
+                const uint4 t = v[s * (EP / 8) + i];
+                w[s][4 * i] = t.x, w[s][4 * i + 1] = t.y, w[s][4 * i + 2] = t.z, w[s][4 * i + 3] = t.w;
+            }
+    }
+};
+
+// Columns of a row of terms: whole steps of 256 bytes of weights.
+__host__ __device__ constexpr int moe_cols(int cols, int wbytes)
+{
+    return (cols + 256 / wbytes - 1) / (256 / wbytes) * (256 / wbytes);
+}
+
+// Bytes between rows of x in shared memory (8-byte types: the 16-byte pieces that a quarter of the
+// warp reads are 32 bytes apart in a row and 16 from row to row; bf16: 16 and 64).
+__host__ __device__ constexpr int moe_x_pitch(int cols, int wbytes)
+{
+    return 2 * moe_cols(cols, wbytes) + (wbytes == 1 ? 16 : 64);
+}
 
 // ---- the lists of picked experts, from the ids in shared memory (all threads; rows <= 32) ----
 // act_e[a] = a-th picked expert (rising), its rows are pairs[act_off[a] .. act_off[a + 1]),
@@ -305,11 +404,11 @@ __device__ __forceinline__ void moe_lists(const MoeParams &p, uint8_t *smem, con
         }
         if (lane == 0) {
             act_off[a0] = (uint16_t)off0;
-            misc[1] = (uint32_t)a0;
+            misc[0] = (uint32_t)a0;
         }
     }
     __syncthreads();
-    const int na = (int)misc[1];
+    const int na = (int)misc[0];
     for (int i = threadIdx.x; i < n; i += blockDim.x) {
         const int row = i / p.top_k, slot = i - row * p.top_k, e = ids[i];
         int lo = 0, hi = na - 1;  // the place of e among the picked
@@ -325,159 +424,266 @@ __device__ __forceinline__ void moe_lists(const MoeParams &p, uint8_t *smem, con
     __syncthreads();
 }
 
-// ---- the ring ----
+// ---- a warp's ring of weight rows ----
+// BYTES to shared memory, the first n of them from src, the others zero.
+template <int BYTES>
+__device__ __forceinline__ void cp_async(uint32_t dst, const void *src, int n)
+{
+    if constexpr (BYTES == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(n)
+                     : "memory");
+}
+
+// Tiles of `rows` rows come in segments of 256 << m bytes per row, m as large as 16 rows' 256 bytes
+// allow (a pitch of 64 mod 128 bytes, so that the 8 rows that a quarter of the warp reads do not
+// collide); rows that do not exist and what lies behind a row's end are zero.  The warp issues its
+// tiles' segments in order, kMoeStages ahead, one group of copies per segment (empty ones past the
+// last, so that the count of groups tells which has landed).
 struct MoeRing {
-    uint32_t base, bars;
-    int stages;
-    __device__ __forceinline__ uint32_t full(int s) const
+    uint32_t base;  // shared-memory address of this warp's stages
+    int rows, m, grain;
+    int q, n;       // next tile to be copied, number of tiles
+    int slot, off, row_bytes;
+    const uint8_t *s0, *s1;  // first row of tile q, and first of its second half (rows half ..)
+    int half, have;          // rows that exist: i < have, half + i < half + have
+
+    __device__ __forceinline__ int seg() const
     {
-        return bars + 16u * (uint32_t)s;
+        return 256 << m;
     }
-    __device__ __forceinline__ uint32_t empty(int s) const
+    __device__ __forceinline__ int pitch() const
     {
-        return bars + 16u * (uint32_t)s + 8u;
+        return seg() + 64;
+    }
+    __device__ __forceinline__ void shape(int r)
+    {
+        rows = r;
+        m = r > 8 ? 0 : r > 4 ? 1 : r > 2 ? 2 : r > 1 ? 3 : 4;
+    }
+
+    // The segment in pieces of 16 bytes, 16 pieces (a half warp) of one row at a time.
+    template <int GRAIN>
+    __device__ __forceinline__ void copy()
+    {
+        const int lane = threadIdx.x & 31, pl = (lane & 15) * 16;
+        const uint32_t dst = base + (uint32_t)(slot * kMoeStage + pl);
+        constexpr int UN = GRAIN == 16 ? 4 : 1;
+#pragma unroll UN
+        for (int c = lane >> 4; c < rows << m; c += 2) {
+            const int r = c >> m, at = off + pl + ((c - (r << m)) << 8);
+            const int h = r < half ? r : r - half;
+            const int n = h < have ? min(16, max(0, row_bytes - at)) : 0;
+            const uint8_t *src = n > 0 ? (r < half ? s0 : s1) + (size_t)h * (size_t)row_bytes + at : s0;
+            const uint32_t d = dst + (uint32_t)(r * pitch() + ((c - (r << m)) << 8));
+            if constexpr (GRAIN == 16) {
+                cp_async<16>(d, src, n);
+            } else if constexpr (GRAIN >= 4) {
+#pragma unroll
+                for (int i = 0; i < 16; i += GRAIN)
+                    cp_async<GRAIN>(d + i, n > i ? src + i : s0, n > i ? GRAIN : 0);
+            } else {  // rows on odd addresses: by value
+                uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (i < n)
+                        w[i / 4] |= (uint32_t)__ldg(src + i) << (8 * (i % 4));
+                st_shared_v4(d, make_uint4(w[0], w[1], w[2], w[3]));
+            }
+        }
+    }
+
+    template <class TileAt>
+    __device__ __forceinline__ void feed(TileAt tile_at)
+    {
+        if (q < n) {
+            if (off == 0)
+                tile_at(q, s0, s1, half, have);
+            if (grain >= 16)
+                copy<16>();
+            else if (grain >= 8)
+                copy<8>();
+            else if (grain >= 4)
+                copy<4>();
+            else
+                copy<1>();
+            slot = slot + 1 == kMoeStages ? 0 : slot + 1;
+            off += seg();
+            if (off >= row_bytes) {
+                off = 0;
+                ++q;
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+
+    // The oldest segment has landed, for the whole warp.
+    __device__ __forceinline__ void wait() const
+    {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kMoeStages - 1) : "memory");
+        __syncwarp();
     }
 };
 
-__device__ __forceinline__ void moe_ring_init(const MoeRing &r)
-{
-    for (int s = 0; s < r.stages; ++s) {
-        mbar_init(r.full(s), 1);
-        mbar_init(r.empty(s), kMoeWarps);
-    }
-    fence_mbar_init_cluster();
-}
-
-// The copying warp's part for one set of 16 rows: their segments one after another.  `src` is this
-// lane's row (lanes 0..15; nullptr: no such row), `bytes` its length.  `it` counts stages.
-__device__ __forceinline__ bool moe_copy_rows(const MoeParams &p, const MoeRing &r, const uint8_t *src, int bytes,
-                                              int n_rows, uint32_t &it, volatile uint32_t *fail)
-{
-    const int lane = threadIdx.x & 31;
-    for (int o = 0; o < bytes; o += kMoeSegment, ++it) {
-        const int s = (int)(it % (uint32_t)r.stages);
-        const uint32_t lap = it / (uint32_t)r.stages;
-        const int len = min(kMoeSegment, bytes - o);
-        if (lap > 0 && !tc_wait_warp(r.empty(s), (lap - 1) & 1, p.wait_ns, fail, p.status, 1))
-            return false;
-        if (lane == 0)
-            mbar_arrive_expect_tx(r.full(s), (uint32_t)(len * n_rows));
-        __syncwarp();
-        if (src)
-            bulk_g2s(r.base + (uint32_t)(s * kMoeStage + lane * kMoePitch), src + o, (uint32_t)len, r.full(s));
-    }
-    return true;
-}
-
-// Waits for the loads of the last stages: nothing is in flight when the CTA leaves.
-__device__ __forceinline__ void moe_drain(const MoeParams &p, const MoeRing &r, uint32_t it)
-{
-    const uint32_t n = min(it, (uint32_t)r.stages);
-    for (uint32_t j = it - n; j < it; ++j) {
-        const uint64_t t0 = globaltimer();
-        while (!mbar_try_wait(r.full((int)(j % (uint32_t)r.stages)), (j / (uint32_t)r.stages) & 1) &&
-               globaltimer() - t0 < p.wait_ns) {
-        }
-    }
-}
-
-// One warp's 128 bytes of each of 16 weight rows against the n-tiles of x: acc += W x.
-// r0 / r1: this thread's rows g and g + 8 at the warp's bytes (shared or global memory); k0: their
-// first column; K: columns of the row; wvec: 16-byte loads allowed; load_x(nt, k, n, words).
-template <int WT, int NS, int NT, class LoadX>
-__device__ __forceinline__ void moe_step(float (&acc)[NT][4], const uint8_t *r0, const uint8_t *r1, bool wvec, int k0,
-                                         int K, int ntc, LoadX load_x)
+// 64 bytes (a piece of 16 per thread) of each of the tile's rows (r0 / r1: this thread's rows g and
+// g + 8 in the stage) against the n-tiles of x: d += W x.  PRE: the first n-tile's x is in b.
+template <int WT, int NT, bool PRE, class Src, int RAW>
+__device__ __forceinline__ void moe_piece(float (&d)[NT][4], const uint8_t *r0, const uint8_t *r1, int k, int ntc,
+                                          const Src &src, const uint32_t (&xrow)[NT], const uint4 (&b)[RAW])
 {
     using W = MoeW<WT>;
-    constexpr int EP = W::EP;
-    const int t = threadIdx.x & 3;
+    constexpr int EP = W::EP, NS = Src::NS;
+    uint32_t a0[EP / 2], a1[EP / 2];
+    W::widen(*reinterpret_cast<const uint4 *>(r0), a0);
+    W::widen(*reinterpret_cast<const uint4 *>(r1), a1);
 #pragma unroll
-    for (int pc = 0; pc < 2; ++pc) {
-        const int ko = pc * 4 * EP + t * EP;  // this thread's values within the step
-        const int n = K - (k0 + ko);
-        uint4 v0, v1;
-        if (wvec && n >= EP) {
-            v0 = *reinterpret_cast<const uint4 *>(r0 + ko * W::BYTES);
-            v1 = *reinterpret_cast<const uint4 *>(r1 + ko * W::BYTES);
-        } else {
-            v0 = load_some<W::BYTES>(r0 + ko * W::BYTES, n);
-            v1 = load_some<W::BYTES>(r1 + ko * W::BYTES, n);
-        }
-        uint32_t a0[EP / 2], a1[EP / 2];
-        W::widen(v0, a0);
-        W::widen(v1, a1);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            if (nt < ntc) {
-                uint32_t b[NS][EP / 2];
-                load_x(nt, k0 + ko, n, b);
-#pragma unroll
-                for (int j = 0; j < EP / 4; ++j)
-#pragma unroll
-                    for (int s = 0; s < NS; ++s)
-                        mma_bf16(acc[nt], a0[2 * j], a1[2 * j], a0[2 * j + 1], a1[2 * j + 1], b[s][2 * j],
-                                 b[s][2 * j + 1]);
+    for (int nt = 0; nt < NT; ++nt) {
+        if (nt < ntc) {
+            uint32_t w[NS][EP / 2];
+            if (PRE && nt == 0) {
+                Src::template terms<EP, W::PERM>(b, w);
+            } else {
+                uint4 v[RAW];
+                src.template load<EP>(xrow[nt], k, v);
+                Src::template terms<EP, W::PERM>(v, w);
             }
+#pragma unroll
+            for (int j = 0; j < EP / 4; ++j)
+#pragma unroll
+                for (int s = 0; s < NS; ++s)
+                    mma_bf16(d[nt], a0[2 * j], a1[2 * j], a0[2 * j + 1], a1[2 * j + 1], w[s][2 * j], w[s][2 * j + 1]);
         }
     }
 }
 
-// Sum over a whole set of 16 rows: this warp takes bytes 128 w .. 128 w + 127 of every segment.
-// Through the ring (row pointers unused) or straight from global memory.  e4m3: sc0 / sc1 are the
-// scales of the thread's rows g and g + 8 by 128-column block.
-template <int WT, int NS, int NT, class LoadX>
-__device__ __forceinline__ bool moe_rows(const MoeParams &p, const MoeRing &r, const uint8_t *smem, bool ring,
-                                         const uint8_t *g0, const uint8_t *g1, int K, const float *sc0,
-                                         const float *sc1, int ntc, uint32_t &it, bool ok, volatile uint32_t *fail,
-                                         float (&acc)[NT][4], LoadX load_x)
+// One tile: acc = (its rows) . x over all columns, in steps of 256 bytes of every row.  i0 / i1: places
+// of this thread's rows g and g + 8 in a stage; sc0 / sc1: their e4m3 scales by 128-column block.
+// Refills the ring as it goes.  A step's two halves are summed apart (two chains of dependent
+// tensor instructions); the sums run on in its accumulators, except that an e4m3 block's (its
+// scale) and an fp32 layer's (the instruction cuts off where fp32 would round) are added in fp32.
+template <int WT, int NT, class Src, class TileAt>
+__device__ __forceinline__ void moe_tile(MoeRing &r, const uint8_t *stages, int &slot, TileAt tile_at, int i0, int i1,
+                                         int K, const float *sc0, const float *sc1, int ntc, const Src &src,
+                                         const uint32_t (&xrow)[NT], float (&acc)[NT][4])
 {
     using W = MoeW<WT>;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2;
-    constexpr int KSEG = kMoeSegment / W::BYTES, KW = 128 / W::BYTES;
+    constexpr int EP = W::EP, RAW = Src::template RAW<EP>, KS = 256 / W::BYTES;
+    // x from global memory is loaded a step ahead where the registers allow (64)
+    constexpr bool PRE = Src::GLOBAL && 4 * RAW * 4 <= 64;
+    constexpr bool FRESH = WT == LL_W_F8 || Src::NS == 3;
+    const int t = threadIdx.x & 3, steps = (K + KS - 1) / KS, blocks = (K + kF8Block - 1) / kF8Block;
+    uint4 b[4][RAW], bn[4][RAW];
+    float f[4] = {1.0f, 1.0f, 1.0f, 1.0f}, fn[4] = {1.0f, 1.0f, 1.0f, 1.0f};  // e4m3: rows g, g + 8 by half
+    float d[2][NT][4];
+    auto load_step = [&](int st) {
+        if constexpr (PRE)
+#pragma unroll
+            for (int pc = 0; pc < 4; ++pc)
+                src.template load<EP>(xrow[0], st * KS + pc * 4 * EP + t * EP, bn[pc]);
+        if constexpr (WT == LL_W_F8) {
+            const int j0 = 2 * st, j1 = min(2 * st + 1, blocks - 1);
+            fn[0] = __ldg(sc0 + j0);
+            fn[1] = __ldg(sc1 + j0);
+            fn[2] = __ldg(sc0 + j1);
+            fn[3] = __ldg(sc1 + j1);
+        }
+    };
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i) {
             acc[nt][i] = 0.0f;
-    for (int kseg = 0; kseg < K; kseg += KSEG, ++it) {
-        const int k0 = kseg + warp * KW;
-        const uint8_t *r0 = g0 + (size_t)k0 * W::BYTES, *r1 = g1 + (size_t)k0 * W::BYTES;
-        int s = 0;
-        if (ring) {
-            s = (int)(it % (uint32_t)r.stages);
-            r0 = smem + s * kMoeStage + g * kMoePitch + warp * 128;
-            r1 = r0 + 8 * kMoePitch;
-            if (ok)
-                ok = tc_wait_warp(r.full(s), (it / (uint32_t)r.stages) & 1, p.wait_ns, fail, p.status, 2);
+            d[0][nt][i] = d[1][nt][i] = 0.0f;
         }
-        if (ok && k0 < K) {
-            if constexpr (WT == LL_W_F8) {
-                float part[NT][4] = {};
-                const float f0 = __ldg(sc0 + k0 / kF8Block), f1 = __ldg(sc1 + k0 / kF8Block);
-                moe_step<WT, NS, NT>(part, r0, r1, ring, k0, K, ntc, load_x);
+    load_step(0);
+    for (int st = 0; st < steps;) {
+        const uint8_t *at = stages + slot * kMoeStage + t * 16;
+        const uint8_t *r0 = at + i0 * r.pitch(), *r1 = at + i1 * r.pitch();
+        const int end = min(steps, st + (1 << r.m));
+        r.wait();
+#pragma unroll 1
+        for (; st < end; ++st) {
+            if constexpr (PRE)
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    acc[nt][0] = fmaf(part[nt][0], f0, acc[nt][0]);
-                    acc[nt][1] = fmaf(part[nt][1], f0, acc[nt][1]);
-                    acc[nt][2] = fmaf(part[nt][2], f1, acc[nt][2]);
-                    acc[nt][3] = fmaf(part[nt][3], f1, acc[nt][3]);
-                }
-            } else {
-                moe_step<WT, NS, NT>(acc, r0, r1, ring, k0, K, ntc, load_x);
-            }
+                for (int pc = 0; pc < 4; ++pc)
+#pragma unroll
+                    for (int i = 0; i < RAW; ++i)
+                        b[pc][i] = bn[pc][i];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                f[i] = fn[i];
+            if (st + 1 < steps)
+                load_step(st + 1);  // on its way while this step is computed
+            if constexpr (FRESH)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        d[0][nt][i] = d[1][nt][i] = 0.0f;
+#pragma unroll
+            for (int pc = 0; pc < 4; ++pc)
+                moe_piece<WT, NT, PRE>(d[pc >> 1], r0 + 64 * pc, r1 + 64 * pc, st * KS + pc * 4 * EP + t * EP, ntc, src, xrow,
+                                  b[pc]);
+            if constexpr (FRESH)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        acc[nt][0] = fmaf(d[h][nt][0], f[2 * h], acc[nt][0]);
+                        acc[nt][1] = fmaf(d[h][nt][1], f[2 * h], acc[nt][1]);
+                        acc[nt][2] = fmaf(d[h][nt][2], f[2 * h + 1], acc[nt][2]);
+                        acc[nt][3] = fmaf(d[h][nt][3], f[2 * h + 1], acc[nt][3]);
+                    }
+            r0 += 256;
+            r1 += 256;
         }
-        if (ring) {
-            __syncwarp();
-            if (lane == 0)
-                mbar_arrive_local(r.empty(s));
-        }
+        __syncwarp();  // every lane has read the stage
+        slot = slot + 1 == kMoeStages ? 0 : slot + 1;
+        r.feed(tile_at);
     }
-    return ok;
+    if constexpr (!FRESH)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                acc[nt][i] = d[0][nt][i] + d[1][nt][i];
+    if constexpr (WT == LL_W_F8)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                acc[nt][i] *= kMoeF8Back;
 }
 
-__device__ __forceinline__ void moe_bar()
+// This thread's pieces of the router's rows e0 and e1 (columns k0 .. k0 + 63) as bf16 terms.
+template <int RT, int NR>
+__device__ __forceinline__ void moe_router_step(const MoeParams &p, uint32_t e0, uint32_t e1, int k0, uint32_t (&a0)[2][3][4],
+                                                uint32_t (&a1)[2][3][4])
 {
-    asm volatile("bar.sync 1, 256;" ::: "memory");  // the computing warps
+    using R = MoeX<RT>;
+    const R src = {static_cast<const uint8_t *>(p.router), (size_t)p.hidden * R::BYTES, p.hidden, p.router_vec != 0};
+    const int t = threadIdx.x & 3;
+    uint4 v[2][2][R::template RAW<8>];
+#pragma unroll
+    for (int pc = 0; pc < 2; ++pc) {
+        const int k = k0 + pc * 32 + t * 8;
+        src.template load<8>(e0, k, v[pc][0]);
+        src.template load<8>(e1, k, v[pc][1]);
+    }
+#pragma unroll
+    for (int pc = 0; pc < 2; ++pc) {
+        uint32_t w[2][NR][4];
+        R::template terms<8, false>(v[pc][0], w[0]);
+        R::template terms<8, false>(v[pc][1], w[1]);
+#pragma unroll
+        for (int s = 0; s < NR; ++s)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                a0[pc][s][j] = w[0][s][j];
+                a1[pc][s][j] = w[1][s][j];
+            }
+    }
 }
 
 // ---- router: logits of every (row, expert), by the whole cluster ----
@@ -486,42 +692,42 @@ __device__ __forceinline__ void moe_logits(const MoeParams &p, uint8_t *smem, co
 {
     using X = MoeX<XT>;
     constexpr int EP = 8, KS = 64;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int tid = threadIdx.x, warp = tid >> 5, g = (tid & 31) >> 2, t = tid & 3;
     const int mt_n = (p.experts + 15) / 16, ksub = mt_n >= kMoeWarps ? 1 : kMoeWarps / mt_n;
     const int tp = (p.rows + 7) / 8 * 8, ntc = tp / 8, H = p.hidden;
     const int rank = (int)cluster_ctarank();
     float *part = reinterpret_cast<float *>(smem + L.part);
     const int steps = (H + KS - 1) / KS, slices = kMoeCluster * ksub;
-    const int esz = p.router_f32 ? 4 : 2;
-    if (warp < kMoeWarps) {
+    const X src = {static_cast<const uint8_t *>(p.x), (size_t)p.ldx * X::BYTES, H, p.x_vec != 0};
+    {
         for (int u = warp; u < mt_n * ksub; u += kMoeWarps) {
             const int mt = u / ksub, ks = u - mt * ksub, sl = rank * ksub + ks;
-            const uint8_t *w0 = static_cast<const uint8_t *>(p.router) +
-                                (size_t)min(mt * 16 + g, p.experts - 1) * H * esz;
-            const uint8_t *w1 = static_cast<const uint8_t *>(p.router) +
-                                (size_t)min(mt * 16 + g + 8, p.experts - 1) * H * esz;
+            const uint32_t e0 = (uint32_t)min(mt * 16 + g, p.experts - 1), e1 = (uint32_t)min(mt * 16 + g + 8, p.experts - 1);
             float acc[NT][4] = {};
+#pragma unroll(NT == 1 ? 4 : 1)
             for (int st = sl * steps / slices; st < (sl + 1) * steps / slices; ++st) {
+                uint4 xb[NT][2][X::template RAW<EP>];
 #pragma unroll
-                for (int pc = 0; pc < 2; ++pc) {
-                    const int k = st * KS + pc * 32 + t * EP, n = H - k;
-                    uint32_t a0[3][EP / 2], a1[3][EP / 2];
-                    if (p.router_f32) {
-                        MoeX<LL_T_F32>::load<EP>(w0, k, n, p.router_vec, a0);
-                        MoeX<LL_T_F32>::load<EP>(w1, k, n, p.router_vec, a1);
-                    } else {
-                        MoeX<LL_T_BF16>::load<EP>(w0, k, n, p.router_vec,
-                                                  reinterpret_cast<uint32_t(&)[1][EP / 2]>(a0[0]));
-                        MoeX<LL_T_BF16>::load<EP>(w1, k, n, p.router_vec,
-                                                  reinterpret_cast<uint32_t(&)[1][EP / 2]>(a1[0]));
-                    }
+                for (int nt = 0; nt < NT; ++nt)
+                    if (nt < ntc)
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-                        if (nt < ntc) {
+                        for (int pc = 0; pc < 2; ++pc) {
+                            const int k = st * KS + pc * 32 + t * EP;
+                            src.template load<EP>((uint32_t)min(nt * 8 + g, p.rows - 1), k, xb[nt][pc]);
+                        }
+                uint32_t a0[2][3][EP / 2], a1[2][3][EP / 2];
+                if (p.router_f32)
+                    moe_router_step<LL_T_F32, 3>(p, e0, e1, st * KS, a0, a1);
+                else
+                    moe_router_step<LL_T_BF16, 1>(p, e0, e1, st * KS, a0, a1);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+                    if (nt < ntc) {
+                        float part4[4] = {};  // each step from zero, then added in fp32
+#pragma unroll
+                        for (int pc = 0; pc < 2; ++pc) {
                             uint32_t b[X::NS][EP / 2];
-                            const int row = min(nt * 8 + g, p.rows - 1);
-                            X::template load<EP>(static_cast<const uint8_t *>(p.x) + (size_t)row * p.ldx * X::BYTES, k,
-                                                 n, p.x_vec, b);
+                            X::template terms<EP, false>(xb[nt][pc], b);
 #pragma unroll
                             for (int ra = 0; ra < 3; ++ra)
                                 if (ra == 0 || p.router_f32) {
@@ -529,11 +735,15 @@ __device__ __forceinline__ void moe_logits(const MoeParams &p, uint8_t *smem, co
                                     for (int s = 0; s < X::NS; ++s)
 #pragma unroll
                                         for (int j = 0; j < EP / 4; ++j)
-                                            mma_bf16(acc[nt], a0[ra][2 * j], a1[ra][2 * j], a0[ra][2 * j + 1],
-                                                     a1[ra][2 * j + 1], b[s][2 * j], b[s][2 * j + 1]);
+                                            mma_bf16(part4, a0[pc][ra][2 * j], a1[pc][ra][2 * j],
+                                                     a0[pc][ra][2 * j + 1], a1[pc][ra][2 * j + 1], b[s][2 * j],
+                                                     b[s][2 * j + 1]);
                                 }
                         }
-                }
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            acc[nt][i] += part4[i];
+                    }
             }
             float *o = part + (size_t)(ks * mt_n + mt) * 16 * tp;
 #pragma unroll
@@ -551,11 +761,11 @@ __device__ __forceinline__ void moe_logits(const MoeParams &p, uint8_t *smem, co
     cluster_sync();
     float *logits = reinterpret_cast<float *>(smem + L.logits);
     const uint32_t pa = smem_u32(part);
-    for (int i = tid; i < p.rows * p.experts; i += kMoeThreads) {
-        const int row = i / p.experts, e = i - row * p.experts;
+    for (int i = tid; i < tp * p.experts; i += kMoeThreads) {
+        const int e = i / tp, row = i - e * tp;  // consecutive threads: consecutive words
         float v = 0.0f;
         for (int ks = 0; ks < ksub; ++ks) {
-            const uint32_t at = pa + (uint32_t)((ks * mt_n * 16 + e) * tp + row) * 4u;
+            const uint32_t at = pa + (uint32_t)(ks * mt_n * 16 * tp + i) * 4u;
             float q[kMoeCluster];
 #pragma unroll
             for (int r = 0; r < kMoeCluster; ++r)
@@ -564,9 +774,10 @@ __device__ __forceinline__ void moe_logits(const MoeParams &p, uint8_t *smem, co
             for (int r = 0; r < kMoeCluster; ++r)
                 v += q[r];
         }
-        logits[row * p.experts + e] = v;
+        if (row < p.rows)
+            logits[row * p.experts + e] = v;
     }
-    // the peers' partial sums are read; matched by the wait at the kernel's end
+    // the peers' partial sums are read; matched by the wait before the rings fill
     __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     __syncthreads();
@@ -582,9 +793,9 @@ __device__ __forceinline__ uint32_t order_key(float v)
 }
 
 // ---- the top_k experts of each row and their weights (one warp per row) ----
+template <int PER>  // experts per lane
 __device__ __forceinline__ void moe_pick(const MoeParams &p, uint8_t *smem, const MoeSmem &L)
 {
-    constexpr int PER = LL_MOE_MAX_EXPERTS / 32;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int *ids = reinterpret_cast<int *>(smem + L.ids);
     float *probs = reinterpret_cast<float *>(smem + L.probs);
@@ -613,39 +824,64 @@ __device__ __forceinline__ void moe_pick(const MoeParams &p, uint8_t *smem, cons
             for (int off = 16; off > 0; off >>= 1)
                 sum += __shfl_xor_sync(0xffffffffu, sum, off);
         }
-        float mine = 0.0f;  // lane j: exp of the j-th picked logit
+        uint32_t mine = 0;  // lane j: the j-th picked expert
+#pragma unroll 1
         for (int j = 0; j < p.top_k; ++j) {
-            uint32_t best = 0u;
-#pragma unroll
-            for (int i = 0; i < PER; ++i)
-                best = max(best, key[i]);
-            best = __reduce_max_sync(0xffffffffu, best);
-            uint32_t at = 0xffffffffu;
+            uint32_t best = 0u, at = 0xffffffffu;
 #pragma unroll
             for (int i = PER - 1; i >= 0; --i)
-                if (key[i] == best && key[i] != 0u)
+                if (key[i] >= best && key[i] != 0u) {  // of equal keys the lowest index
+                    best = key[i];
                     at = (uint32_t)(lane + 32 * i);
-            at = __reduce_min_sync(0xffffffffu, at);
-            const float ex = expf(lg[at] - top);
+                }
+            const uint32_t top_key = __reduce_max_sync(0xffffffffu, best);
+            at = __reduce_min_sync(0xffffffffu, best == top_key ? at : 0xffffffffu);
             if (lane == j)
-                mine = ex;
-            if (p.renorm)
-                sum += ex;
+                mine = at;
 #pragma unroll
             for (int i = 0; i < PER; ++i)
                 if (at == (uint32_t)(lane + 32 * i))
                     key[i] = 0u;
-            if (lane == 0)
-                ids[row * p.top_k + j] = (int)at;
         }
-        if (lane < p.top_k)
-            probs[row * p.top_k + lane] = mine / sum;
+        const float ex = lane < p.top_k ? expf(lg[mine] - top) : 0.0f;
+        if (p.renorm) {
+            sum = ex;
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1)
+                sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        }
+        if (lane < p.top_k) {
+            ids[row * p.top_k + lane] = (int)mine;
+            probs[row * p.top_k + lane] = ex / sum;
+        }
     }
     __syncthreads();
 }
 
+// Kernel 1: the rows of x as planes of bf16 terms in shared memory, zero behind the last column.
+template <int WT, int XT>
+__device__ __forceinline__ void moe_stage_x(const MoeParams &p, uint8_t *to)
+{
+    using W = MoeW<WT>;
+    using X = MoeX<XT>;
+    const int pitch = moe_x_pitch(p.hidden, W::BYTES), chunks = moe_cols(p.hidden, W::BYTES) / 8;
+    const X src = {static_cast<const uint8_t *>(p.x), (size_t)p.ldx * X::BYTES, p.hidden, p.x_vec != 0};
+    for (int i = threadIdx.x; i < p.rows * chunks; i += kMoeThreads) {
+        const int row = i / chunks, c = i - row * chunks;
+        uint4 v[X::template RAW<8>];
+        src.template load<8>((uint32_t)row, c * 8, v);
+        uint32_t w[X::NS][4];
+        X::template terms<8, W::PERM>(v, w);
+#pragma unroll
+        for (int s = 0; s < X::NS; ++s)
+            *reinterpret_cast<uint4 *>(to + (size_t)(s * p.rows + row) * pitch + c * 16) =
+                make_uint4(w[s][0], w[s][1], w[s][2], w[s][3]);
+    }
+}
+
 // ---- kernel 1: router, choice, and the activations of the picked experts ----
-template <int WT, int XT, int NT>
+// NT n-tiles of 8 rows; STAGED: x in shared memory (else it is read from global memory as it goes).
+template <int WT, int XT, int NT, bool STAGED>
 __global__ void __launch_bounds__(kMoeThreads, 1) ll_moe_up_kernel(const __grid_constant__ MoeParams p)
 {
     using W = MoeW<WT>;
@@ -653,20 +889,18 @@ __global__ void __launch_bounds__(kMoeThreads, 1) ll_moe_up_kernel(const __grid_
     constexpr int NSH = XT == LL_T_F32 ? 3 : 2;  // bf16 terms of an activation
     extern __shared__ __align__(128) uint8_t moe_smem_raw[];
     uint8_t *smem = moe_smem_raw;
-    const MoeSmem L = moe_smem(p, true, NT);
+    const MoeSmem L = moe_smem(p, true);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    uint32_t *misc = reinterpret_cast<uint32_t *>(smem + L.misc);
-    volatile uint32_t *fail = misc;
-    const MoeRing ring = {smem_u32(smem), smem_u32(smem + L.bars), p.stages};
-    if (tid == 0) {
-        misc[0] = 0;
-        moe_ring_init(ring);
-    }
+    const uint32_t *misc = reinterpret_cast<const uint32_t *>(smem + L.misc);
     griddep_wait();
     griddep_launch_dependents();
-    __syncthreads();
+    if constexpr (STAGED)
+        moe_stage_x<WT, XT>(p, smem + L.x);
     moe_logits<XT, NT>(p, smem, L);
-    moe_pick(p, smem, L);
+    if (p.experts <= 64)
+        moe_pick<2>(p, smem, L);
+    else
+        moe_pick<LL_MOE_MAX_EXPERTS / 32>(p, smem, L);
     const int n_pairs = p.rows * p.top_k;
     if (blockIdx.x == 0) {
         for (int i = tid; i < n_pairs; i += kMoeThreads) {
@@ -684,125 +918,101 @@ __global__ void __launch_bounds__(kMoeThreads, 1) ll_moe_up_kernel(const __grid_
     const uint16_t *act_e = reinterpret_cast<const uint16_t *>(smem + L.act_e);
     const uint16_t *act_off = reinterpret_cast<const uint16_t *>(smem + L.act_off);
     const uint16_t *pairs = reinterpret_cast<const uint16_t *>(smem + L.pairs);
-    const int na = (int)misc[1], F = p.inter, H = p.hidden;
+    const int na = (int)misc[0], F = p.inter, H = p.hidden;
 
-    // Tiles of ch channels (at most 8 gated, 16 not), as many rounds over the CTAs as the widest tile
-    // needs and ch as small as keeps that number, so that the CTAs' shares are even.
-    const int ch_max = p.gated ? 8 : 16, G = (int)gridDim.x;
-    const int rounds = (int)(((long long)na * F + (long long)ch_max * G - 1) / ((long long)ch_max * G));
-    int ch = min(ch_max, max(1, (int)(((long long)na * F + (long long)rounds * G - 1) / ((long long)rounds * G))));
-    while (ch < ch_max && (long long)na * ((F + ch - 1) / ch) > (long long)rounds * G)
+    // Tiles of ch channels (at most 8 gated, 16 not): as many rounds over the warps as the widest tile
+    // needs, and ch as small as keeps that number, so that the warps' shares are even.
+    const int ch_max = p.gated ? 8 : 16, G = (int)gridDim.x * kMoeWarps, me = (int)blockIdx.x * kMoeWarps + warp;
+    const int all = na * F;  // at most LL_MOE_MAX_ROWS LL_MOE_MAX_TOPK LL_MOE_MAX_DIM = 2^25
+    const int slots = (all + ch_max * G - 1) / (ch_max * G) * G;
+    int ch = min(ch_max, (all + slots - 1) / slots);
+    int per_e = (F + ch - 1) / ch;
+    if (ch < ch_max && na * per_e > slots) {  // every expert's last tile is short
         ++ch;
-    const int per_e = (F + ch - 1) / ch;
-    const long long total = (long long)na * per_e;
-    const int lo = (int)(total * blockIdx.x / G), hi = (int)(total * (blockIdx.x + 1) / G);
-    const size_t row_bytes = (size_t)H * W::BYTES;
-    // weight row r of a tile (nullptr: none), and its channel
-    auto row_at = [&](int a, int f0, int r, int &f) -> const uint8_t * {
-        const bool up = p.gated && r >= 8;
-        const int i = up ? r - 8 : r;
-        f = f0 + i;
-        if (i >= ch || f >= F)
-            return nullptr;
-        return (up ? p.wu : p.wg) + ((size_t)act_e[a] * F + f) * row_bytes;
-    };
-    uint32_t it = 0;
-    if (warp == kMoeWarps) {
-        if (p.up_ring) {
-            for (int tile = lo; tile < hi; ++tile) {
-                const int a = tile / per_e, f0 = (tile - a * per_e) * ch;
-                int f;
-                const uint8_t *src = lane < 16 ? row_at(a, f0, lane, f) : nullptr;
-                const int n_rows = __popc(__ballot_sync(0xffffffffu, src != nullptr));
-                if (!moe_copy_rows(p, ring, src, (int)row_bytes, n_rows, it, fail))
-                    break;
-            }
-            if (lane == 0)
-                moe_drain(p, ring, it);
-        }
-    } else {
-        bool ok = true;
-        int buf = 0;
-        for (int tile = lo; tile < hi; ++tile, buf ^= 1) {
-            const int a = tile / per_e, f0 = (tile - a * per_e) * ch, e = act_e[a];
-            const int pos0 = act_off[a], cnt = act_off[a + 1] - pos0, ntc = (cnt + 7) >> 3;
-            const uint8_t *xrow[NT];
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-                xrow[nt] = static_cast<const uint8_t *>(p.x) +
-                           (size_t)(pairs[pos0 + min(nt * 8 + g, cnt - 1)] & 0xff) * p.ldx * X::BYTES;
-            // rows past the tile's end: any row of the tile (their sums are not used)
-            int fa, fb;
-            const uint8_t *g0 = row_at(a, f0, g, fa), *g1 = row_at(a, f0, g + 8, fb);
-            const uint8_t *first = row_at(a, f0, 0, fb);
-            const int c0 = g0 ? f0 + g : f0;
-            const int c1 = p.gated ? c0 : (g1 ? f0 + g + 8 : f0);
-            g0 = g0 ? g0 : first;
-            g1 = g1 ? g1 : first;
-            const float *sc0 = nullptr, *sc1 = nullptr;
-            if constexpr (WT == LL_W_F8) {
-                const int kb = (H + kF8Block - 1) / kF8Block, fb_n = (F + kF8Block - 1) / kF8Block;
-                sc0 = p.sg + ((size_t)e * fb_n + c0 / kF8Block) * kb;
-                sc1 = (p.gated ? p.su : p.sg) + ((size_t)e * fb_n + c1 / kF8Block) * kb;
-            }
-            float acc[NT][4];
-            ok = moe_rows<WT, X::NS, NT>(p, ring, smem, p.up_ring != 0, g0, g1, H, sc0, sc1, ntc, it, ok, fail, acc,
-                                         [&](int nt, int k, int n, uint32_t(&b)[X::NS][W::EP / 2]) {
-                                             X::template load<W::EP>(xrow[nt], k, n, p.x_vec, b);
-                                         });
-            float4 *red = reinterpret_cast<float4 *>(smem + L.red) + buf * (kMoeWarps * NT * 32);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-                if (nt < ntc)
-                    red[(warp * NT + nt) * 32 + lane] = make_float4(acc[nt][0], acc[nt][1], acc[nt][2], acc[nt][3]);
-            moe_bar();
-            if (ok && warp < ntc) {  // warp nt: the n-tile's sums over the warps, in their order
-                float4 v = red[warp * 32 + lane];
-#pragma unroll
-                for (int w = 1; w < kMoeWarps; ++w) {
-                    const float4 q = red[(w * NT + warp) * 32 + lane];
-                    v.x += q.x, v.y += q.y, v.z += q.z, v.w += q.w;
-                }
-                if constexpr (WT == LL_W_I8) {
-                    const float q0 = __ldg(p.sg + (size_t)e * F + c0);
-                    const float q1 = __ldg((p.gated ? p.su : p.sg) + (size_t)e * F + c1);
-                    v.x *= q0, v.y *= q0, v.z *= q1, v.w *= q1;
-                }
-                const int c = warp * 8 + 2 * t;  // columns c and c + 1 of the expert's rows
-                auto put = [&](int col, int f, float val) {
-                    __nv_bfloat16 *h = p.hid + (size_t)(pos0 + col) * p.hid_ld + f;
-                    uint32_t w[NSH];
-                    split_pair<NSH>(val, 0.0f, w);
-#pragma unroll
-                    for (int s = 0; s < NSH; ++s)
-                        h[(size_t)s * p.hid_plane] = __ushort_as_bfloat16((unsigned short)(w[s] & 0xffffu));
-                };
-                if (p.gated) {
-                    if (g < ch && f0 + g < F) {
-                        if (c < cnt)
-                            put(c, f0 + g, ops_act(v.x, p.act) * v.z);
-                        if (c + 1 < cnt)
-                            put(c + 1, f0 + g, ops_act(v.y, p.act) * v.w);
-                    }
-                } else {
-                    if (g < ch && f0 + g < F) {
-                        if (c < cnt)
-                            put(c, f0 + g, ops_act(v.x, p.act));
-                        if (c + 1 < cnt)
-                            put(c + 1, f0 + g, ops_act(v.y, p.act));
-                    }
-                    if (g + 8 < ch && f0 + g + 8 < F) {
-                        if (c < cnt)
-                            put(c, f0 + g + 8, ops_act(v.z, p.act));
-                        if (c + 1 < cnt)
-                            put(c + 1, f0 + g + 8, ops_act(v.w, p.act));
-                    }
-                }
-            }
-        }
+        per_e = (F + ch - 1) / ch;
     }
-    __syncwarp();
+    const int total = na * per_e, base = total / G, rest = total - base * G;
+    const int lo = me * base + min(me, rest), hi = lo + base + (me < rest ? 1 : 0);
+    const size_t row_bytes = (size_t)H * W::BYTES;
+    // Rows of a tile's stage: its gate rows, then (gated) the up rows of the same channels.
+    auto tile_at = [&](int q, const uint8_t *&s0, const uint8_t *&s1, int &half, int &have) {
+        const int tile = lo + q, a = tile / per_e, f0 = (tile - a * per_e) * ch;
+        const size_t at = ((size_t)act_e[a] * F + f0) * row_bytes;
+        s0 = p.wg + at;
+        s1 = p.wu + (p.gated ? at : 0);
+        half = ch;
+        have = min(ch, F - f0);
+    };
+    const uint8_t *stages = smem + warp * (kMoeStages * kMoeStage);
+    MoeRing ring = {};
+    ring.base = smem_u32(stages);
+    ring.shape(p.gated ? 2 * ch : ch);
+    ring.grain = p.up_grain;
+    ring.n = hi - lo;
+    ring.row_bytes = (int)row_bytes;
+    // the rings' place still holds the logits' parts: the cluster's CTAs have read them
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    for (int s = 0; s < kMoeStages; ++s)
+        ring.feed(tile_at);
+    using Src = std::conditional_t<STAGED, MoeTerms<X::NS, true>, X>;
+    Src src;
+    if constexpr (STAGED) {
+        const int pitch = moe_x_pitch(H, W::BYTES);
+        src = {smem + L.x, (size_t)p.rows * (size_t)pitch, (uint32_t)pitch};
+    } else {
+        src = {static_cast<const uint8_t *>(p.x), (size_t)p.ldx * X::BYTES, H, p.x_vec != 0};
+    }
+    int slot = 0;
+    for (int tile = lo; tile < hi; ++tile) {
+        const int a = tile / per_e, f0 = (tile - a * per_e) * ch, e = act_e[a];
+        const int pos0 = act_off[a], cnt = act_off[a + 1] - pos0, ntc = (cnt + 7) >> 3;
+        uint32_t xrow[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+            xrow[nt] = pairs[pos0 + min(nt * 8 + g, cnt - 1)] & 0xffu;
+        // rows past the tile's end: its last one again (their sums are not used)
+        const int chs = min(ch, F - f0), i0 = min(g, chs - 1);
+        const int c0 = f0 + i0, c1 = p.gated ? c0 : f0 + min(g + 8, chs - 1);
+        const int i1 = p.gated ? ch + i0 : c1 - f0;
+        const float *sc0 = nullptr, *sc1 = nullptr;
+        if constexpr (WT == LL_W_F8) {
+            const int kb = (H + kF8Block - 1) / kF8Block, fb = (F + kF8Block - 1) / kF8Block;
+            sc0 = p.sg + ((size_t)e * fb + c0 / kF8Block) * kb;
+            sc1 = (p.gated ? p.su : p.sg) + ((size_t)e * fb + c1 / kF8Block) * kb;
+        }
+        float acc[NT][4];
+        moe_tile<WT, NT>(ring, stages, slot, tile_at, i0, i1, H, sc0, sc1, ntc, src, xrow, acc);
+        float q0 = 1.0f, q1 = 1.0f;
+        if constexpr (WT == LL_W_I8) {
+            q0 = __ldg(p.sg + (size_t)e * F + c0);
+            q1 = __ldg((p.gated ? p.su : p.sg) + (size_t)e * F + c1);
+        }
+        // An activation into its planes, in the order that kernel 2 wants; behind the last one zeros up
+        // to a whole step.
+        auto put = [&](int col, int f, float val) {
+            const int at = W::PERM ? (f & ~3) | ((f & 1) << 1) | ((f >> 1) & 1) : f;
+            __nv_bfloat16 *h = p.hid + (size_t)(pos0 + col) * p.hid_ld + at;
+            uint32_t w[NSH];
+            split_pair<NSH>(W::PERM ? val * kMoeF8Up : val, 0.0f, w);
+#pragma unroll
+            for (int s = 0; s < NSH; ++s)
+                h[(size_t)s * p.hid_plane] = __ushort_as_bfloat16((unsigned short)(w[s] & 0xffffu));
+        };
+        if (f0 + ch >= F)
+            for (int i = lane; i < cnt * (p.hid_ld - F); i += 32)
+                put(i / (p.hid_ld - F), F + i % (p.hid_ld - F), 0.0f);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int c = nt * 8 + 2 * t + j;  // column: one of the expert's rows of x
+                const float v0 = acc[nt][j] * q0, v1 = acc[nt][2 + j] * q1;
+                if (c < cnt && g < chs)
+                    put(c, f0 + g, p.gated ? ops_act(v0, p.act) * v1 : ops_act(v0, p.act));
+                if (!p.gated && c < cnt && g + 8 < chs)
+                    put(c, f0 + g + 8, ops_act(v1, p.act));
+            }
+    }
 }
 
 // ---- kernel 2: down projection and the weighted sum ----
@@ -812,16 +1022,10 @@ __global__ void __launch_bounds__(kMoeThreads, 1) ll_moe_down_kernel(const __gri
     using W = MoeW<WT>;
     extern __shared__ __align__(128) uint8_t moe_smem_raw[];
     uint8_t *smem = moe_smem_raw;
-    const MoeSmem L = moe_smem(p, false, NT);
+    const MoeSmem L = moe_smem(p, false);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    uint32_t *misc = reinterpret_cast<uint32_t *>(smem + L.misc);
-    volatile uint32_t *fail = misc;
-    const MoeRing ring = {smem_u32(smem), smem_u32(smem + L.bars), p.stages};
-    if (tid == 0) {
-        misc[0] = 0;
-        moe_ring_init(ring);
-    }
-    float *part = reinterpret_cast<float *>(smem + L.red);  // [warp][row][16 channels]
+    const uint32_t *misc = reinterpret_cast<const uint32_t *>(smem + L.misc);
+    float *part = reinterpret_cast<float *>(smem + L.part);  // [warp][row][16 channels]
     for (int i = tid; i < kMoeWarps * p.rows * 16; i += kMoeThreads)
         part[i] = 0.0f;
     griddep_wait();
@@ -836,110 +1040,98 @@ __global__ void __launch_bounds__(kMoeThreads, 1) ll_moe_down_kernel(const __gri
     const uint16_t *act_e = reinterpret_cast<const uint16_t *>(smem + L.act_e);
     const uint16_t *act_off = reinterpret_cast<const uint16_t *>(smem + L.act_off);
     const uint16_t *pairs = reinterpret_cast<const uint16_t *>(smem + L.pairs);
-    const int na = (int)misc[1], F = p.inter, H = p.hidden, G = (int)gridDim.x;
+    const int na = (int)misc[0], F = p.inter, H = p.hidden, G = (int)gridDim.x;
     const int rounds = (H + 16 * G - 1) / (16 * G), R = (H + rounds * G - 1) / (rounds * G);
     const size_t row_bytes = (size_t)F * W::BYTES;
-    uint32_t it = 0;
-    if (warp == kMoeWarps) {
-        if (p.down_ring) {
-            bool ok = true;
-            for (int n0 = (int)blockIdx.x * R; n0 < H && ok; n0 += G * R) {
-                const int n_rows = min(R, H - n0);
-                for (int a = 0; a < na && ok; ++a) {
-                    const uint8_t *src =
-                        lane < n_rows ? p.wd + ((size_t)act_e[a] * H + n0 + lane) * row_bytes : nullptr;
-                    ok = moe_copy_rows(p, ring, src, (int)row_bytes, n_rows, it, fail);
-                }
+    // The CTA's R channels and the picked experts are shared out over the warps as (expert, rs
+    // channels), rs as large as leaves every warp something to do.
+    int rs = R;
+    while (rs > 1 && (R + rs - 1) / rs * na < kMoeWarps)
+        rs = (rs + 1) / 2;
+    const int subs = (R + rs - 1) / rs, units = subs * na;
+    const int mine_n = units > warp ? (units - warp + kMoeWarps - 1) / kMoeWarps : 0;  // of this warp, per item
+    const int first = (int)blockIdx.x * R, items = first < H ? (H - first + G * R - 1) / (G * R) : 0;
+    auto tile_at = [&](int q, const uint8_t *&s0, const uint8_t *&s1, int &half, int &have) {
+        const int item = q / mine_n, u = warp + (q - item * mine_n) * kMoeWarps;
+        const int a = u / subs, r = (u - a * subs) * rs, n = first + item * G * R + r;
+        s0 = s1 = p.wd + ((size_t)act_e[a] * H + min(n, H - 1)) * row_bytes;
+        half = rs;
+        have = min(min(rs, R - r), H - n);
+    };
+    const uint8_t *stages = smem + warp * (kMoeStages * kMoeStage);
+    MoeRing ring = {};
+    ring.base = smem_u32(stages);
+    ring.shape(rs);
+    ring.grain = p.down_grain;
+    ring.n = items * mine_n;
+    ring.row_bytes = (int)row_bytes;
+    for (int s = 0; s < kMoeStages; ++s)
+        ring.feed(tile_at);
+    const MoeTerms<NSH, false> src = {reinterpret_cast<const uint8_t *>(p.hid), (size_t)p.hid_plane * 2,
+                                      (uint32_t)p.hid_ld * 2u};
+    int slot = 0;
+    float *mine = part + warp * p.rows * 16;
+    for (int item = 0; item < items; ++item) {
+        const int n0 = first + item * G * R, n_rows = min(R, H - n0);
+        for (int u = warp; u < units; u += kMoeWarps) {
+            const int a = u / subs, rr = (u - a * subs) * rs;
+            const int e = act_e[a], pos0 = act_off[a], cnt = act_off[a + 1] - pos0, ntc = (cnt + 7) >> 3;
+            uint32_t hrow[NT];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+                hrow[nt] = (uint32_t)(pos0 + min(nt * 8 + g, cnt - 1));
+            // rows past the end: the last one again (their sums are not used; none at all: row n0)
+            const int last = max(0, min(rs, n_rows - rr) - 1), i0 = min(g, last), i1 = min(g + 8, last);
+            const int c0 = min(n0 + rr + i0, H - 1), c1 = min(n0 + rr + i1, H - 1);
+            const float *sc0 = nullptr, *sc1 = nullptr;
+            if constexpr (WT == LL_W_F8) {
+                const int kb = (F + kF8Block - 1) / kF8Block, hb = (H + kF8Block - 1) / kF8Block;
+                sc0 = p.sd + ((size_t)e * hb + c0 / kF8Block) * kb;
+                sc1 = p.sd + ((size_t)e * hb + c1 / kF8Block) * kb;
             }
-            if (lane == 0)
-                moe_drain(p, ring, it);
-        }
-    } else {
-        bool ok = true;
-        float *mine = part + warp * p.rows * 16;
-        for (int n0 = (int)blockIdx.x * R; n0 < H; n0 += G * R) {
-            const int n_rows = min(R, H - n0);
-            const int c0 = n0 + min(g, n_rows - 1), c1 = n0 + min(g + 8, n_rows - 1);
-            for (int a = 0; a < na; ++a) {
-                const int e = act_e[a], pos0 = act_off[a], cnt = act_off[a + 1] - pos0, ntc = (cnt + 7) >> 3;
-                const __nv_bfloat16 *hrow[NT];
+            float acc[NT][4];
+            moe_tile<WT, NT>(ring, stages, slot, tile_at, i0, i1, F, sc0, sc1, ntc, src, hrow, acc);
+            float q0 = 1.0f, q1 = 1.0f;
+            if constexpr (WT == LL_W_I8) {
+                q0 = __ldg(p.sd + (size_t)e * H + c0);
+                q1 = __ldg(p.sd + (size_t)e * H + c1);
+            }
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-                    hrow[nt] = p.hid + (size_t)(pos0 + min(nt * 8 + g, cnt - 1)) * p.hid_ld;
-                const uint8_t *g0 = p.wd + ((size_t)e * H + c0) * row_bytes, *g1 = p.wd + ((size_t)e * H + c1) * row_bytes;
-                const float *sc0 = nullptr, *sc1 = nullptr;
-                if constexpr (WT == LL_W_F8) {
-                    const int kb = (F + kF8Block - 1) / kF8Block, hb = (H + kF8Block - 1) / kF8Block;
-                    sc0 = p.sd + ((size_t)e * hb + c0 / kF8Block) * kb;
-                    sc1 = p.sd + ((size_t)e * hb + c1 / kF8Block) * kb;
-                }
-                float acc[NT][4];
-                ok = moe_rows<WT, NSH, NT>(
-                    p, ring, smem, p.down_ring != 0, g0, g1, F, sc0, sc1, ntc, it, ok, fail, acc,
-                    [&](int nt, int k, int n, uint32_t(&b)[NSH][W::EP / 2]) {
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int s = 0; s < NSH; ++s) {
-                            const __nv_bfloat16 *q = hrow[nt] + (size_t)s * p.hid_plane + k;
-#pragma unroll
-                            for (int i = 0; i < W::EP / 8; ++i) {
-                                uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                                if (n >= 8 * (i + 1)) {
-                                    v = __ldcg(reinterpret_cast<const uint4 *>(q) + i);
-                                } else if (n > 8 * i) {  // the row's last values
-                                    uint32_t h[4] = {0, 0, 0, 0};
-#pragma unroll
-                                    for (int j = 0; j < 8; ++j)
-                                        if (8 * i + j < n)
-                                            h[j / 2] |= (uint32_t)__ldcg(reinterpret_cast<const unsigned short *>(q) +
-                                                                         8 * i + j)
-                                                        << (16 * (j & 1));
-                                    v = make_uint4(h[0], h[1], h[2], h[3]);
-                                }
-                                b[s][4 * i] = v.x, b[s][4 * i + 1] = v.y, b[s][4 * i + 2] = v.z, b[s][4 * i + 3] = v.w;
-                            }
-                        }
-                    });
-                if constexpr (WT == LL_W_I8) {
-                    const float q0 = __ldg(p.sd + (size_t)e * H + c0), q1 = __ldg(p.sd + (size_t)e * H + c1);
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-                        acc[nt][0] *= q0, acc[nt][1] *= q0, acc[nt][2] *= q1, acc[nt][3] *= q1;
-                }
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const int c = nt * 8 + 2 * t + j;
-                        if (c < cnt) {
-                            const int pr = pairs[pos0 + c], row = pr & 0xff;
-                            const float w = probs[row * p.top_k + (pr >> 8)];
-                            mine[row * 16 + g] = fmaf(w, acc[nt][j], mine[row * 16 + g]);
-                            mine[row * 16 + g + 8] = fmaf(w, acc[nt][2 + j], mine[row * 16 + g + 8]);
-                        }
+                for (int j = 0; j < 2; ++j) {
+                    const int c = nt * 8 + 2 * t + j;
+                    if (c < cnt) {
+                        const int pr = pairs[pos0 + c], row = pr & 0xff;
+                        const float w = probs[row * p.top_k + (pr >> 8)];
+                        if (g < min(rs, n_rows - rr))
+                            mine[row * 16 + rr + g] = fmaf(w, acc[nt][j] * q0, mine[row * 16 + rr + g]);
+                        if (g + 8 < min(rs, n_rows - rr))
+                            mine[row * 16 + rr + g + 8] = fmaf(w, acc[nt][2 + j] * q1, mine[row * 16 + rr + g + 8]);
                     }
-                __syncwarp();  // another lane may add to the same place for the next expert
-            }
-            moe_bar();
-            for (int i = tid; i < p.rows * 16; i += kMoeWarps * 32) {
-                const int row = i >> 4, r = i & 15;
-                float v = 0.0f;
-#pragma unroll
-                for (int w = 0; w < kMoeWarps; ++w) {
-                    v += part[w * p.rows * 16 + i];
-                    part[w * p.rows * 16 + i] = 0.0f;
                 }
-                if (ok && r < n_rows) {
-                    const size_t o = (size_t)row * p.ldy + n0 + r;
-                    if (p.x_type == LL_T_F32)
-                        static_cast<float *>(p.y)[o] = v;
-                    else if (p.x_type == LL_T_BF16)
-                        static_cast<__nv_bfloat16 *>(p.y)[o] = __float2bfloat16_rn(v);
-                    else
-                        static_cast<__half *>(p.y)[o] = __float2half_rn(v);
-                }
-            }
-            moe_bar();
+            __syncwarp();  // another lane may add to the same place for the next expert
         }
+        __syncthreads();
+        for (int i = tid; i < p.rows * 16; i += kMoeThreads) {
+            const int row = i >> 4, r = i & 15;
+            float v = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kMoeWarps; ++w) {
+                v += part[w * p.rows * 16 + i];
+                part[w * p.rows * 16 + i] = 0.0f;
+            }
+            if (r < n_rows) {
+                const size_t o = (size_t)row * p.ldy + n0 + r;
+                if (p.x_type == LL_T_F32)
+                    static_cast<float *>(p.y)[o] = v;
+                else if (p.x_type == LL_T_BF16)
+                    static_cast<__nv_bfloat16 *>(p.y)[o] = __float2bfloat16_rn(v);
+                else
+                    static_cast<__half *>(p.y)[o] = __float2half_rn(v);
+            }
+        }
+        __syncthreads();
     }
 }
 
@@ -949,6 +1141,13 @@ int launch_moe_i8(MoeParams &p, int device, cudaStream_t st);
 int launch_moe_f8(MoeParams &p, int device, cudaStream_t st);
 
 constexpr int kMoeSmemCap = 226 * 1024;
+
+template <int WT, int XT>
+int moe_x_bytes(const MoeParams &p)
+{
+    const long long b = (long long)moe_terms(XT) * p.rows * moe_x_pitch(p.hidden, MoeW<WT>::BYTES);
+    return (int)std::min<long long>(b, 1 << 24);
+}
 
 // One kernel with its own dynamic shared memory; `cluster` CTAs per cluster (0: none).
 inline int moe_launch(const void *fn, bool *ready, MoeParams &p, int smem, int grid, int cluster, bool dependent,
@@ -1007,50 +1206,49 @@ inline int moe_clusters(const void *fn, int *n)
     return LL_OK;
 }
 
-template <int WT, int XT, int NT>
+template <int WT, int XT, int NT, bool STAGED>
 int launch_moe_typed(MoeParams &p, int device, cudaStream_t st)
 {
     static bool up_ready[kOpsMaxDevices], down_ready[kOpsMaxDevices];
     static int sm_count[kOpsMaxDevices], cluster_count[kOpsMaxDevices];
     constexpr int NSH = XT == LL_T_F32 ? 3 : 2;
+    const void *up = reinterpret_cast<const void *>(&ll_moe_up_kernel<WT, XT, NT, STAGED>);
+    const void *down = reinterpret_cast<const void *>(&ll_moe_down_kernel<WT, NSH, NT>);
     int sms = __atomic_load_n(&sm_count[device], __ATOMIC_ACQUIRE);
     if (sms == 0) {
         LL_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
         __atomic_store_n(&sm_count[device], sms, __ATOMIC_RELEASE);
     }
-    p.stages = 0;
-    const int rest_up = moe_smem(p, true, NT).total, rest_down = moe_smem(p, false, NT).total;
-    p.stages = std::min(kMoeMaxStages, (kMoeSmemCap - rest_up) / kMoeStage);
-    if (p.stages < 2) {
-        llh::set_error("ll_moe_forward: the router of %d experts x %d rows leaves no shared memory", p.experts, p.rows);
-        return LL_ERR_BAD_DESC;
-    }
-    // one wave of clusters: a GPC whose SMs are not a multiple of 8 leaves some out
+    // one wave of clusters: a GPC whose SMs are not a multiple of the cluster leaves some out
     int clusters = __atomic_load_n(&cluster_count[device], __ATOMIC_ACQUIRE);
     if (clusters == 0) {
-        LL_TRY(moe_clusters(reinterpret_cast<const void *>(&ll_moe_up_kernel<WT, XT, NT>), &clusters));
+        LL_TRY(moe_clusters(up, &clusters));
         __atomic_store_n(&cluster_count[device], clusters, __ATOMIC_RELEASE);
     }
-    const int grid_up = clusters * kMoeCluster;
-    LL_TRY(moe_launch(reinterpret_cast<const void *>(&ll_moe_up_kernel<WT, XT, NT>), up_ready, p,
-                      moe_smem(p, true, NT).total, grid_up, kMoeCluster, false, device, st));
-    p.stages = std::min(kMoeMaxStages, (kMoeSmemCap - rest_down) / kMoeStage);
-    const int grid_down = std::min(sms, p.hidden);
-    return moe_launch(reinterpret_cast<const void *>(&ll_moe_down_kernel<WT, NSH, NT>), down_ready, p,
-                      moe_smem(p, false, NT).total, grid_down, 0, true, device, st);
+    LL_TRY(moe_launch(up, up_ready, p, moe_smem(p, true).total + (STAGED ? moe_x_bytes<WT, XT>(p) : 0),
+                      clusters * kMoeCluster, kMoeCluster, false, device, st));
+    return moe_launch(down, down_ready, p, moe_smem(p, false).total, std::min(sms, p.hidden), 0, true, device, st);
+}
+
+// Up to 8 rows whose terms fit beside the rings take the kernel that stages x.
+template <int WT, int XT>
+int launch_moe_rows(MoeParams &p, int device, cudaStream_t st)
+{
+    if (p.rows <= 8 && moe_smem(p, true).total + moe_x_bytes<WT, XT>(p) <= kMoeSmemCap)
+        return launch_moe_typed<WT, XT, 1, true>(p, device, st);
+    return launch_moe_typed<WT, XT, 4, false>(p, device, st);
 }
 
 template <int WT>
 int launch_moe(MoeParams &p, int device, cudaStream_t st)
 {
-    const bool few = p.rows <= 8;
     switch (p.x_type) {
     case LL_T_BF16:
-        return few ? launch_moe_typed<WT, LL_T_BF16, 1>(p, device, st) : launch_moe_typed<WT, LL_T_BF16, 4>(p, device, st);
+        return launch_moe_rows<WT, LL_T_BF16>(p, device, st);
     case LL_T_F16:
-        return few ? launch_moe_typed<WT, LL_T_F16, 1>(p, device, st) : launch_moe_typed<WT, LL_T_F16, 4>(p, device, st);
+        return launch_moe_rows<WT, LL_T_F16>(p, device, st);
     default:
-        return few ? launch_moe_typed<WT, LL_T_F32, 1>(p, device, st) : launch_moe_typed<WT, LL_T_F32, 4>(p, device, st);
+        return launch_moe_rows<WT, LL_T_F32>(p, device, st);
     }
 }
 

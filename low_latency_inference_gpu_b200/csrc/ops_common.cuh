@@ -8,6 +8,7 @@
 #include <cstdint>
 
 #include "common.h"
+#include "tc_layer.cuh"
 
 namespace llk {
 
@@ -31,6 +32,27 @@ __device__ __forceinline__ float ops_act(float v, int act)
     if (act == LL_ACT_SILU)
         return v / (1.0f + expf(-v));
     return v;
+}
+
+// Warp-collective bounded wait on a barrier of this CTA.  The timer is read only when the first look
+// fails: reading it takes about a microsecond, more than most of these waits.
+__device__ __forceinline__ bool ops_wait_warp(uint32_t bar, uint32_t parity, unsigned long long bound_ns,
+                                              volatile uint32_t *fail, unsigned *status, uint32_t role)
+{
+#pragma unroll 1
+    for (int i = 0; i < 16; ++i) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done)
+            : "r"(bar), "r"(parity)
+            : "memory");
+        if (__all_sync(0xffffffffu, done != 0u))
+            return true;
+    }
+    return tc_wait_warp(bar, parity, bound_ns, fail, status, role);
 }
 
 // ---- e4m3 ----
