@@ -252,12 +252,24 @@ __global__ void __launch_bounds__(kDsThreads, 1) ll_dense_fp8_kernel(const __gri
         for (int j = 0; j < nkb; ++j) {
             if (j % kDsScaleKb == 0) {  // the next blocks' scales, a copy per warp: no warp waits for another
                 const int n = min(kDsScaleKb, nkb - j);
+                float f[kDsScaleKb];
+#pragma unroll
+                for (int jj = 0; jj < kDsScaleKb; ++jj)
+                    f[jj] = jj < n ? __ldg(sw + j + jj) : 0.0f;
                 __syncwarp();
-                for (int i = lane; i < n * NT; i += 32) {
-                    const int c = i / n, jj = i - c * n;  // consecutive lanes: consecutive blocks of a row
+#pragma unroll
+                for (int c0 = 0; c0 < NT; c0 += 32) {  // a row's blocks per lane, all loads at once
+                    const int c = c0 + lane;
                     const long long row = t0 + c;
-                    w_sc[jj * NT + c] =
-                        row < p.rows ? __ldg(p.sx + row * p.nkb + kb0 + j + jj) * __ldg(sw + j + jj) : 0.0f;
+                    const float *px = p.sx + row * p.nkb + kb0 + j;
+                    float v[kDsScaleKb];
+#pragma unroll
+                    for (int jj = 0; jj < kDsScaleKb; ++jj)
+                        v[jj] = c < NT && row < p.rows && jj < n ? __ldg(px + jj) : 0.0f;
+                    if (c < NT)
+#pragma unroll
+                        for (int jj = 0; jj < kDsScaleKb; ++jj)
+                            w_sc[jj * NT + c] = v[jj] * f[jj];
                 }
                 __syncwarp();
             }
@@ -339,6 +351,361 @@ __global__ void __launch_bounds__(kDsThreads, 1) ll_dense_fp8_kernel(const __gri
         cluster_sync();  // nobody leaves while a peer may still read its partial tile
 }
 
+// ---------------------------------------------------------------------------------------------
+// Many rows: D[128 rows x 256 channels] = X tile . W tile^T on one persistent CTA per SM, lane = row.
+// A K block takes the tensor cores 512 cycles (128 x 256 x 128 at 8192 multiply-adds a cycle); its
+// way out (32 K values from TMEM, as many fused multiply-adds by the block's scales: one factor
+// per thread, sx of its row times sw of its 128 channels) takes the eight warps of the epilogue
+// about 300, so the two accumulators in turn keep the tensor cores fed.
+//   warp 0      TMA producer (X box 16 KB + W box 32 KB per K block, 4 stages)
+//   warp 1      TMEM allocation (all 512 columns); one thread issues the MMAs
+//   warps 4-11  warps 4-7 channels 0..127 of the tile, warps 8-11 the other 128: 128 sums per
+//               thread in registers; at a tile's end bias, activation and a staged store
+constexpr int kDlThreads = 384;
+constexpr int kDlM = 128, kDlN = 256, kDlStages = 4;
+constexpr int kDlStage = (kDlM + kDlN) * kF8Block;
+constexpr int kDlOut = 32 * 128;                             // staging of a warp: 32 rows of 128 bytes
+constexpr int kDlOffOut = kDlStages * kDlStage;
+constexpr int kDlOffBar = kDlOffOut + 8 * kDlOut;            // full[S], empty[S], accfull[2], accempty[2], done
+constexpr int kDlOffMisc = kDlOffBar + 8 * (2 * kDlStages + 5);
+constexpr int kDlAlloc = kDlOffMisc + 16 + 1024;
+static_assert(kDlAlloc <= 227 * 1024, "shared memory");
+
+// 32 lanes x 32 consecutive fp32 columns; the wait is separate.
+__device__ __forceinline__ void tc_ld_32cols_async(uint32_t taddr, uint32_t (&r)[32])
+{
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+}
+
+// Waits for the loads into r: the registers are operands, so that no use of them moves before the wait.
+__device__ __forceinline__ void tc_wait_ld_32(uint32_t (&r)[32])
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                   "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                   "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                   "+r"(r[30]), "+r"(r[31])
+                 :
+                 : "memory");
+}
+
+// acc += v * s for 32 columns, two at a time.
+__device__ __forceinline__ void fma_32cols(float *acc, const uint32_t (&v)[32], float s)
+{
+#pragma unroll
+    for (int i = 0; i < 32; i += 2)
+        asm("{\n\t.reg .b64 a, b, c;\n\t"
+            "mov.b64 a, {%0, %1};\n\t"
+            "mov.b64 b, {%2, %3};\n\t"
+            "mov.b64 c, {%4, %4};\n\t"
+            "fma.rn.f32x2 a, b, c, a;\n\t"
+            "mov.b64 {%0, %1}, a;\n\t}"
+            : "+f"(acc[i]), "+f"(acc[i + 1])
+            : "r"(v[i]), "r"(v[i + 1]), "f"(s));
+}
+
+// The warp's 32 rows x 32 columns (thread = row, in registers) through its staging tile (16-byte pieces,
+// piece j of row r at j ^ (r & 7)), so that 8 lanes hold 128 bytes of a row: there bias and
+// activation are applied, four values a lane at a time (one copy of the activation's code, where
+// one per register would stream tens of KB through the instruction cache), and the results
+// stored, or (e4m3) put back for the threads' group maxima.
+__device__ __forceinline__ void dl_store_32cols(const DenseF8Params &p, uint8_t *out, float *acc, long long row0, int c0)
+{
+    const int lane = threadIdx.x & 31, j = lane & 7, c = c0 + 4 * j, have = p.M - c;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        *reinterpret_cast<float4 *>(out + lane * 128 + ((i ^ (lane & 7)) << 4)) =
+            make_float4(acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]);
+    float bias[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        bias[e] = p.bias && e < have ? __ldg(p.bias + c + e) : 0.0f;
+    __syncwarp();
+#pragma unroll 1
+    for (int i = 0; i < 8; ++i) {
+        const int r = 4 * i + (lane >> 3);
+        float4 *at = reinterpret_cast<float4 *>(out + r * 128 + ((j ^ (r & 7)) << 4));
+        const float4 q = *at;
+        float v[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            v[e] = e < have ? ops_act(v[e] + bias[e], p.act) : 0.0f;
+        const long long row = row0 + r;
+        if (p.y_type == LL_T_F8) {
+            *at = make_float4(v[0], v[1], v[2], v[3]);
+        } else if (row < p.rows && have > 0) {
+            if (p.y_type == LL_T_F32) {
+                float *y = static_cast<float *>(p.y) + row * p.ldy + c;
+                if (have >= 4 && p.y_vec) {
+                    *reinterpret_cast<float4 *>(y) = make_float4(v[0], v[1], v[2], v[3]);
+                } else {
+                    for (int e = 0; e < 4; ++e)
+                        if (e < have)
+                            y[e] = v[e];
+                }
+            } else {
+                uint16_t h[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    h[e] = p.y_type == LL_T_BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v[e]))
+                                                 : __half_as_ushort(__float2half_rn(v[e]));
+                uint16_t *y = static_cast<uint16_t *>(p.y) + row * p.ldy + c;
+                if (have >= 4 && p.y_vec) {
+                    *reinterpret_cast<uint2 *>(y) =
+                        make_uint2((uint32_t)h[0] | ((uint32_t)h[1] << 16), (uint32_t)h[2] | ((uint32_t)h[3] << 16));
+                } else {
+                    for (int e = 0; e < 4; ++e)
+                        if (e < have)
+                            y[e] = h[e];
+                }
+            }
+        }
+    }
+    __syncwarp();
+    if (p.y_type == LL_T_F8) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float4 q = *reinterpret_cast<const float4 *>(out + lane * 128 + ((i ^ (lane & 7)) << 4));
+            acc[4 * i] = q.x, acc[4 * i + 1] = q.y, acc[4 * i + 2] = q.z, acc[4 * i + 3] = q.w;
+        }
+        __syncwarp();
+    }
+}
+
+// The same rows' 128 columns as e4m3: a thread has a whole group, so its scale is the thread's own.
+__device__ __forceinline__ void dl_store_e4m3(const DenseF8Params &p, uint8_t *out, const float (&acc)[128],
+                                              long long row0, int c0)
+{
+    const int lane = threadIdx.x & 31, mblocks = (p.M + kF8Block - 1) / kF8Block;
+    float amax = 0.0f, s, inv;
+#pragma unroll
+    for (int i = 0; i < 128; ++i)
+        amax = fmaxf(amax, fabsf(acc[i]));  // columns past M are zero
+    e4m3_scale(amax, false, s, inv);
+    if (row0 + lane < p.rows)
+        p.sy[(row0 + lane) * mblocks + c0 / kF8Block] = s;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        *reinterpret_cast<uint4 *>(out + lane * 128 + ((i ^ (lane & 7)) << 4)) =
+            make_uint4(group_e4m3x4(acc + 16 * i, false, s, inv), group_e4m3x4(acc + 16 * i + 4, false, s, inv),
+                       group_e4m3x4(acc + 16 * i + 8, false, s, inv), group_e4m3x4(acc + 16 * i + 12, false, s, inv));
+    __syncwarp();
+    const bool vec = (p.ldy & 15) == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0;
+#pragma unroll 1
+    for (int i = 0; i < 8; ++i) {
+        const int r = 4 * i + (lane >> 3), j = lane & 7, have = p.M - (c0 + 16 * j);
+        const uint8_t *at = out + r * 128 + ((j ^ (r & 7)) << 4);
+        if (row0 + r < p.rows && have > 0) {
+            uint8_t *y = static_cast<uint8_t *>(p.y) + (row0 + r) * p.ldy + c0 + 16 * j;
+            if (vec && have >= 16) {
+                *reinterpret_cast<uint4 *>(y) = *reinterpret_cast<const uint4 *>(at);
+            } else {
+                for (int e = 0; e < min(16, have); ++e)
+                    y[e] = at[e];
+            }
+        }
+    }
+    __syncwarp();
+}
+
+__global__ void __launch_bounds__(kDlThreads, 1) ll_dense_fp8_large_kernel(const __grid_constant__ DenseF8Params p)
+{
+    constexpr int S = kDlStages;
+    extern __shared__ uint8_t dl_smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(dl_smem_raw) + 1023) & ~uintptr_t(1023));
+    const uint32_t sbase = smem_u32(smem);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    uint32_t *misc = reinterpret_cast<uint32_t *>(smem + kDlOffMisc);
+    volatile uint32_t *fail = misc + 1;
+    auto bar = [&](int i) { return sbase + (uint32_t)kDlOffBar + 8u * (uint32_t)i; };
+    auto b_full = [&](int s) { return bar(s); };
+    auto b_empty = [&](int s) { return bar(S + s); };
+    auto b_accf = [&](int b) { return bar(2 * S + b); };
+    auto b_acce = [&](int b) { return bar(2 * S + 2 + b); };
+    const uint32_t b_done = bar(2 * S + 4);
+    const int mt_n = (p.rows + kDlM - 1) / kDlM, nt_n = (p.M + kDlN - 1) / kDlN, tiles = mt_n * nt_n;
+    // Tiles in bands of 16 row tiles, rows fastest: CTAs that run at once share rows of W and of x in L2.
+    auto tile_at = [&](int tile, int &mt, int &nt) {
+        const int band = tile / (16 * nt_n), first = band * 16, in = tile - band * 16 * nt_n;
+        const int h = min(16, mt_n - first);
+        nt = in / h;
+        mt = first + in - nt * h;
+    };
+
+    if (tid == 0) {
+        for (int s = 0; s < S; ++s) {
+            mbar_init(b_full(s), 1);
+            mbar_init(b_empty(s), 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(b_accf(b), 1);
+            mbar_init(b_acce(b), 8);
+        }
+        mbar_init(b_done, 1);
+        misc[1] = 0;
+        fence_mbar_init_cluster();
+        prefetch_tmap(&p.tm_w);
+        prefetch_tmap(&p.tm_x);
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                         sbase + (uint32_t)kDlOffMisc),
+                     "r"(512u)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = misc[0];
+    int issued = 0;
+
+    if (warp < 4) {
+        // 384 threads were launched with 168 registers each: 256 x 224 + 128 x 56 is just that
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp == 0) {
+            if (lane == 0) {
+                bool ok = true;
+                for (int tile = (int)blockIdx.x; tile < tiles && ok; tile += (int)gridDim.x) {
+                    int mt, nt;
+                    tile_at(tile, mt, nt);
+                    for (int kb = 0; kb < p.nkb; ++kb) {
+                        const int s = issued % S;
+                        if (issued >= S &&
+                            !tc_wait(b_empty(s), ((issued / S) - 1) & 1, p.wait_ns, fail, p.status, 1)) {
+                            ok = false;
+                            break;
+                        }
+                        mbar_arrive_expect_tx(b_full(s), kDlStage);
+                        tma_load_2d(sbase + s * kDlStage, &p.tm_x, kb * kF8Block, mt * kDlM, b_full(s));
+                        tma_load_2d(sbase + s * kDlStage + kDlM * kF8Block, &p.tm_w, kb * kF8Block, nt * kDlN, b_full(s));
+                        ++issued;
+                    }
+                }
+            }
+        } else if (warp == 1) {
+            if (lane == 0) {
+                constexpr uint32_t idesc = tc_idesc_e4m3(kDlN);
+                int g = 0;
+                bool ok = true;
+                for (int tile = (int)blockIdx.x; tile < tiles && ok; tile += (int)gridDim.x)
+                    for (int kb = 0; kb < p.nkb; ++kb, ++g) {
+                        const int s = g % S, b = g & 1;
+                        if ((g >= 2 && !tc_wait(b_acce(b), ((g / 2) - 1) & 1, p.wait_ns, fail, p.status, 2)) ||
+                            !tc_wait(b_full(s), (g / S) & 1, p.wait_ns, fail, p.status, 3)) {
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after();
+                        const uint32_t x = sbase + s * kDlStage, w = x + kDlM * kF8Block;
+#pragma unroll
+                        for (int kk = 0; kk < 4; ++kk)
+                            tc_mma_f8(tmem + (uint32_t)(b * kDlN), sw128_kmajor_desc(x + kk * 32),
+                                      sw128_kmajor_desc(w + kk * 32), idesc, kk != 0);
+                        tc_commit(b_empty(s));
+                        tc_commit(b_accf(b));
+                    }
+                tc_commit(b_done);
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        const int quad = warp & 3, half = (warp - 4) >> 2, mblocks = (p.M + kF8Block - 1) / kF8Block;
+        const uint32_t tq = tmem + ((uint32_t)(32 * quad) << 16) + (uint32_t)(half * 128);
+        uint8_t *out = smem + kDlOffOut + (warp - 4) * kDlOut;
+        int g = 0;
+        bool ok = true;
+        for (int tile = (int)blockIdx.x; tile < tiles && ok; tile += (int)gridDim.x) {
+            int mt, nt;
+            tile_at(tile, mt, nt);
+            const long long row0 = (long long)mt * kDlM + 32 * quad;
+            const int c0 = nt * kDlN + half * 128, block = c0 / kF8Block;
+            const float *sx = p.sx + min(row0 + lane, (long long)p.rows - 1) * p.nkb;
+            const float *sw = p.sw + (size_t)min(block, mblocks - 1) * p.nkb;
+            float acc[128];
+#pragma unroll
+            for (int i = 0; i < 128; ++i)
+                acc[i] = 0.0f;
+            float f[4], fn[4];  // the scales of four K blocks, and of the next four
+            auto load_scales = [&](int kb) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    fn[i] = kb + i < p.nkb ? __ldg(sx + kb + i) * __ldg(sw + kb + i) : 0.0f;
+            };
+            load_scales(0);
+            for (int kb0 = 0; kb0 < p.nkb && ok; kb0 += 4) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    f[i] = fn[i];
+                load_scales(kb0 + 4);
+                for (int i = 0; i < 4 && kb0 + i < p.nkb; ++i, ++g) {
+                    const int b = g & 1;
+                    if (!ops_wait_warp(b_accf(b), (g / 2) & 1, p.wait_ns, fail, p.status, 4)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const float s = i == 0 ? f[0] : i == 1 ? f[1] : i == 2 ? f[2] : f[3];
+                    const uint32_t at = tq + (uint32_t)(b * kDlN);
+                    uint32_t v0[32], v1[32];
+                    tc_ld_32cols_async(at, v0);
+                    tc_wait_ld_32(v0);
+                    tc_ld_32cols_async(at + 32, v1);
+                    fma_32cols(acc, v0, s);
+                    tc_wait_ld_32(v1);
+                    tc_ld_32cols_async(at + 64, v0);
+                    fma_32cols(acc + 32, v1, s);
+                    tc_wait_ld_32(v0);
+                    tc_ld_32cols_async(at + 96, v1);
+                    fma_32cols(acc + 64, v0, s);
+                    tc_wait_ld_32(v1);
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0)
+                        mbar_arrive_local(b_acce(b));
+                    fma_32cols(acc + 96, v1, s);
+                }
+            }
+            if (ok && c0 < p.M) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    dl_store_32cols(p, out, acc + 32 * i, row0, c0 + 32 * i);
+                if (p.y_type == LL_T_F8)
+                    dl_store_e4m3(p, out, acc, row0, c0);
+            }
+        }
+    }
+    if (warp == 0 && lane == 0 && *fail) {  // loads in flight land before the shared memory is given back
+        for (int j = max(0, issued - S); j < issued; ++j) {
+            const uint64_t w0 = globaltimer();
+            while (!mbar_try_wait(b_full(j % S), (j / S) & 1) && globaltimer() - w0 < p.wait_ns) {
+            }
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        if (lane == 0) {
+            const uint64_t w0 = globaltimer();
+            while (!mbar_try_wait(b_done, 0) && globaltimer() - w0 < p.wait_ns) {
+            }
+        }
+        __syncwarp();
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
 }  // namespace llk
 
 namespace {
@@ -382,6 +749,22 @@ int launch_few(const DenseF8Params &p, int splits, int device, cudaStream_t st)
     cfg.numAttrs = 1;
     void *args[] = {const_cast<DenseF8Params *>(&p)};
     LL_CUDA_TRY(cudaLaunchKernelExC(&cfg, fn, args));
+    return LL_OK;
+}
+
+int launch_many(const DenseF8Params &p, int device, cudaStream_t st)
+{
+    static int sm_count[kOpsMaxDevices];
+    const void *fn = reinterpret_cast<const void *>(&ll_dense_fp8_large_kernel);
+    int sms = __atomic_load_n(&sm_count[device], __ATOMIC_ACQUIRE);
+    if (sms == 0) {
+        LL_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kDlAlloc));
+        LL_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
+        __atomic_store_n(&sm_count[device], sms, __ATOMIC_RELEASE);
+    }
+    const long long tiles = (long long)((p.rows + kDlM - 1) / kDlM) * ((p.M + kDlN - 1) / kDlN);
+    ll_dense_fp8_large_kernel<<<(unsigned)std::min<long long>(tiles, sms), kDlThreads, kDlAlloc, st>>>(p);
+    LL_CUDA_TRY(cudaGetLastError());
     return LL_OK;
 }
 
@@ -448,18 +831,22 @@ extern "C" int ll_dense_fp8(const uint8_t *d_W, const float *d_sw, const float *
     p.y_vec = (ldy % 4 == 0 && (reinterpret_cast<uintptr_t>(d_y) % v4) == 0) ? 1 : 0;
     p.status = status;
     p.wait_ns = kOpsWaitNs;
-    const int nt = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
-    if (!f8_map(&p.tm_w, d_W, K, M, ldw, 128) || !f8_map(&p.tm_x, d_x, K, rows, ldx, nt)) {
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const long long large_tiles = (long long)((rows + kDlM - 1) / kDlM) * ((M + kDlN - 1) / kDlN);
+    const bool many = rows > 128 && large_tiles >= 74;
+    const int nt = many ? kDlM : rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+    if (!f8_map(&p.tm_w, d_W, K, M, ldw, many ? kDlN : 128) || !f8_map(&p.tm_x, d_x, K, rows, ldx, nt)) {
         llh::set_error("%s: the tensor maps could not be encoded", op);
         return LL_ERR_CUDA;
     }
+    if (many)
+        return launch_many(p, dev, st);
     // Splits: as many CTAs as SMs, each with two K blocks at least.
     const long long tiles = (long long)((M + 127) / 128) * ((rows + nt - 1) / nt);
     int splits = 1;
     while (splits < 8 && tiles * splits * 2 <= 148 && p.nkb >= splits * 4)
         splits *= 2;
     p.kb_split = (p.nkb + splits - 1) / splits;
-    const cudaStream_t st = static_cast<cudaStream_t>(stream);
     switch (nt) {
     case 16:
         return launch_few<16>(p, splits, dev, st);

@@ -320,7 +320,9 @@ class DenseCase:
 
 SHAPES = [(1, 16, 16), (1, 2048, 2048), (2, 128, 128), (7, 130, 260), (16, 64, 1000), (17, 200, 129), (32, 512, 4096),
           (33, 128, 640), (64, 384, 256), (65, 1000, 1100), (128, 257, 300), (129, 256, 512), (300, 520, 400),
-          (256, 2048, 2048), (640, 1280, 384)]
+          (256, 2048, 2048), (640, 1280, 384),
+          # enough tiles of 128 x 256 for the many-row kernel: whole ones, ragged ones, one K block and several
+          (1300, 1700, 200), (1280, 2048, 128), (2500, 1030, 700), (9601, 130, 1300)]
 
 
 @pytest.mark.gpu
