@@ -11,6 +11,7 @@
 
 #include "ops_common.cuh"
 #include "tc_layer.cuh"
+#include "tc_swap2.cuh"
 #include "tmap.h"
 
 namespace llk {
@@ -213,7 +214,7 @@ __global__ void __launch_bounds__(kDsThreads, 1) ll_dense_fp8_kernel(const __gri
         if (lane == 0) {
             for (int j = 0; j < nkb; ++j) {
                 const int s = j % S;
-                if (j >= S && !tc_wait(b_empty(s), ((j / S) - 1) & 1, p.wait_ns, fail, p.status, 1))
+                if (j >= S && !ops_wait(b_empty(s), ((j / S) - 1) & 1, p.wait_ns, fail, p.status, 1))
                     break;
                 mbar_arrive_expect_tx(b_full(s), L::STAGE);
                 tma_load_2d(sbase + s * L::STAGE, &p.tm_w, (kb0 + j) * kF8Block, m0, b_full(s));
@@ -226,9 +227,9 @@ __global__ void __launch_bounds__(kDsThreads, 1) ll_dense_fp8_kernel(const __gri
             constexpr uint32_t idesc = tc_idesc_e4m3(NT);
             for (int j = 0; j < nkb; ++j) {
                 const int s = j % S, b = j & 1;
-                if (j >= 2 && !tc_wait(b_acce(b), ((j / 2) - 1) & 1, p.wait_ns, fail, p.status, 2))
+                if (j >= 2 && !ops_wait(b_acce(b), ((j / 2) - 1) & 1, p.wait_ns, fail, p.status, 2))
                     break;
-                if (!tc_wait(b_full(s), (j / S) & 1, p.wait_ns, fail, p.status, 3))
+                if (!ops_wait(b_full(s), (j / S) & 1, p.wait_ns, fail, p.status, 3))
                     break;
                 tc_fence_after();
                 const uint32_t a = sbase + s * L::STAGE, x = a + L::WB;
@@ -342,8 +343,10 @@ __global__ void __launch_bounds__(kDsThreads, 1) ll_dense_fp8_kernel(const __gri
                 v[0] += q.x, v[1] += q.y, v[2] += q.z, v[3] += q.w;
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                v[i] = ops_act(v[i] + bias[i], p.act);
+            for (int i = 0; i < 4; ++i) {
+                v[i] += bias[i];
+                v[i] = p.y_type == LL_T_F32 ? ops_act(v[i], p.act) : ops_act_fast(v[i], p.act);
+            }
             store_y4(p, t0 + c, m, v, mtile);
         }
     }
@@ -352,24 +355,55 @@ __global__ void __launch_bounds__(kDsThreads, 1) ll_dense_fp8_kernel(const __gri
 }
 
 // ---------------------------------------------------------------------------------------------
-// Many rows: D[128 rows x 256 channels] = X tile . W tile^T on one persistent CTA per SM, lane = row.
-// A K block takes the tensor cores 512 cycles (128 x 256 x 128 at 8192 multiply-adds a cycle); its
-// way out (32 K values from TMEM, as many fused multiply-adds by the block's scales: one factor
-// per thread, sx of its row times sw of its 128 channels) takes the eight warps of the epilogue
-// about 300, so the two accumulators in turn keep the tensor cores fed.
-//   warp 0      TMA producer (X box 16 KB + W box 32 KB per K block, 4 stages)
-//   warp 1      TMEM allocation (all 512 columns); one thread issues the MMAs
+// Many rows: D[256 rows x 256 channels] = X tile . W tile^T on pairs of SMs (cta_group::2, one
+// persistent cluster of two CTAs per pair), lane = row, 128 rows per CTA.  Each CTA loads its
+// rows of x and half of the tile's channels; the 2-SM instruction reads the other half from the
+// peer, so an SM's shared memory takes in 32 KB and gives 32 KB per K block of 512 tensor cycles,
+// just its 128 bytes a cycle (a 128 x 256 tile of one SM wants 192 and ran at 2.3 PFLOP/s).
+// A K block's way out is 32 K values per CTA from TMEM and as many multiply-adds by the block's
+// scales (one factor per thread: sx of its row times sw of its 128 channels), beside the tensor
+// cores' work on the next block.
+//   warp 0      TMA producer (x box 16 KB + W box 16 KB per K block, 5 stages)
+//   warp 1      TMEM allocation (all 512 columns, two accumulators); in CTA 0 one thread issues the MMAs
 //   warps 4-11  warps 4-7 channels 0..127 of the tile, warps 8-11 the other 128: 128 sums per
 //               thread in registers; at a tile's end bias, activation and a staged store
 constexpr int kDlThreads = 384;
-constexpr int kDlM = 128, kDlN = 256, kDlStages = 4;
-constexpr int kDlStage = (kDlM + kDlN) * kF8Block;
-constexpr int kDlOut = 32 * 128;                             // staging of a warp: 32 rows of 128 bytes
+constexpr int kDlM = 128, kDlN = 256, kDlStages = 5;         // rows per CTA, channels per pair
+constexpr int kDlStage = (kDlM + kDlN / 2) * kF8Block;
+constexpr int kDlOut = 32 * 256;                             // staging of a warp: 32 rows of 64 fp32 values
 constexpr int kDlOffOut = kDlStages * kDlStage;
 constexpr int kDlOffBar = kDlOffOut + 8 * kDlOut;            // full[S], empty[S], accfull[2], accempty[2], done
 constexpr int kDlOffMisc = kDlOffBar + 8 * (2 * kDlStages + 5);
 constexpr int kDlAlloc = kDlOffMisc + 16 + 1024;
 static_assert(kDlAlloc <= 227 * 1024, "shared memory");
+
+// Instruction descriptor of the pair: M = 256 (128 per CTA), N = n.
+__host__ __device__ constexpr uint32_t tc_idesc_e4m3_pair(int n)
+{
+    return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(256 >> 4) << 24);
+}
+
+__device__ __forceinline__ void tc_mma_f8_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                               uint32_t accumulate)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// 2-D tensor load of this CTA's tile whose completion bytes go to an mbarrier of the pair (cluster
+// address: CTA 0's barrier); no multicast.
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap *tm, int x, int y, uint32_t cluster_bar)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
+        "[%4];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(tm)), "r"(x), "r"(y), "r"(cluster_bar)
+        : "memory");
+}
 
 // 32 lanes x 32 consecutive fp32 columns; the wait is separate.
 __device__ __forceinline__ void tc_ld_32cols_async(uint32_t taddr, uint32_t (&r)[32])
@@ -398,83 +432,99 @@ __device__ __forceinline__ void tc_wait_ld_32(uint32_t (&r)[32])
                  : "memory");
 }
 
-// acc += v * s for 32 columns, two at a time.
+// acc += v * s for 32 columns.
 __device__ __forceinline__ void fma_32cols(float *acc, const uint32_t (&v)[32], float s)
 {
 #pragma unroll
-    for (int i = 0; i < 32; i += 2)
-        asm("{\n\t.reg .b64 a, b, c;\n\t"
-            "mov.b64 a, {%0, %1};\n\t"
-            "mov.b64 b, {%2, %3};\n\t"
-            "mov.b64 c, {%4, %4};\n\t"
-            "fma.rn.f32x2 a, b, c, a;\n\t"
-            "mov.b64 {%0, %1}, a;\n\t}"
-            : "+f"(acc[i]), "+f"(acc[i + 1])
-            : "r"(v[i]), "r"(v[i + 1]), "f"(s));
+    for (int i = 0; i < 32; ++i)
+        acc[i] = fmaf(__uint_as_float(v[i]), s, acc[i]);
 }
 
-// The warp's 32 rows x 32 columns (thread = row, in registers) through its staging tile (16-byte pieces,
-// piece j of row r at j ^ (r & 7)), so that 8 lanes hold 128 bytes of a row: there bias and
-// activation are applied, four values a lane at a time (one copy of the activation's code, where
-// one per register would stream tens of KB through the instruction cache), and the results
-// stored, or (e4m3) put back for the threads' group maxima.
-__device__ __forceinline__ void dl_store_32cols(const DenseF8Params &p, uint8_t *out, float *acc, long long row0, int c0)
+// The warp's 32 rows x 64 columns (thread = row, in registers) through its staging tile (16-byte pieces,
+// piece j of row r at j ^ (r & 7) within its 128 bytes), so that 8 lanes hold a row's 64 values, 8
+// each: there bias and activation are applied and the results stored, 16 bytes a lane for a
+// 16-bit type, or (e4m3) put back for the threads' group maxima.  The activation runs here, on 8
+// values at a time, and not on the 128 registers: one copy of its code, where one per register
+// would stream tens of KB through the instruction cache.
+template <int YT, int ACT>
+__device__ __forceinline__ void dl_store_64cols(const DenseF8Params &p, uint8_t *out, float *acc, long long row0, int c0)
 {
-    const int lane = threadIdx.x & 31, j = lane & 7, c = c0 + 4 * j, have = p.M - c;
+    const int lane = threadIdx.x & 31, j = lane & 7, c = c0 + 8 * j, have = p.M - c;
+    auto piece = [&](int r, int i) {  // 16 pieces of a row: two stretches of 8
+        return reinterpret_cast<float4 *>(out + r * 256 + (i >> 3) * 128 + (((i ^ r) & 7) << 4));
+    };
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        *reinterpret_cast<float4 *>(out + lane * 128 + ((i ^ (lane & 7)) << 4)) =
-            make_float4(acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]);
-    float bias[4];
+    for (int i = 0; i < 16; ++i)
+        *piece(lane, i) = make_float4(acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]);
+    float bias[8];
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
+    for (int e = 0; e < 8; ++e)
         bias[e] = p.bias && e < have ? __ldg(p.bias + c + e) : 0.0f;
     __syncwarp();
-#pragma unroll 1
-    for (int i = 0; i < 8; ++i) {
-        const int r = 4 * i + (lane >> 3);
-        float4 *at = reinterpret_cast<float4 *>(out + r * 128 + ((j ^ (r & 7)) << 4));
-        const float4 q = *at;
-        float v[4] = {q.x, q.y, q.z, q.w};
+    const long long left = p.rows - row0;  // rows of the tile that exist
+    if (have >= 8 && (YT == LL_T_F8 || p.y_vec)) {
+        constexpr int ESZ = YT == LL_T_F32 ? 4 : 2;
+        uint8_t *y = static_cast<uint8_t *>(p.y) + ((row0 + (lane >> 3)) * p.ldy + c) * ESZ;
+#pragma unroll 4
+        for (int i = 0; i < 8; ++i, y += 4 * p.ldy * ESZ) {
+            const int r = 4 * i + (lane >> 3);
+            const float4 q0 = *piece(r, 2 * j), q1 = *piece(r, 2 * j + 1);
+            float v[8] = {q0.x, q0.y, q0.z, q0.w, q1.x, q1.y, q1.z, q1.w};
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            v[e] = e < have ? ops_act(v[e] + bias[e], p.act) : 0.0f;
-        const long long row = row0 + r;
-        if (p.y_type == LL_T_F8) {
-            *at = make_float4(v[0], v[1], v[2], v[3]);
-        } else if (row < p.rows && have > 0) {
-            if (p.y_type == LL_T_F32) {
-                float *y = static_cast<float *>(p.y) + row * p.ldy + c;
-                if (have >= 4 && p.y_vec) {
-                    *reinterpret_cast<float4 *>(y) = make_float4(v[0], v[1], v[2], v[3]);
-                } else {
-                    for (int e = 0; e < 4; ++e)
-                        if (e < have)
-                            y[e] = v[e];
+            for (int e = 0; e < 8; ++e)
+                v[e] = YT == LL_T_F32 ? ops_act(v[e] + bias[e], ACT) : ops_act_fast(v[e] + bias[e], ACT);
+            if constexpr (YT == LL_T_F8) {
+                *piece(r, 2 * j) = make_float4(v[0], v[1], v[2], v[3]);
+                *piece(r, 2 * j + 1) = make_float4(v[4], v[5], v[6], v[7]);
+            } else if constexpr (YT == LL_T_F32) {
+                if (r < left) {
+                    reinterpret_cast<float4 *>(y)[0] = make_float4(v[0], v[1], v[2], v[3]);
+                    reinterpret_cast<float4 *>(y)[1] = make_float4(v[4], v[5], v[6], v[7]);
                 }
             } else {
-                uint16_t h[4];
+                uint32_t h[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    h[e] = p.y_type == LL_T_BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v[e]))
-                                                 : __half_as_ushort(__float2half_rn(v[e]));
-                uint16_t *y = static_cast<uint16_t *>(p.y) + row * p.ldy + c;
-                if (have >= 4 && p.y_vec) {
-                    *reinterpret_cast<uint2 *>(y) =
-                        make_uint2((uint32_t)h[0] | ((uint32_t)h[1] << 16), (uint32_t)h[2] | ((uint32_t)h[3] << 16));
-                } else {
-                    for (int e = 0; e < 4; ++e)
-                        if (e < have)
-                            y[e] = h[e];
+                for (int e = 0; e < 4; ++e) {
+                    if constexpr (YT == LL_T_BF16) {
+                        const __nv_bfloat162 t = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
+                        h[e] = *reinterpret_cast<const uint32_t *>(&t);
+                    } else {
+                        const __half2 t = __floats2half2_rn(v[2 * e], v[2 * e + 1]);
+                        h[e] = *reinterpret_cast<const uint32_t *>(&t);
+                    }
+                }
+                if (r < left)
+                    *reinterpret_cast<uint4 *>(y) = make_uint4(h[0], h[1], h[2], h[3]);
+            }
+        }
+    } else {  // the last channels, or rows that do not start on 16 bytes: value by value
+#pragma unroll 1
+        for (int i = 0; i < 8; ++i) {
+            const int r = 4 * i + (lane >> 3);
+#pragma unroll 1
+            for (int e = 0; e < 8; ++e) {
+                float *at = reinterpret_cast<float *>(piece(r, 2 * j + (e >> 2))) + (e & 3);
+                float v = *at + (p.bias && e < have ? __ldg(p.bias + c + e) : 0.0f);
+                v = YT == LL_T_F32 ? ops_act(v, ACT) : ops_act_fast(v, ACT);
+                const long long o = (row0 + r) * p.ldy + c + e;
+                if constexpr (YT == LL_T_F8) {
+                    *at = e < have ? v : 0.0f;
+                } else if (r < left && e < have) {
+                    if constexpr (YT == LL_T_F32)
+                        static_cast<float *>(p.y)[o] = v;
+                    else if constexpr (YT == LL_T_BF16)
+                        static_cast<__nv_bfloat16 *>(p.y)[o] = __float2bfloat16_rn(v);
+                    else
+                        static_cast<__half *>(p.y)[o] = __float2half_rn(v);
                 }
             }
         }
     }
     __syncwarp();
-    if (p.y_type == LL_T_F8) {
+    if constexpr (YT == LL_T_F8) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float4 q = *reinterpret_cast<const float4 *>(out + lane * 128 + ((i ^ (lane & 7)) << 4));
+        for (int i = 0; i < 16; ++i) {
+            const float4 q = *piece(lane, i);
             acc[4 * i] = q.x, acc[4 * i + 1] = q.y, acc[4 * i + 2] = q.z, acc[4 * i + 3] = q.w;
         }
         __syncwarp();
@@ -499,14 +549,13 @@ __device__ __forceinline__ void dl_store_e4m3(const DenseF8Params &p, uint8_t *o
             make_uint4(group_e4m3x4(acc + 16 * i, false, s, inv), group_e4m3x4(acc + 16 * i + 4, false, s, inv),
                        group_e4m3x4(acc + 16 * i + 8, false, s, inv), group_e4m3x4(acc + 16 * i + 12, false, s, inv));
     __syncwarp();
-    const bool vec = (p.ldy & 15) == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0;
-#pragma unroll 1
+#pragma unroll 2
     for (int i = 0; i < 8; ++i) {
         const int r = 4 * i + (lane >> 3), j = lane & 7, have = p.M - (c0 + 16 * j);
         const uint8_t *at = out + r * 128 + ((j ^ (r & 7)) << 4);
         if (row0 + r < p.rows && have > 0) {
             uint8_t *y = static_cast<uint8_t *>(p.y) + (row0 + r) * p.ldy + c0 + 16 * j;
-            if (vec && have >= 16) {
+            if (p.y_vec && have >= 16) {
                 *reinterpret_cast<uint4 *>(y) = *reinterpret_cast<const uint4 *>(at);
             } else {
                 for (int e = 0; e < min(16, have); ++e)
@@ -517,6 +566,36 @@ __device__ __forceinline__ void dl_store_e4m3(const DenseF8Params &p, uint8_t *o
     __syncwarp();
 }
 
+template <int YT, int ACT>
+__device__ __forceinline__ void dl_store_act(const DenseF8Params &p, uint8_t *out, float (&acc)[128], long long row0,
+                                             int c0)
+{
+    dl_store_64cols<YT, ACT>(p, out, acc, row0, c0);
+    if (c0 + 64 < p.M)
+        dl_store_64cols<YT, ACT>(p, out, acc + 64, row0, c0 + 64);
+    if constexpr (YT == LL_T_F8) {
+        if (c0 + 64 >= p.M)
+#pragma unroll
+            for (int i = 64; i < 128; ++i)
+                acc[i] = 0.0f;
+        dl_store_e4m3(p, out, acc, row0, c0);
+    }
+}
+
+template <int YT>
+__device__ __forceinline__ void dl_store(const DenseF8Params &p, uint8_t *out, float (&acc)[128], long long row0, int c0)
+{
+    if (p.act == LL_ACT_RELU)
+        dl_store_act<YT, LL_ACT_RELU>(p, out, acc, row0, c0);
+    else if (p.act == LL_ACT_GELU)
+        dl_store_act<YT, LL_ACT_GELU>(p, out, acc, row0, c0);
+    else if (p.act == LL_ACT_SILU)
+        dl_store_act<YT, LL_ACT_SILU>(p, out, acc, row0, c0);
+    else
+        dl_store_act<YT, LL_ACT_IDENTITY>(p, out, acc, row0, c0);
+}
+
+template <int YT>
 __global__ void __launch_bounds__(kDlThreads, 1) ll_dense_fp8_large_kernel(const __grid_constant__ DenseF8Params p)
 {
     constexpr int S = kDlStages;
@@ -532,11 +611,14 @@ __global__ void __launch_bounds__(kDlThreads, 1) ll_dense_fp8_large_kernel(const
     auto b_accf = [&](int b) { return bar(2 * S + b); };
     auto b_acce = [&](int b) { return bar(2 * S + 2 + b); };
     const uint32_t b_done = bar(2 * S + 4);
-    const int mt_n = (p.rows + kDlM - 1) / kDlM, nt_n = (p.M + kDlN - 1) / kDlN, tiles = mt_n * nt_n;
-    // Tiles in bands of 16 row tiles, rows fastest: CTAs that run at once share rows of W and of x in L2.
+    const uint32_t rank = cluster_ctarank();  // the pair is the cluster
+    const bool lead = rank == 0u;
+    const int pair = (int)blockIdx.x >> 1, pairs = (int)gridDim.x >> 1;
+    const int mt_n = (p.rows + 2 * kDlM - 1) / (2 * kDlM), nt_n = (p.M + kDlN - 1) / kDlN, tiles = mt_n * nt_n;
+    // Tiles in bands of 8 row tiles, rows fastest: pairs that run at once share rows of W and of x in L2.
     auto tile_at = [&](int tile, int &mt, int &nt) {
-        const int band = tile / (16 * nt_n), first = band * 16, in = tile - band * 16 * nt_n;
-        const int h = min(16, mt_n - first);
+        const int band = tile / (8 * nt_n), first = band * 8, in = tile - band * 8 * nt_n;
+        const int h = min(8, mt_n - first);
         nt = in / h;
         mt = first + in - nt * h;
     };
@@ -548,7 +630,7 @@ __global__ void __launch_bounds__(kDlThreads, 1) ll_dense_fp8_large_kernel(const
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(b_accf(b), 1);
-            mbar_init(b_acce(b), 8);
+            mbar_init(b_acce(b), 16);  // CTA 0's: eight warps of each CTA
         }
         mbar_init(b_done, 1);
         misc[1] = 0;
@@ -557,14 +639,15 @@ __global__ void __launch_bounds__(kDlThreads, 1) ll_dense_fp8_large_kernel(const
         prefetch_tmap(&p.tm_x);
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                          sbase + (uint32_t)kDlOffMisc),
                      "r"(512u)
                      : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
     tc_fence_before();
     __syncthreads();
+    cluster_sync();  // both CTAs' barriers are initialised and their tensor memory allocated
     tc_fence_after();
     const uint32_t tmem = misc[0];
     int issued = 0;
@@ -575,33 +658,36 @@ __global__ void __launch_bounds__(kDlThreads, 1) ll_dense_fp8_large_kernel(const
         if (warp == 0) {
             if (lane == 0) {
                 bool ok = true;
-                for (int tile = (int)blockIdx.x; tile < tiles && ok; tile += (int)gridDim.x) {
+                for (int tile = pair; tile < tiles && ok; tile += pairs) {
                     int mt, nt;
                     tile_at(tile, mt, nt);
                     for (int kb = 0; kb < p.nkb; ++kb) {
                         const int s = issued % S;
                         if (issued >= S &&
-                            !tc_wait(b_empty(s), ((issued / S) - 1) & 1, p.wait_ns, fail, p.status, 1)) {
+                            !ops_wait(b_empty(s), ((issued / S) - 1) & 1, p.wait_ns, fail, p.status, 1)) {
                             ok = false;
                             break;
                         }
-                        mbar_arrive_expect_tx(b_full(s), kDlStage);
-                        tma_load_2d(sbase + s * kDlStage, &p.tm_x, kb * kF8Block, mt * kDlM, b_full(s));
-                        tma_load_2d(sbase + s * kDlStage + kDlM * kF8Block, &p.tm_w, kb * kF8Block, nt * kDlN, b_full(s));
+                        if (lead)
+                            mbar_arrive_expect_tx(b_full(s), 2 * kDlStage);  // both CTAs' loads land on this barrier
+                        const uint32_t full = mapa(b_full(s), 0u);
+                        tma_load_2d_pair(sbase + s * kDlStage, &p.tm_x, kb * kF8Block, (2 * mt + (int)rank) * kDlM, full);
+                        tma_load_2d_pair(sbase + s * kDlStage + kDlM * kF8Block, &p.tm_w, kb * kF8Block,
+                                         nt * kDlN + (int)rank * (kDlN / 2), full);
                         ++issued;
                     }
                 }
             }
         } else if (warp == 1) {
-            if (lane == 0) {
-                constexpr uint32_t idesc = tc_idesc_e4m3(kDlN);
+            if (lead && lane == 0) {
+                constexpr uint32_t idesc = tc_idesc_e4m3_pair(kDlN);
                 int g = 0;
                 bool ok = true;
-                for (int tile = (int)blockIdx.x; tile < tiles && ok; tile += (int)gridDim.x)
+                for (int tile = pair; tile < tiles && ok; tile += pairs)
                     for (int kb = 0; kb < p.nkb; ++kb, ++g) {
                         const int s = g % S, b = g & 1;
-                        if ((g >= 2 && !tc_wait(b_acce(b), ((g / 2) - 1) & 1, p.wait_ns, fail, p.status, 2)) ||
-                            !tc_wait(b_full(s), (g / S) & 1, p.wait_ns, fail, p.status, 3)) {
+                        if ((g >= 2 && !ops_wait(b_acce(b), ((g / 2) - 1) & 1, p.wait_ns, fail, p.status, 2)) ||
+                            !ops_wait(b_full(s), (g / S) & 1, p.wait_ns, fail, p.status, 3)) {
                             ok = false;
                             break;
                         }
@@ -609,12 +695,12 @@ __global__ void __launch_bounds__(kDlThreads, 1) ll_dense_fp8_large_kernel(const
                         const uint32_t x = sbase + s * kDlStage, w = x + kDlM * kF8Block;
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk)
-                            tc_mma_f8(tmem + (uint32_t)(b * kDlN), sw128_kmajor_desc(x + kk * 32),
-                                      sw128_kmajor_desc(w + kk * 32), idesc, kk != 0);
-                        tc_commit(b_empty(s));
-                        tc_commit(b_accf(b));
+                            tc_mma_f8_pair(tmem + (uint32_t)(b * kDlN), sw128_kmajor_desc(x + kk * 32),
+                                           sw128_kmajor_desc(w + kk * 32), idesc, kk != 0);
+                        tc_commit_both(b_empty(s));
+                        tc_commit_both(b_accf(b));
                     }
-                tc_commit(b_done);
+                tc_commit_both(b_done);
             }
         }
     } else {
@@ -624,10 +710,10 @@ __global__ void __launch_bounds__(kDlThreads, 1) ll_dense_fp8_large_kernel(const
         uint8_t *out = smem + kDlOffOut + (warp - 4) * kDlOut;
         int g = 0;
         bool ok = true;
-        for (int tile = (int)blockIdx.x; tile < tiles && ok; tile += (int)gridDim.x) {
+        for (int tile = pair; tile < tiles && ok; tile += pairs) {
             int mt, nt;
             tile_at(tile, mt, nt);
-            const long long row0 = (long long)mt * kDlM + 32 * quad;
+            const long long row0 = ((long long)mt * 2 + rank) * kDlM + 32 * quad;
             const int c0 = nt * kDlN + half * 128, block = c0 / kF8Block;
             const float *sx = p.sx + min(row0 + lane, (long long)p.rows - 1) * p.nkb;
             const float *sw = p.sw + (size_t)min(block, mblocks - 1) * p.nkb;
@@ -670,21 +756,20 @@ __global__ void __launch_bounds__(kDlThreads, 1) ll_dense_fp8_large_kernel(const
                     tc_wait_ld_32(v1);
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0)
-                        mbar_arrive_local(b_acce(b));
+                    if (lane == 0) {
+                        if (lead)
+                            mbar_arrive_local(b_acce(b));
+                        else
+                            mbar_arrive_remote_cta(mapa(b_acce(b), 0u));
+                    }
                     fma_32cols(acc + 96, v1, s);
                 }
             }
-            if (ok && c0 < p.M) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    dl_store_32cols(p, out, acc + 32 * i, row0, c0 + 32 * i);
-                if (p.y_type == LL_T_F8)
-                    dl_store_e4m3(p, out, acc, row0, c0);
-            }
+            if (ok && c0 < p.M)
+                dl_store<YT>(p, out, acc, row0, c0);
         }
     }
-    if (warp == 0 && lane == 0 && *fail) {  // loads in flight land before the shared memory is given back
+    if (lead && warp == 0 && lane == 0 && *fail) {  // both CTAs' loads in flight land before the shared memory is given back
         for (int j = max(0, issued - S); j < issued; ++j) {
             const uint64_t w0 = globaltimer();
             while (!mbar_try_wait(b_full(j % S), (j / S) & 1) && globaltimer() - w0 < p.wait_ns) {
@@ -700,9 +785,12 @@ __global__ void __launch_bounds__(kDlThreads, 1) ll_dense_fp8_large_kernel(const
             while (!mbar_try_wait(b_done, 0) && globaltimer() - w0 < p.wait_ns) {
             }
         }
-        __syncwarp();
+    }
+    __syncthreads();
+    cluster_sync();  // the pair's MMAs are complete in both CTAs, and nobody arrives at the peer any more
+    if (warp == 1) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
     }
 }
 
@@ -752,19 +840,32 @@ int launch_few(const DenseF8Params &p, int splits, int device, cudaStream_t st)
     return LL_OK;
 }
 
+template <int YT>
 int launch_many(const DenseF8Params &p, int device, cudaStream_t st)
 {
     static int sm_count[kOpsMaxDevices];
-    const void *fn = reinterpret_cast<const void *>(&ll_dense_fp8_large_kernel);
+    const void *fn = reinterpret_cast<const void *>(&ll_dense_fp8_large_kernel<YT>);
     int sms = __atomic_load_n(&sm_count[device], __ATOMIC_ACQUIRE);
     if (sms == 0) {
         LL_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kDlAlloc));
         LL_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
         __atomic_store_n(&sm_count[device], sms, __ATOMIC_RELEASE);
     }
-    const long long tiles = (long long)((p.rows + kDlM - 1) / kDlM) * ((p.M + kDlN - 1) / kDlN);
-    ll_dense_fp8_large_kernel<<<(unsigned)std::min<long long>(tiles, sms), kDlThreads, kDlAlloc, st>>>(p);
-    LL_CUDA_TRY(cudaGetLastError());
+    const long long tiles = (long long)((p.rows + 2 * kDlM - 1) / (2 * kDlM)) * ((p.M + kDlN - 1) / kDlN);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2u * (unsigned)std::min<long long>(tiles, sms / 2));
+    cfg.blockDim = dim3(kDlThreads);
+    cfg.dynamicSmemBytes = kDlAlloc;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = 2;
+    at[0].val.clusterDim.y = 1;
+    at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    void *args[] = {const_cast<DenseF8Params *>(&p)};
+    LL_CUDA_TRY(cudaLaunchKernelExC(&cfg, fn, args));
     return LL_OK;
 }
 
@@ -832,15 +933,20 @@ extern "C" int ll_dense_fp8(const uint8_t *d_W, const float *d_sw, const float *
     p.status = status;
     p.wait_ns = kOpsWaitNs;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const long long large_tiles = (long long)((rows + kDlM - 1) / kDlM) * ((M + kDlN - 1) / kDlN);
-    const bool many = rows > 128 && large_tiles >= 74;
+    const long long large_tiles = (long long)((rows + 2 * kDlM - 1) / (2 * kDlM)) * ((M + kDlN - 1) / kDlN);
+    const bool many = rows > 128 && large_tiles >= 37;
     const int nt = many ? kDlM : rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
-    if (!f8_map(&p.tm_w, d_W, K, M, ldw, many ? kDlN : 128) || !f8_map(&p.tm_x, d_x, K, rows, ldx, nt)) {
+    if (!f8_map(&p.tm_w, d_W, K, M, ldw, 128) || !f8_map(&p.tm_x, d_x, K, rows, ldx, nt)) {
         llh::set_error("%s: the tensor maps could not be encoded", op);
         return LL_ERR_CUDA;
     }
-    if (many)
-        return launch_many(p, dev, st);
+    if (many) {
+        p.y_vec = ((ldy * type_bytes(y_type)) % 16 == 0 && (reinterpret_cast<uintptr_t>(d_y) & 15) == 0) ? 1 : 0;
+        return y_type == LL_T_F32    ? launch_many<LL_T_F32>(p, dev, st)
+               : y_type == LL_T_BF16 ? launch_many<LL_T_BF16>(p, dev, st)
+               : y_type == LL_T_F16  ? launch_many<LL_T_F16>(p, dev, st)
+                                     : launch_many<LL_T_F8>(p, dev, st);
+    }
     // Splits: as many CTAs as SMs, each with two K blocks at least.
     const long long tiles = (long long)((M + 127) / 128) * ((rows + nt - 1) / nt);
     int splits = 1;

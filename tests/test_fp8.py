@@ -321,7 +321,7 @@ class DenseCase:
 SHAPES = [(1, 16, 16), (1, 2048, 2048), (2, 128, 128), (7, 130, 260), (16, 64, 1000), (17, 200, 129), (32, 512, 4096),
           (33, 128, 640), (64, 384, 256), (65, 1000, 1100), (128, 257, 300), (129, 256, 512), (300, 520, 400),
           (256, 2048, 2048), (640, 1280, 384),
-          # enough tiles of 128 x 256 for the many-row kernel: whole ones, ragged ones, one K block and several
+          # enough tiles of 256 x 256 for the many-row kernel: whole ones, ragged ones, one K block and several
           (1300, 1700, 200), (1280, 2048, 128), (2500, 1030, 700), (9601, 130, 1300)]
 
 
@@ -356,7 +356,7 @@ def test_dense_special_values():
 
 @pytest.mark.gpu
 @pytest.mark.timeout(300)
-@pytest.mark.parametrize("rows", [1, 40, 700])
+@pytest.mark.parametrize("rows", [1, 40, 700, 3500])
 def test_dense_repeats_bit_for_bit_on_streams_and_in_graphs(rows):
     import torch
 
