@@ -707,6 +707,7 @@ __global__ void __launch_bounds__(kDlThreads, 1) ll_dense_fp8_large_kernel(const
         asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         const int quad = warp & 3, half = (warp - 4) >> 2, mblocks = (p.M + kF8Block - 1) / kF8Block;
         const uint32_t tq = tmem + ((uint32_t)(32 * quad) << 16) + (uint32_t)(half * 128);
+        const bool s_vec = p.nkb % 4 == 0 && ((reinterpret_cast<uintptr_t>(p.sx) | reinterpret_cast<uintptr_t>(p.sw)) & 15) == 0;
         uint8_t *out = smem + kDlOffOut + (warp - 4) * kDlOut;
         int g = 0;
         bool ok = true;
@@ -721,17 +722,29 @@ __global__ void __launch_bounds__(kDlThreads, 1) ll_dense_fp8_large_kernel(const
 #pragma unroll
             for (int i = 0; i < 128; ++i)
                 acc[i] = 0.0f;
-            float f[4], fn[4];  // the scales of four K blocks, and of the next four
+            // the scales of four K blocks, and those of the next four on their way (multiplied when they
+            // are needed).  A warp's 32 rows are 32 lines: one 16-byte load where the rows allow it
+            // instead of four, each of which would hold the load unit for 32 cycles.
+            float f[4], fx[4], fw[4];
             auto load_scales = [&](int kb) {
+                if (s_vec) {
+                    const float4 a = kb < p.nkb ? __ldg(reinterpret_cast<const float4 *>(sx + kb)) : make_float4(0, 0, 0, 0);
+                    const float4 c = kb < p.nkb ? __ldg(reinterpret_cast<const float4 *>(sw + kb)) : make_float4(0, 0, 0, 0);
+                    fx[0] = a.x, fx[1] = a.y, fx[2] = a.z, fx[3] = a.w;
+                    fw[0] = c.x, fw[1] = c.y, fw[2] = c.z, fw[3] = c.w;
+                } else {
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    fn[i] = kb + i < p.nkb ? __ldg(sx + kb + i) * __ldg(sw + kb + i) : 0.0f;
+                    for (int i = 0; i < 4; ++i) {
+                        fx[i] = kb + i < p.nkb ? __ldg(sx + kb + i) : 0.0f;
+                        fw[i] = kb + i < p.nkb ? __ldg(sw + kb + i) : 0.0f;
+                    }
+                }
             };
             load_scales(0);
             for (int kb0 = 0; kb0 < p.nkb && ok; kb0 += 4) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    f[i] = fn[i];
+                    f[i] = fx[i] * fw[i];
                 load_scales(kb0 + 4);
                 for (int i = 0; i < 4 && kb0 + i < p.nkb; ++i, ++g) {
                     const int b = g & 1;
