@@ -679,28 +679,40 @@ __global__ void __launch_bounds__(kDlThreads, 1) ll_dense_fp8_large_kernel(const
                 }
             }
         } else if (warp == 1) {
-            if (lead && lane == 0) {
+            if (lead) {  // the whole warp, so that the loop runs on uniform registers; one lane issues
                 constexpr uint32_t idesc = tc_idesc_e4m3_pair(kDlN);
-                int g = 0;
+                const uint64_t dx = sw128_kmajor_desc(sbase), dw = sw128_kmajor_desc(sbase + kDlM * kF8Block);
+                const int mine = tiles > pair ? (tiles - pair + pairs - 1) / pairs : 0, total = mine * p.nkb;
+                const bool one = elect_one();
+                uint32_t s = 0, s_lap = 0;   // stage, and its phase
+                uint32_t b = 0, b_lap = 1;   // accumulator; a fresh barrier counts as just emptied
                 bool ok = true;
-                for (int tile = pair; tile < tiles && ok; tile += pairs)
-                    for (int kb = 0; kb < p.nkb; ++kb, ++g) {
-                        const int s = g % S, b = g & 1;
-                        if ((g >= 2 && !ops_wait(b_acce(b), ((g / 2) - 1) & 1, p.wait_ns, fail, p.status, 2)) ||
-                            !ops_wait(b_full(s), (g / S) & 1, p.wait_ns, fail, p.status, 3)) {
-                            ok = false;
-                            break;
-                        }
-                        tc_fence_after();
-                        const uint32_t x = sbase + s * kDlStage, w = x + kDlM * kF8Block;
+                for (int g = 0; g < total; ++g) {
+                    ok = ops_wait_warp(b_acce((int)b), b_lap, p.wait_ns, fail, p.status, 2) &&
+                         ops_wait_warp(b_full((int)s), s_lap, p.wait_ns, fail, p.status, 3);
+                    if (!ok)
+                        break;
+                    tc_fence_after();
+                    if (one) {
+                        const uint64_t ax = dx + (uint64_t)(s * (kDlStage >> 4)), aw = dw + (uint64_t)(s * (kDlStage >> 4));
+                        const uint32_t acc = tmem + b * kDlN;
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk)
-                            tc_mma_f8_pair(tmem + (uint32_t)(b * kDlN), sw128_kmajor_desc(x + kk * 32),
-                                           sw128_kmajor_desc(w + kk * 32), idesc, kk != 0);
-                        tc_commit_both(b_empty(s));
-                        tc_commit_both(b_accf(b));
+                            tc_mma_f8_pair(acc, ax + 2 * kk, aw + 2 * kk, idesc, kk != 0);
+                        tc_commit_both(b_empty((int)s));
+                        tc_commit_both(b_accf((int)b));
                     }
-                tc_commit_both(b_done);
+                    __syncwarp();
+                    if (++s == S) {
+                        s = 0;
+                        s_lap ^= 1u;
+                    }
+                    b ^= 1u;
+                    b_lap ^= b == 0u ? 1u : 0u;
+                }
+                if (one)
+                    tc_commit_both(b_done);
+                __syncwarp();
             }
         }
     } else {
@@ -757,15 +769,14 @@ __global__ void __launch_bounds__(kDlThreads, 1) ll_dense_fp8_large_kernel(const
                     const uint32_t at = tq + (uint32_t)(b * kDlN);
                     uint32_t v0[32], v1[32];
                     tc_ld_32cols_async(at, v0);
-                    tc_wait_ld_32(v0);
                     tc_ld_32cols_async(at + 32, v1);
-                    fma_32cols(acc, v0, s);
+                    tc_wait_ld_32(v0);
                     tc_wait_ld_32(v1);
+                    fma_32cols(acc, v0, s);
                     tc_ld_32cols_async(at + 64, v0);
                     fma_32cols(acc + 32, v1, s);
-                    tc_wait_ld_32(v0);
                     tc_ld_32cols_async(at + 96, v1);
-                    fma_32cols(acc + 64, v0, s);
+                    tc_wait_ld_32(v0);
                     tc_wait_ld_32(v1);
                     tc_fence_before();
                     __syncwarp();
@@ -775,6 +786,7 @@ __global__ void __launch_bounds__(kDlThreads, 1) ll_dense_fp8_large_kernel(const
                         else
                             mbar_arrive_remote_cta(mapa(b_acce(b), 0u));
                     }
+                    fma_32cols(acc + 64, v0, s);
                     fma_32cols(acc + 96, v1, s);
                 }
             }

@@ -100,6 +100,19 @@ __device__ __forceinline__ bool ops_wait_warp(uint32_t bar, uint32_t parity, uns
     return tc_wait_warp(bar, parity, bound_ns, fail, status, role);
 }
 
+// One lane of a converged warp, the same one every time: true there.  With the warp converged around it the
+// compiler keeps addresses and descriptors in uniform registers.
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t p;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(p));
+    return p != 0u;
+}
+
 // ---- e4m3 ----
 
 // Two fp32 values to e4m3 (nearest, ties to even, beyond the largest to the largest), lo in bits 0..7.
