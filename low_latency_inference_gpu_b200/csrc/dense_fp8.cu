@@ -131,12 +131,17 @@ __device__ __forceinline__ void store_y4(const DenseF8Params &p, long long row, 
 
 // ---------------------------------------------------------------------------------------------
 // Few rows: D[128 channels x NT rows] = W tile . X^T, so a weight tile is the MMA's A operand and
-// few rows are a narrow N.  The K blocks of a tile are split over the CTAs of one cluster (grid z),
-// which add their partial tiles through distributed shared memory in rank order.
+// few rows are a narrow N.  The K blocks of a tile are split over the CTAs of one cluster (grid z);
+// each CTA sends the sums of every row to the CTA that owns the row (rank = row mod splits), through
+// distributed shared memory, and the owner adds them in rank order.  Latency is what counts here:
+//   * up to 8 accumulators in tensor memory, so that the MMAs of all K blocks of a CTA are issued
+//     as their operands land and wait for nobody;
+//   * 4 stages of 18 KB at 16 rows, so that two CTAs fit an SM and the next launch's set-up
+//     (barriers, tensor memory, tensor maps) runs beside this one's end (programmatic dependent launch).
 //   warp 0     TMA producer (W box 16 KB + X box NT * 128 B per K block)
-//   warp 1     TMEM allocation; one thread issues the MMAs (two accumulators in turn)
+//   warp 1     TMEM allocation; one lane issues the MMAs
 //   warps 2-5  lane = channel: TMEM -> registers, times the block's scales
-//   all        sum of the cluster's partials of this CTA's rows, bias, activation, store
+//   all        sums of this CTA's rows, bias, activation, store
 constexpr int kDsThreads = 192;
 constexpr int kDsScaleKb = 8;  // K blocks whose scales are staged at once
 
@@ -145,23 +150,70 @@ struct DsSmem {
     static constexpr int WB = 128 * kF8Block;
     static constexpr int XB = NT * kF8Block;
     static constexpr int STAGE = WB + XB;
-    static constexpr int STAGES = NT <= 32 ? 8 : 6;
-    static constexpr int OFF_SC = STAGES * STAGE;  // sx * sw: [4 warps][kDsScaleKb][NT] fp32
-    static constexpr int OFF_BAR = OFF_SC + 4 * kDsScaleKb * NT * 4;  // full[S], empty[S], accfull[2], accempty[2], done
-    static constexpr int N_BAR = 2 * STAGES + 5;
-    static constexpr int OFF_MISC = OFF_BAR + 8 * N_BAR;          // tmem base, fail flag
+    static constexpr int STAGES = NT <= 32 ? 4 : NT == 64 ? 4 : 5;
+    static constexpr int ACC = NT == 16 ? 8 : NT == 32 ? 8 : 4;    // accumulators
+    static constexpr uint32_t TMEM_COLS = ACC * NT;                // 128, 256, 256, 512
+    static constexpr int OFF_SC = STAGES * STAGE;                  // sx * sw: [4 warps][kDsScaleKb][NT] fp32
+    static constexpr int OFF_PART = NT <= 32 ? OFF_SC + 4 * kDsScaleKb * NT * 4 : 0;  // [NT][128] fp32
+    // full[S], empty[S], accfull[A], accempty[A], done
+    static constexpr int OFF_BAR = OFF_SC + 4 * kDsScaleKb * NT * 4 + (NT <= 32 ? NT * 512 : 0);
+    static constexpr int N_BAR = 2 * STAGES + 2 * ACC + 1;
+    static constexpr int OFF_MISC = OFF_BAR + 8 * N_BAR;           // tmem base, fail flag
     static constexpr int ALLOC = OFF_MISC + 16 + 1024;
-    static constexpr int PART_LD = 128;                           // partial tile [NT][128] in the idle ring
-    static_assert(NT * PART_LD * 4 <= STAGES * STAGE, "the partial tile fits the ring");
+    // NT <= 32: a place of its own for the received sums; else in the ring, once the whole cluster has
+    // read its last stage
+    static constexpr bool OWN_PART = NT <= 32;
+    static_assert(OWN_PART || NT * 512 <= STAGES * STAGE, "the sums fit the ring");
     static_assert(ALLOC <= 227 * 1024, "shared memory");
-    static constexpr uint32_t TMEM_COLS = 2 * NT < 32 ? 32 : 2 * NT;
 };
+
+__device__ __forceinline__ void cluster_arrive()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ void cluster_wait()
+{
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ void st_cluster_f32(uint32_t cluster_addr, float v)
+{
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_addr), "f"(v) : "memory");
+}
+
+// The sums of the rows of this CTA (row c of the tile at slot c / SPLITS, rank r's share at [slot][r]).
+template <int NT, int SPLITS>
+__device__ __forceinline__ void ds_finish(const DenseF8Params &p, const float *part, long long t0, int rank, int mtile)
+{
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, m = mtile * 128 + 4 * lane;
+    float bias[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        bias[i] = p.bias && m + i < p.M ? __ldg(p.bias + m + i) : 0.0f;
+    const int mine = (int)min((long long)(NT - rank + SPLITS - 1) / SPLITS,
+                              (p.rows - t0 - rank + SPLITS - 1) / SPLITS);  // rows c = rank + SPLITS slot that exist
+    for (int slot = warp; slot < mine; slot += kDsThreads / 32) {
+        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int r = 0; r < SPLITS; ++r) {
+            const float4 q = *reinterpret_cast<const float4 *>(part + (slot * SPLITS + r) * 128 + 4 * lane);
+            v[0] += q.x, v[1] += q.y, v[2] += q.z, v[3] += q.w;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[i] += bias[i];
+            v[i] = p.y_type == LL_T_F32 ? ops_act(v[i], p.act) : ops_act_fast(v[i], p.act);
+        }
+        store_y4(p, t0 + rank + SPLITS * slot, m, v, mtile);
+    }
+}
 
 template <int NT>
 __global__ void __launch_bounds__(kDsThreads, 1) ll_dense_fp8_kernel(const __grid_constant__ DenseF8Params p)
 {
     using L = DsSmem<NT>;
-    constexpr int S = L::STAGES;
+    constexpr int S = L::STAGES, A = L::ACC;
     extern __shared__ uint8_t ds_smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(ds_smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t sbase = smem_u32(smem);
@@ -169,13 +221,13 @@ __global__ void __launch_bounds__(kDsThreads, 1) ll_dense_fp8_kernel(const __gri
     uint32_t *misc = reinterpret_cast<uint32_t *>(smem + L::OFF_MISC);
     volatile uint32_t *fail = misc + 1;
     float *s_sc = reinterpret_cast<float *>(smem + L::OFF_SC);
-    float *s_part = reinterpret_cast<float *>(smem);
+    float *s_part = reinterpret_cast<float *>(smem + L::OFF_PART);
     auto bar = [&](int i) { return sbase + (uint32_t)L::OFF_BAR + 8u * (uint32_t)i; };
     auto b_full = [&](int s) { return bar(s); };
     auto b_empty = [&](int s) { return bar(S + s); };
     auto b_accf = [&](int b) { return bar(2 * S + b); };
-    auto b_acce = [&](int b) { return bar(2 * S + 2 + b); };
-    const uint32_t b_done = bar(2 * S + 4);
+    auto b_acce = [&](int b) { return bar(2 * S + A + b); };
+    const uint32_t b_done = bar(2 * S + 2 * A);
 
     const int splits = (int)gridDim.z, rank = (int)blockIdx.z;  // the cluster is the z extent
     const int mtile = blockIdx.x, m0 = mtile * 128;
@@ -187,7 +239,7 @@ __global__ void __launch_bounds__(kDsThreads, 1) ll_dense_fp8_kernel(const __gri
             mbar_init(b_full(s), 1);
             mbar_init(b_empty(s), 1);
         }
-        for (int b = 0; b < 2; ++b) {
+        for (int b = 0; b < A; ++b) {
             mbar_init(b_accf(b), 1);
             mbar_init(b_acce(b), 4);
         }
@@ -208,6 +260,10 @@ __global__ void __launch_bounds__(kDsThreads, 1) ll_dense_fp8_kernel(const __gri
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = misc[0];
+    griddep_wait();  // operands, scales and outputs belong to the launches before until here
+    griddep_launch_dependents();
+    if (splits > 1 && L::OWN_PART)
+        cluster_arrive();  // this CTA runs: its shared memory may be written to
 
     int issued = 0;  // producer: K blocks whose loads were started
     if (warp == 0) {
@@ -222,26 +278,30 @@ __global__ void __launch_bounds__(kDsThreads, 1) ll_dense_fp8_kernel(const __gri
                 issued = j + 1;
             }
         }
+        __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0) {
-            constexpr uint32_t idesc = tc_idesc_e4m3(NT);
-            for (int j = 0; j < nkb; ++j) {
-                const int s = j % S, b = j & 1;
-                if (j >= 2 && !ops_wait(b_acce(b), ((j / 2) - 1) & 1, p.wait_ns, fail, p.status, 2))
-                    break;
-                if (!ops_wait(b_full(s), (j / S) & 1, p.wait_ns, fail, p.status, 3))
-                    break;
-                tc_fence_after();
-                const uint32_t a = sbase + s * L::STAGE, x = a + L::WB;
+        constexpr uint32_t idesc = tc_idesc_e4m3(NT);
+        const uint64_t da = sw128_kmajor_desc(sbase), db = sw128_kmajor_desc(sbase + L::WB);
+        const bool one = elect_one();
+        for (int j = 0; j < nkb; ++j) {
+            const int s = j % S, b = j % A;
+            if ((j >= A && !ops_wait_warp(b_acce(b), ((j / A) - 1) & 1, p.wait_ns, fail, p.status, 2)) ||
+                !ops_wait_warp(b_full(s), (j / S) & 1, p.wait_ns, fail, p.status, 3))
+                break;
+            tc_fence_after();
+            if (one) {
+                const uint64_t off = (uint64_t)(s * (L::STAGE >> 4));
 #pragma unroll
                 for (int kk = 0; kk < 4; ++kk)
-                    tc_mma_f8(tmem + (uint32_t)(b * NT), sw128_kmajor_desc(a + kk * 32), sw128_kmajor_desc(x + kk * 32),
-                              idesc, kk != 0);
+                    tc_mma_f8(tmem + (uint32_t)(b * NT), da + off + 2 * kk, db + off + 2 * kk, idesc, kk != 0);
                 tc_commit(b_empty(s));
                 tc_commit(b_accf(b));
             }
-            tc_commit(b_done);
+            __syncwarp();
         }
+        if (one)
+            tc_commit(b_done);
+        __syncwarp();
     } else {
         const int quad = warp & 3, chan = 32 * quad + lane;
         float *w_sc = s_sc + quad * (kDsScaleKb * NT);
@@ -250,6 +310,7 @@ __global__ void __launch_bounds__(kDsThreads, 1) ll_dense_fp8_kernel(const __gri
 #pragma unroll
         for (int c = 0; c < NT; ++c)
             acc[c] = 0.0f;
+        bool ok = true;
         for (int j = 0; j < nkb; ++j) {
             if (j % kDsScaleKb == 0) {  // the next blocks' scales, a copy per warp: no warp waits for another
                 const int n = min(kDsScaleKb, nkb - j);
@@ -274,8 +335,9 @@ __global__ void __launch_bounds__(kDsThreads, 1) ll_dense_fp8_kernel(const __gri
                 }
                 __syncwarp();
             }
-            const int b = j & 1;
-            if (!ops_wait_warp(b_accf(b), (j / 2) & 1, p.wait_ns, fail, p.status, 4))
+            const int b = j % A;
+            ok = ops_wait_warp(b_accf(b), (j / A) & 1, p.wait_ns, fail, p.status, 4);
+            if (!ok)
                 break;
             tc_fence_after();
             const float *sc = w_sc + (j % kDsScaleKb) * NT;
@@ -297,11 +359,25 @@ __global__ void __launch_bounds__(kDsThreads, 1) ll_dense_fp8_kernel(const __gri
             if (lane == 0)
                 mbar_arrive_local(b_acce(b));
         }
-        // every MMA has read the ring before the partial tile overwrites it
+        // every MMA of this CTA has read its stage
         ops_wait_warp(b_done, 0, p.wait_ns, fail, p.status, 5);
+        if (splits > 1) {
+            if (!L::OWN_PART)
+                cluster_arrive();  // its ring may be written to
+            cluster_wait();
+        }
+        // row c's sums of this CTA to the owner's [c / splits][rank]
+        const uint32_t part = smem_u32(s_part) + (uint32_t)chan * 4u;
+        if (splits == 1) {
 #pragma unroll
-        for (int c = 0; c < NT; ++c)
-            s_part[c * L::PART_LD + chan] = acc[c];
+            for (int c = 0; c < NT; ++c)
+                s_part[c * 128 + chan] = acc[c];
+        } else {
+            const int log2 = 31 - __clz(splits), mask = splits - 1;
+#pragma unroll
+            for (int c = 0; c < NT; ++c)
+                st_cluster_f32(mapa(part + (uint32_t)((((c >> log2) << log2) + rank) * 512), (uint32_t)(c & mask)), acc[c]);
+        }
     }
     // A CTA that gave up leaves loads in flight: they land before its shared memory is given back.
     if (warp == 0 && lane == 0 && *fail) {
@@ -312,8 +388,18 @@ __global__ void __launch_bounds__(kDsThreads, 1) ll_dense_fp8_kernel(const __gri
         }
     }
     __syncwarp();
+    if (splits > 1 && warp < 2) {  // the producers' part of the barrier that the others have passed
+        if (!L::OWN_PART)
+            cluster_arrive();
+        cluster_wait();
+    }
     tc_fence_before();
-    __syncthreads();
+    if (splits > 1) {
+        cluster_arrive();  // this CTA's sums are with their owners
+        cluster_wait();
+    } else {
+        __syncthreads();
+    }
     if (warp == 1) {
         if (*fail && lane == 0) {
             const uint64_t w0 = globaltimer();
@@ -325,33 +411,16 @@ __global__ void __launch_bounds__(kDsThreads, 1) ll_dense_fp8_kernel(const __gri
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(L::TMEM_COLS)
                      : "memory");
     }
-    if (splits > 1)
-        cluster_sync();  // every partial tile of the cluster is written
-
-    const uint32_t part = smem_u32(s_part);
     if (*fail == 0) {
-        const int m = m0 + 4 * lane;
-        float bias[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            bias[i] = p.bias && m + i < p.M ? __ldg(p.bias + m + i) : 0.0f;
-        for (int c = rank + splits * warp; c < NT && t0 + c < p.rows; c += splits * (kDsThreads / 32)) {
-            const uint32_t at = part + (uint32_t)(c * L::PART_LD + 4 * lane) * 4u;
-            float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            for (int r = 0; r < splits; ++r) {
-                const float4 q = ld_cluster_v4(mapa(at, (uint32_t)r));
-                v[0] += q.x, v[1] += q.y, v[2] += q.z, v[3] += q.w;
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                v[i] += bias[i];
-                v[i] = p.y_type == LL_T_F32 ? ops_act(v[i], p.act) : ops_act_fast(v[i], p.act);
-            }
-            store_y4(p, t0 + c, m, v, mtile);
-        }
+        if (splits == 1)
+            ds_finish<NT, 1>(p, s_part, t0, rank, mtile);
+        else if (splits == 2)
+            ds_finish<NT, 2>(p, s_part, t0, rank, mtile);
+        else if (splits == 4)
+            ds_finish<NT, 4>(p, s_part, t0, rank, mtile);
+        else
+            ds_finish<NT, 8>(p, s_part, t0, rank, mtile);
     }
-    if (splits > 1)
-        cluster_sync();  // nobody leaves while a peer may still read its partial tile
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -853,13 +922,15 @@ int launch_few(const DenseF8Params &p, int splits, int device, cudaStream_t st)
     cfg.blockDim = dim3(kDsThreads);
     cfg.dynamicSmemBytes = (size_t)DsSmem<NT>::ALLOC;
     cfg.stream = st;
-    cudaLaunchAttribute at[1];
+    cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = 1;
     at[0].val.clusterDim.y = 1;
     at[0].val.clusterDim.z = (unsigned)splits;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     void *args[] = {const_cast<DenseF8Params *>(&p)};
     LL_CUDA_TRY(cudaLaunchKernelExC(&cfg, fn, args));
     return LL_OK;
