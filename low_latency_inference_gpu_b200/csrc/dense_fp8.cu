@@ -150,9 +150,9 @@ struct DsSmem {
     static constexpr int WB = 128 * kF8Block;
     static constexpr int XB = NT * kF8Block;
     static constexpr int STAGE = WB + XB;
-    static constexpr int STAGES = NT <= 32 ? 4 : NT == 64 ? 4 : 5;
-    static constexpr int ACC = NT == 16 ? 8 : NT == 32 ? 8 : 4;    // accumulators
-    static constexpr uint32_t TMEM_COLS = ACC * NT;                // 128, 256, 256, 512
+    static constexpr int STAGES = NT <= 32 ? 4 : 5;
+    static constexpr int ACC = NT <= 32 ? 8 : 4;                   // accumulators
+    static constexpr uint32_t TMEM_COLS = ACC * NT;                // 128, 256 or 512
     static constexpr int OFF_SC = STAGES * STAGE;                  // sx * sw: [4 warps][kDsScaleKb][NT] fp32
     static constexpr int OFF_PART = NT <= 32 ? OFF_SC + 4 * kDsScaleKb * NT * 4 : 0;  // [NT][128] fp32
     // full[S], empty[S], accfull[A], accempty[A], done
@@ -1029,9 +1029,15 @@ extern "C" int ll_dense_fp8(const uint8_t *d_W, const float *d_sw, const float *
     p.status = status;
     p.wait_ns = kOpsWaitNs;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    // Which kernel, measured in a graph on B200 (us; many-row kernel / few-row kernel at its best):
+    //   32 tiles of 256 x 256 and more: 1024 x 2048 x 1024 12.6 / 13.2, 512 x 4096 x 4096 26 / 33,
+    //   768 x 4096 x 4096 27 / 57; fewer leave too many SMs idle: 256 x 4096 x 4096 25.5 / 19.9.
+    // Rows per tile of the few-row kernel: 32 (16 for up to 16 rows); 128 once those tiles alone fill
+    // the SMs: 1500 x 900 x 900 13.7 against 15.2 at 32, 256 x 2048 x 2048 9.6 against 8.1 at 32.
     const long long large_tiles = (long long)((rows + 2 * kDlM - 1) / (2 * kDlM)) * ((M + kDlN - 1) / kDlN);
-    const bool many = rows > 128 && large_tiles >= 37;
-    const int nt = many ? kDlM : rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+    const bool many = rows > 128 && large_tiles >= 32;
+    const long long mtiles = (M + 127) / 128;
+    const int nt = many ? kDlM : rows <= 16 ? 16 : mtiles * ((rows + 127) / 128) >= 96 ? 128 : 32;
     if (!f8_map(&p.tm_w, d_W, K, M, ldw, 128) || !f8_map(&p.tm_x, d_x, K, rows, ldx, nt)) {
         llh::set_error("%s: the tensor maps could not be encoded", op);
         return LL_ERR_CUDA;
@@ -1043,10 +1049,13 @@ extern "C" int ll_dense_fp8(const uint8_t *d_W, const float *d_sw, const float *
                : y_type == LL_T_F16  ? launch_many<LL_T_F16>(p, dev, st)
                                      : launch_many<LL_T_F8>(p, dev, st);
     }
-    // Splits: as many CTAs as SMs, each with two K blocks at least.
-    const long long tiles = (long long)((M + 127) / 128) * ((rows + nt - 1) / nt);
+    // Splits of K (CTAs of a cluster): up to one CTA per SM with two K blocks each, or two small CTAs per SM
+    // with four blocks each (64 x 4096 x 4096: 8.3 us at 256 CTAs, 9.3 at 128); not 8 splits for that, whose
+    // exchange costs more than the shorter sums save (200 x 640 x 8192: 12.5 us at 280 CTAs, 10.3 at 140).
+    const long long tiles = mtiles * ((rows + nt - 1) / nt);
     int splits = 1;
-    while (splits < 8 && tiles * splits * 2 <= 148 && p.nkb >= splits * 4)
+    while (splits < 8 && ((tiles * splits * 2 <= 148 && p.nkb >= splits * 4) ||
+                          (tiles * splits * 2 <= 296 && splits <= 2 && nt <= 32 && p.nkb >= splits * 8)))
         splits *= 2;
     p.kb_split = (p.nkb + splits - 1) / splits;
     switch (nt) {
@@ -1054,8 +1063,6 @@ extern "C" int ll_dense_fp8(const uint8_t *d_W, const float *d_sw, const float *
         return launch_few<16>(p, splits, dev, st);
     case 32:
         return launch_few<32>(p, splits, dev, st);
-    case 64:
-        return launch_few<64>(p, splits, dev, st);
     default:
         return launch_few<128>(p, splits, dev, st);
     }

@@ -4,14 +4,14 @@
 //   amax = max |x[r, 128 g .. 128 g + 127]|,  s = amax / 448 (or the power of two at or above),
 //   q = e4m3 nearest to x / s.
 //
-// One pass: 16 lanes hold a group in registers (8 values each), agree on amax by four
-// shuffles, and write 8 bytes each.  Bound by memory for many rows, by the launch for few.
+// One pass: 8 lanes hold a group in registers (16 values each), agree on amax by three
+// shuffles, and write 16 bytes each.  Bound by memory for many rows, by the launch for few.
 #include "ops_common.cuh"
 
 namespace llk {
 
 constexpr int kQtThreads = 256;
-constexpr int kQtLanes = 16;                          // lanes per group
+constexpr int kQtLanes = 8;                           // lanes per group
 constexpr int kQtPer = kF8Block / kQtLanes;           // values per lane
 constexpr int kQtGroups = kQtThreads / kQtLanes;      // groups per block and step
 
@@ -42,68 +42,130 @@ __device__ __forceinline__ float to_f32(__half v)
     return __half2float(v);
 }
 
-__device__ __forceinline__ void load8(const float *p, float (&v)[kQtPer])
+__device__ __forceinline__ void load_all(const float *p, float (&v)[kQtPer])
 {
-    const float4 a = __ldg(reinterpret_cast<const float4 *>(p)), b = __ldg(reinterpret_cast<const float4 *>(p) + 1);
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-}
-
-template <typename T>
-__device__ __forceinline__ void load8(const T *p, float (&v)[kQtPer])
-{
-    const uint4 a = __ldg(reinterpret_cast<const uint4 *>(p));
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const T *h = reinterpret_cast<const T *>(&w[i]);
-        v[2 * i] = to_f32(h[0]);
-        v[2 * i + 1] = to_f32(h[1]);
+    for (int j = 0; j < kQtPer / 4; ++j) {
+        const float4 a = __ldg(reinterpret_cast<const float4 *>(p) + j);
+        v[4 * j] = a.x, v[4 * j + 1] = a.y, v[4 * j + 2] = a.z, v[4 * j + 3] = a.w;
     }
 }
 
-// VEC: every row of x starts on 16 bytes and every row of q on 8.
-template <typename T, bool VEC>
+template <typename T>
+__device__ __forceinline__ void load_all(const T *p, float (&v)[kQtPer])
+{
+#pragma unroll
+    for (int j = 0; j < kQtPer / 8; ++j) {
+        const uint4 a = __ldg(reinterpret_cast<const uint4 *>(p) + j);
+        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const T *h = reinterpret_cast<const T *>(&w[i]);
+            v[8 * j + 2 * i] = to_f32(h[0]);
+            v[8 * j + 2 * i + 1] = to_f32(h[1]);
+        }
+    }
+}
+
+// Four values of a 16-bit type as four e4m3 bytes, without a slow path.  v and amax have at most 11
+// significant bits, a border of two e4m3 values 5, so v * 448 / amax is either on a border or at
+// least 2^-17 (relative) away from it; v / s differs from it by the rounding of s alone, one
+// factor for the whole group within 2^-24.  So where s is not exact, a factor of 1 +- 2^-20
+// towards the side on which that rounding puts the quotients decides the ties and changes nothing
+// else; where it is (or is the smallest scale), one correction step makes the quotient exact.
+struct Scale16 {
+    float s, inv, by;  // by: the reciprocal with the group's factor
+    bool exact;
+};
+
+__device__ __forceinline__ Scale16 scale16(float amax, float s, float inv)
+{
+    const float d = fmaf(-kF8Max, s, amax);  // exact: s is amax / 448 to 2^-24
+    const bool exact = d == 0.0f || s <= 0x1p-126f;
+    return {s, inv, exact ? inv : inv * (d > 0.0f ? 1.0f + 0x1p-20f : 1.0f - 0x1p-20f), exact};
+}
+
+__device__ __forceinline__ uint32_t e4m3x4_of16(const float *v, const Scale16 &g)
+{
+    float t[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        t[i] = v[i] * g.by;
+    if (g.exact)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            t[i] = fmaf(fmaf(-t[i], g.s, v[i]), g.inv, t[i]);
+    return f32x2_to_e4m3(t[0], t[1]) | (f32x2_to_e4m3(t[2], t[3]) << 16);
+}
+
+// VEC: every row of x and of q starts on 16 bytes.  U groups per 8 lanes, kQtGroups apart.
+template <typename T, bool VEC, int U>
 __global__ void __launch_bounds__(kQtThreads) ll_quantize_fp8_kernel(const T *__restrict__ x, long long ldx, int dim,
                                                                      uint32_t n_groups, FastDiv per_row,
                                                                      uint8_t *__restrict__ q, long long ldq,
                                                                      float *__restrict__ s, bool pow2)
 {
-    const uint32_t g = blockIdx.x * kQtGroups + threadIdx.x / kQtLanes;
-    const uint32_t row = (uint32_t)(((uint64_t)g * per_row.m) >> per_row.shift);
-    const int col = (int)(g - row * per_row.d) * kF8Block + (threadIdx.x % kQtLanes) * kQtPer;
-    const int have = g < n_groups ? min(kQtPer, dim - col) : 0;  // <= 0: nothing of the row is left here
-    const T *px = x + (size_t)row * (size_t)ldx + col;
-    float v[kQtPer];
-    if (VEC && have == kQtPer) {
-        load8(px, v);
-    } else {
+    const uint32_t g0 = blockIdx.x * (kQtGroups * U) + threadIdx.x / kQtLanes;
+    uint32_t row[U];
+    int col[U], have[U];
+    float v[U][kQtPer];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const uint32_t g = g0 + u * kQtGroups;
+        row[u] = (uint32_t)(((uint64_t)g * per_row.m) >> per_row.shift);
+        col[u] = (int)(g - row[u] * per_row.d) * kF8Block + (threadIdx.x % kQtLanes) * kQtPer;
+        have[u] = g < n_groups ? min(kQtPer, dim - col[u]) : 0;  // <= 0: nothing of the row is left here
+        const T *px = x + (size_t)row[u] * (size_t)ldx + col[u];
+        if (VEC && have[u] == kQtPer) {
+            load_all(px, v[u]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kQtPer; ++i)
+                v[u][i] = i < have[u] ? to_f32(px[i]) : 0.0f;
+        }
+    }
+    float amax[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        amax[u] = 0.0f;
 #pragma unroll
         for (int i = 0; i < kQtPer; ++i)
-            v[i] = i < have ? to_f32(px[i]) : 0.0f;
+            amax[u] = fmaxf(amax[u], fabsf(v[u][i]));
     }
-    float amax = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kQtPer; ++i)
-        amax = fmaxf(amax, fabsf(v[i]));
 #pragma unroll
     for (int off = kQtLanes / 2; off > 0; off >>= 1)
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
-    float sc, inv;
-    e4m3_scale(amax, pow2, sc, inv);
-    const uint2 o = make_uint2(group_e4m3x4(v, pow2, sc, inv), group_e4m3x4(v + 4, pow2, sc, inv));
-    if (have <= 0)
-        return;
-    uint8_t *pq = q + (size_t)row * (size_t)ldq + col;
-    if (VEC && have == kQtPer) {
-        *reinterpret_cast<uint2 *>(pq) = o;
-    } else {
 #pragma unroll
-        for (int i = 0; i < kQtPer; ++i)
-            if (i < have)
-                pq[i] = (uint8_t)((i < 4 ? o.x >> (8 * i) : o.y >> (8 * (i - 4))) & 0xffu);
+        for (int u = 0; u < U; ++u)
+            amax[u] = fmaxf(amax[u], __shfl_xor_sync(0xffffffffu, amax[u], off));
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        float sc, inv;
+        e4m3_scale(amax[u], pow2, sc, inv);
+        uint32_t o[kQtPer / 4];
+        if (sizeof(T) == 2 && !pow2) {
+            const Scale16 g = scale16(amax[u], sc, inv);
+#pragma unroll
+            for (int i = 0; i < kQtPer / 4; ++i)
+                o[i] = e4m3x4_of16(v[u] + 4 * i, g);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kQtPer / 4; ++i)
+                o[i] = group_e4m3x4(v[u] + 4 * i, pow2, sc, inv);
+        }
+        if (have[u] <= 0)
+            continue;
+        uint8_t *pq = q + (size_t)row[u] * (size_t)ldq + col[u];
+        if (VEC && have[u] == kQtPer) {
+            *reinterpret_cast<uint4 *>(pq) = make_uint4(o[0], o[1], o[2], o[3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kQtPer; ++i)
+                if (i < have[u])
+                    pq[i] = (uint8_t)(o[i / 4] >> (8 * (i % 4)));
+        }
+        if (threadIdx.x % kQtLanes == 0)
+            s[g0 + u * kQtGroups] = sc;
     }
-    if (threadIdx.x % kQtLanes == 0)
-        s[g] = sc;
 }
 
 template <typename T>
@@ -112,13 +174,16 @@ void launch_quantize(const void *x, long long ldx, int rows, int dim, bool pow2,
 {
     const uint32_t per_row = (uint32_t)((dim + kF8Block - 1) / kF8Block), n = (uint32_t)rows * per_row;
     const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (ldx * (long long)sizeof(T)) % 16 == 0 &&
-                     (reinterpret_cast<uintptr_t>(q) & 7) == 0 && ldq % 8 == 0;
-    const dim3 grid((n + kQtGroups - 1) / kQtGroups);
+                     (reinterpret_cast<uintptr_t>(q) & 15) == 0 && ldq % 16 == 0;
     const FastDiv fd = fast_div(per_row);
-    if (vec)
-        ll_quantize_fp8_kernel<T, true><<<grid, kQtThreads, 0, st>>>((const T *)x, ldx, dim, n, fd, q, ldq, s, pow2);
+    auto go = [&](auto kernel, int u) {
+        kernel<<<dim3((n + kQtGroups * u - 1) / (kQtGroups * u)), kQtThreads, 0, st>>>((const T *)x, ldx, dim, n, fd, q, ldq,
+                                                                                      s, pow2);
+    };
+    if (!vec)
+        go(ll_quantize_fp8_kernel<T, false, 1>, 1);
     else
-        ll_quantize_fp8_kernel<T, false><<<grid, kQtThreads, 0, st>>>((const T *)x, ldx, dim, n, fd, q, ldq, s, pow2);
+        go(ll_quantize_fp8_kernel<T, true, 1>, 1);
 }
 
 __device__ unsigned g_ops_status;  // see llh::ops_status_word

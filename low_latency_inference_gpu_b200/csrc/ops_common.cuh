@@ -123,33 +123,42 @@ __device__ __forceinline__ uint32_t f32x2_to_e4m3(float lo, float hi)
     return r;
 }
 
-// e4m3 nearest to the exact quotient v / s (two of them).  The quotient of two 24-bit
-// significands that is not itself on the border of two e4m3 values (5 significant bits) is
-// at least 2^-30 (relative) away from it, so the 53-bit quotient lies on the right side;
-// rounding it to odd in fp32 keeps that side for the final rounding.
-static __device__ __noinline__ uint32_t quot_e4m3_exact(float v0, float v1, float s)
+// The value of an e4m3 code without sign (exact).
+__device__ __forceinline__ float e4m3_value(uint32_t code)
 {
-    float f[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const double d = (double)(i ? v1 : v0) / (double)s;
-        f[i] = __double2float_rz(d);
-        if ((double)f[i] != d && f[i] == f[i])
-            f[i] = __uint_as_float(__float_as_uint(f[i]) | 1u);
-    }
-    return f32x2_to_e4m3(f[0], f[1]);
+    uint32_t h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)code));
+    return __low2float(*reinterpret_cast<const __half2 *>(&h));
 }
 
-// e4m3 of v0 / s and v1 / s given inv = 1 / s rounded.  v * inv is within 2^-23 (relative) of
-// the quotient; where both ends of an interval of +-2^-22 round to one e4m3 value that is the
-// answer, and else (about one pair in 2^17, or a tie) the exact quotient decides.
+// Of two neighbouring e4m3 codes (one byte each, of v's sign) the one nearest to the exact quotient v / s:
+// the sign of |v| - border * s, one fused operation, says on which side of the border (5 significant
+// bits, exact) the quotient lies; a tie goes to the even code.
+__device__ __forceinline__ uint32_t nearer_e4m3(float v, float s, uint32_t a, uint32_t b)
+{
+    const uint32_t lo = min(a, b) & 0x7fu, hi = max(a, b) & 0x7fu, sign = a & 0x80u;
+    const float border = 0.5f * (e4m3_value(lo) + e4m3_value(hi));
+    const float side = fmaf(-border, s, fabsf(v));
+    return sign | (side > 0.0f ? hi : side < 0.0f ? lo : lo + (lo & 1u));
+}
+
+// e4m3 of v0 / s and v1 / s given inv = 1 / s to 2^-23.  The quotient lies between v times inv (1 + 2^-21)
+// and v times inv (1 - 2^-21), each rounded; where both are one e4m3 value that is the answer.
+// Else a border lies between: rare for fp32, but 16-bit values often are ties up to the rounding
+// of s, so the exact side is decided in a few operations.
 __device__ __forceinline__ uint32_t quot_e4m3(float v0, float v1, float s, float inv)
 {
-    const float t0 = v0 * inv, t1 = v1 * inv;
-    constexpr float kUp = 1.0f + 0x1p-22f, kDown = 1.0f - 0x1p-22f;
-    const uint32_t a = f32x2_to_e4m3(t0 * kUp, t1 * kUp);
-    const uint32_t b = f32x2_to_e4m3(t0 * kDown, t1 * kDown);
-    return a == b ? a : quot_e4m3_exact(v0, v1, s);
+    const float up = inv * (1.0f + 0x1p-21f), down = inv * (1.0f - 0x1p-21f);
+    const uint32_t a = f32x2_to_e4m3(v0 * up, v1 * up);
+    const uint32_t b = f32x2_to_e4m3(v0 * down, v1 * down);
+    if (a == b)
+        return a;
+    uint32_t o = a;
+    if ((a ^ b) & 0xffu)
+        o = (o & 0xff00u) | nearer_e4m3(v0, s, a & 0xffu, b & 0xffu);
+    if ((a ^ b) & 0xff00u)
+        o = (o & 0xffu) | (nearer_e4m3(v1, s, a >> 8, b >> 8) << 8);
+    return o;
 }
 
 // The scale of a group whose largest magnitude is amax: amax / 448, or the next power of two at
@@ -169,7 +178,7 @@ __device__ __forceinline__ void e4m3_scale(float amax, bool pow2, float &s, floa
         inv = e >= 254u ? 0.0f : __uint_as_float((254u - e) << 23);
     } else {
         s = q;
-        inv = __frcp_rn(q);
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(q));
     }
 }
 

@@ -221,6 +221,30 @@ def test_quantize_ties_and_borders():
 
 @pytest.mark.gpu
 @pytest.mark.timeout(300)
+@pytest.mark.parametrize("x_type", [ll.T_BF16, ll.T_F16])
+def test_quantize_16_bit_ties(x_type):
+    # 16-bit quotients are often ties up to the rounding of the scale: every significand against every
+    # largest magnitude's (bf16), or a spread of them (fp16), over the octaves of e4m3 and below
+    bits = 8 if x_type == ll.T_BF16 else 11
+    sig = np.arange(2 ** (bits - 1), 2 ** bits)[:: 1 if bits == 8 else 8].astype(np.float64)
+    rows = []
+    for a in sig:
+        v = (sig[None, :] * np.exp2(-np.arange(0, 20, 3))[:, None]).ravel()
+        v = v[v <= a]
+        for i in range(0, v.size, F8 - 1):
+            g = np.zeros(F8)
+            part = v[i:i + F8 - 1]
+            g[:part.size], g[-1] = part * np.where(np.arange(part.size) % 2, -1, 1), a
+            rows.append(g)
+    x = (np.stack(rows) * np.exp2(1 - bits)).astype(np.float32)
+    q, s, x = run_quantize(x, x_type)
+    want_q, want_s = quantize_rows(x)
+    assert np.array_equal(s, want_s)
+    assert np.array_equal(decode(q), decode(want_q))
+
+
+@pytest.mark.gpu
+@pytest.mark.timeout(300)
 @pytest.mark.parametrize("pow2", [False, True])
 def test_quantize_special_values(pow2):
     x = np.ones((6, 256), np.float32)
