@@ -12,7 +12,7 @@
 // tensor memory; at these widths the memory is the bound and the warp-level instruction is at a
 // few per cent of its rate.
 // Every warp works alone: it takes whole tiles (up to 16 weight rows, all columns), copies their
-// rows into a ring of its own (asynchronous copies, kMoeStages stages of 4 KB, refilled as soon as
+// rows into a ring of its own (asynchronous copies, stages of 4 KB, refilled as soon as
 // a stage is read) and keeps the tile's sums in registers.  Nothing is handed from warp to warp on
 // the way, so the warps drift apart and cover each other's latencies, and nothing is waited for
 // that could fail to come.
@@ -37,12 +37,21 @@
 
 namespace llk {
 
-constexpr int kMoeWarps = 8;
-constexpr int kMoeThreads = 32 * kMoeWarps;
+// Warps of a CTA and stages of a warp's ring: for up to 8 rows 8 warps, whose tiles are few; for more rows,
+// where every expert has work and a step takes longer, 16 with shorter rings (32 rows of 64 experts
+// 2048 x 1024 bf16: MOE_W16 us, MOE_W8 at 8 warps).
+__host__ __device__ constexpr int moe_warps(int nt)
+{
+    return nt == 1 ? 8 : 16;
+}
+__host__ __device__ constexpr int moe_stages(int nt)
+{
+    return nt == 1 ? 4 : 2;
+}
 constexpr int kMoeCluster = 4;          // kernel 1
 constexpr int kMoeStage = 5120;         // bytes of a ring stage: 16 rows of 256 + 64, or fewer longer ones
-constexpr int kMoeStages = 4;           // stages of a warp's ring
-constexpr int kMoeRing = kMoeWarps * kMoeStages * kMoeStage;
+constexpr int kMoeRing = moe_warps(1) * moe_stages(1) * kMoeStage;
+static_assert(moe_warps(4) * moe_stages(4) == moe_warps(1) * moe_stages(1), "one size of the rings");
 constexpr int kMoeMaxPairs = LL_MOE_MAX_ROWS * LL_MOE_MAX_TOPK;
 
 struct MoeParams {
@@ -76,7 +85,7 @@ __host__ __device__ inline int moe_up16(int v)
     return (v + 15) & ~15;
 }
 
-__host__ __device__ inline MoeSmem moe_smem(const MoeParams &p, bool up)
+__host__ __device__ inline MoeSmem moe_smem(const MoeParams &p, bool up, int warps)
 {
     MoeSmem s;
     const int n = p.rows * p.top_k, picked = p.experts < n ? p.experts : n;
@@ -92,7 +101,7 @@ __host__ __device__ inline MoeSmem moe_smem(const MoeParams &p, bool up)
     s.part = moe_up16(4 * p.rows * p.experts);  // kernel 1: at most 32 + 64 KB with the logits
     s.x = o;  // kernel 1: the rows of x, where they are staged
     if (!up)
-        s.part = o, o += kMoeWarps * p.rows * 16 * 4;
+        s.part = o, o += warps * p.rows * 16 * 4;
     s.total = o;
     return s;
 }
@@ -439,8 +448,9 @@ __device__ __forceinline__ void cp_async(uint32_t dst, const void *src, int n)
 // Tiles of `rows` rows come in segments of 256 << m bytes per row, m as large as 16 rows' 256 bytes
 // allow (a pitch of 64 mod 128 bytes, so that the 8 rows that a quarter of the warp reads do not
 // collide); rows that do not exist and what lies behind a row's end are zero.  The warp issues its
-// tiles' segments in order, kMoeStages ahead, one group of copies per segment (empty ones past the
+// tiles' segments in order, STAGES ahead, one group of copies per segment (empty ones past the
 // last, so that the count of groups tells which has landed).
+template <int STAGES>
 struct MoeRing {
     uint32_t base;  // shared-memory address of this warp's stages
     int rows, m, grain;
@@ -508,7 +518,7 @@ struct MoeRing {
                 copy<4>();
             else
                 copy<1>();
-            slot = slot + 1 == kMoeStages ? 0 : slot + 1;
+            slot = slot + 1 == STAGES ? 0 : slot + 1;
             off += seg();
             if (off >= row_bytes) {
                 off = 0;
@@ -521,7 +531,7 @@ struct MoeRing {
     // The oldest segment has landed, for the whole warp.
     __device__ __forceinline__ void wait() const
     {
-        asm volatile("cp.async.wait_group %0;" ::"n"(kMoeStages - 1) : "memory");
+        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
         __syncwarp();
     }
 };
@@ -559,11 +569,10 @@ __device__ __forceinline__ void moe_piece(float (&d)[NT][4], const uint8_t *r0, 
 
 // One tile: acc = (its rows) . x over all columns, in steps of 256 bytes of every row.  i0 / i1: places
 // of this thread's rows g and g + 8 in a stage; sc0 / sc1: their e4m3 scales by 128-column block.
-// Refills the ring as it goes.  A step's two halves are summed apart (two chains of dependent
-// tensor instructions); the sums run on in its accumulators, except that an e4m3 block's (its
+// Refills the ring as it goes.  The sums run on in the tensor instruction's accumulators, except that an e4m3 block's (its
 // scale) and an fp32 layer's (the instruction cuts off where fp32 would round) are added in fp32.
 template <int WT, int NT, class Src, class TileAt>
-__device__ __forceinline__ void moe_tile(MoeRing &r, const uint8_t *stages, int &slot, TileAt tile_at, int i0, int i1,
+__device__ __forceinline__ void moe_tile(MoeRing<moe_stages(NT)> &r, const uint8_t *stages, int &slot, TileAt tile_at, int i0, int i1,
                                          int K, const float *sc0, const float *sc1, int ntc, const Src &src,
                                          const uint32_t (&xrow)[NT], float (&acc)[NT][4])
 {
@@ -575,7 +584,9 @@ __device__ __forceinline__ void moe_tile(MoeRing &r, const uint8_t *stages, int 
     const int t = threadIdx.x & 3, steps = (K + KS - 1) / KS, blocks = (K + kF8Block - 1) / kF8Block;
     uint4 b[4][RAW], bn[4][RAW];
     float f[4] = {1.0f, 1.0f, 1.0f, 1.0f}, fn[4] = {1.0f, 1.0f, 1.0f, 1.0f};  // e4m3: rows g, g + 8 by half
-    float d[2][NT][4];
+    // one n-tile: two chains of dependent tensor instructions, a step's halves; more: one, for the registers
+    constexpr int CH = NT == 1 ? 2 : 1;
+    float d[CH][NT][4];
     auto load_step = [&](int st) {
         if constexpr (PRE)
 #pragma unroll
@@ -594,7 +605,9 @@ __device__ __forceinline__ void moe_tile(MoeRing &r, const uint8_t *stages, int 
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             acc[nt][i] = 0.0f;
-            d[0][nt][i] = d[1][nt][i] = 0.0f;
+#pragma unroll
+            for (int h = 0; h < CH; ++h)
+                d[h][nt][i] = 0.0f;
         }
     load_step(0);
     for (int st = 0; st < steps;) {
@@ -615,31 +628,37 @@ __device__ __forceinline__ void moe_tile(MoeRing &r, const uint8_t *stages, int 
                 f[i] = fn[i];
             if (st + 1 < steps)
                 load_step(st + 1);  // on its way while this step is computed
-            if constexpr (FRESH)
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+            for (int half = 0; half < 2; half += CH) {
+                if constexpr (FRESH)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        d[0][nt][i] = d[1][nt][i] = 0.0f;
+                    for (int h = 0; h < CH; ++h)
 #pragma unroll
-            for (int pc = 0; pc < 4; ++pc)
-                moe_piece<WT, NT, PRE>(d[pc >> 1], r0 + 64 * pc, r1 + 64 * pc, st * KS + pc * 4 * EP + t * EP, ntc, src, xrow,
-                                  b[pc]);
-            if constexpr (FRESH)
+                        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+                            for (int i = 0; i < 4; ++i)
+                                d[h][nt][i] = 0.0f;
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        acc[nt][0] = fmaf(d[h][nt][0], f[2 * h], acc[nt][0]);
-                        acc[nt][1] = fmaf(d[h][nt][1], f[2 * h], acc[nt][1]);
-                        acc[nt][2] = fmaf(d[h][nt][2], f[2 * h + 1], acc[nt][2]);
-                        acc[nt][3] = fmaf(d[h][nt][3], f[2 * h + 1], acc[nt][3]);
-                    }
+                for (int pc = 2 * half; pc < 2 * (half + CH); ++pc)
+                    moe_piece<WT, NT, PRE>(d[(pc >> 1) - half], r0 + 64 * pc, r1 + 64 * pc,
+                                           st * KS + pc * 4 * EP + t * EP, ntc, src, xrow, b[pc]);
+                if constexpr (FRESH)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int h = 0; h < CH; ++h) {
+                            const float f0 = f[2 * (half + h)], f1 = f[2 * (half + h) + 1];
+                            acc[nt][0] = fmaf(d[h][nt][0], f0, acc[nt][0]);
+                            acc[nt][1] = fmaf(d[h][nt][1], f0, acc[nt][1]);
+                            acc[nt][2] = fmaf(d[h][nt][2], f1, acc[nt][2]);
+                            acc[nt][3] = fmaf(d[h][nt][3], f1, acc[nt][3]);
+                        }
+            }
             r0 += 256;
             r1 += 256;
         }
         __syncwarp();  // every lane has read the stage
-        slot = slot + 1 == kMoeStages ? 0 : slot + 1;
+        slot = slot + 1 == moe_stages(NT) ? 0 : slot + 1;
         r.feed(tile_at);
     }
     if constexpr (!FRESH)
@@ -647,7 +666,7 @@ __device__ __forceinline__ void moe_tile(MoeRing &r, const uint8_t *stages, int 
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                acc[nt][i] = d[0][nt][i] + d[1][nt][i];
+                acc[nt][i] = d[0][nt][i] + (CH == 2 ? d[CH - 1][nt][i] : 0.0f);
     if constexpr (WT == LL_W_F8)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -693,14 +712,15 @@ __device__ __forceinline__ void moe_logits(const MoeParams &p, uint8_t *smem, co
     using X = MoeX<XT>;
     constexpr int EP = 8, KS = 64;
     const int tid = threadIdx.x, warp = tid >> 5, g = (tid & 31) >> 2, t = tid & 3;
-    const int mt_n = (p.experts + 15) / 16, ksub = mt_n >= kMoeWarps ? 1 : kMoeWarps / mt_n;
+    constexpr int WARPS = moe_warps(NT);
+    const int mt_n = (p.experts + 15) / 16, ksub = mt_n >= WARPS ? 1 : WARPS / mt_n;
     const int tp = (p.rows + 7) / 8 * 8, ntc = tp / 8, H = p.hidden;
     const int rank = (int)cluster_ctarank();
     float *part = reinterpret_cast<float *>(smem + L.part);
     const int steps = (H + KS - 1) / KS, slices = kMoeCluster * ksub;
     const X src = {static_cast<const uint8_t *>(p.x), (size_t)p.ldx * X::BYTES, H, p.x_vec != 0};
     {
-        for (int u = warp; u < mt_n * ksub; u += kMoeWarps) {
+        for (int u = warp; u < mt_n * ksub; u += WARPS) {
             const int mt = u / ksub, ks = u - mt * ksub, sl = rank * ksub + ks;
             const uint32_t e0 = (uint32_t)min(mt * 16 + g, p.experts - 1), e1 = (uint32_t)min(mt * 16 + g + 8, p.experts - 1);
             float acc[NT][4] = {};
@@ -761,7 +781,7 @@ __device__ __forceinline__ void moe_logits(const MoeParams &p, uint8_t *smem, co
     cluster_sync();
     float *logits = reinterpret_cast<float *>(smem + L.logits);
     const uint32_t pa = smem_u32(part);
-    for (int i = tid; i < tp * p.experts; i += kMoeThreads) {
+    for (int i = tid; i < tp * p.experts; i += 32 * WARPS) {
         const int e = i / tp, row = i - e * tp;  // consecutive threads: consecutive words
         float v = 0.0f;
         for (int ks = 0; ks < ksub; ++ks) {
@@ -799,7 +819,7 @@ __device__ __forceinline__ void moe_pick(const MoeParams &p, uint8_t *smem, cons
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int *ids = reinterpret_cast<int *>(smem + L.ids);
     float *probs = reinterpret_cast<float *>(smem + L.probs);
-    for (int row = warp; row < p.rows; row += kMoeThreads / 32) {
+    for (int row = warp; row < p.rows; row += (int)blockDim.x / 32) {
         const float *lg = reinterpret_cast<const float *>(smem + L.logits) + row * p.experts;
         uint32_t key[PER];
         float l[PER];
@@ -866,7 +886,7 @@ __device__ __forceinline__ void moe_stage_x(const MoeParams &p, uint8_t *to)
     using X = MoeX<XT>;
     const int pitch = moe_x_pitch(p.hidden, W::BYTES), chunks = moe_cols(p.hidden, W::BYTES) / 8;
     const X src = {static_cast<const uint8_t *>(p.x), (size_t)p.ldx * X::BYTES, p.hidden, p.x_vec != 0};
-    for (int i = threadIdx.x; i < p.rows * chunks; i += kMoeThreads) {
+    for (int i = threadIdx.x; i < p.rows * chunks; i += (int)blockDim.x) {
         const int row = i / chunks, c = i - row * chunks;
         uint4 v[X::template RAW<8>];
         src.template load<8>((uint32_t)row, c * 8, v);
@@ -882,14 +902,15 @@ __device__ __forceinline__ void moe_stage_x(const MoeParams &p, uint8_t *to)
 // ---- kernel 1: router, choice, and the activations of the picked experts ----
 // NT n-tiles of 8 rows; STAGED: x in shared memory (else it is read from global memory as it goes).
 template <int WT, int XT, int NT, bool STAGED>
-__global__ void __launch_bounds__(kMoeThreads, 1) ll_moe_up_kernel(const __grid_constant__ MoeParams p)
+__global__ void __launch_bounds__(32 * moe_warps(NT), 1) ll_moe_up_kernel(const __grid_constant__ MoeParams p)
 {
     using W = MoeW<WT>;
     using X = MoeX<XT>;
     constexpr int NSH = XT == LL_T_F32 ? 3 : 2;  // bf16 terms of an activation
     extern __shared__ __align__(128) uint8_t moe_smem_raw[];
     uint8_t *smem = moe_smem_raw;
-    const MoeSmem L = moe_smem(p, true);
+    constexpr int WARPS = moe_warps(NT), THREADS = 32 * WARPS, STAGES = moe_stages(NT);
+    const MoeSmem L = moe_smem(p, true, WARPS);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const uint32_t *misc = reinterpret_cast<const uint32_t *>(smem + L.misc);
     griddep_wait();
@@ -903,7 +924,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1) ll_moe_up_kernel(const __grid_
         moe_pick<LL_MOE_MAX_EXPERTS / 32>(p, smem, L);
     const int n_pairs = p.rows * p.top_k;
     if (blockIdx.x == 0) {
-        for (int i = tid; i < n_pairs; i += kMoeThreads) {
+        for (int i = tid; i < n_pairs; i += THREADS) {
             const int id = reinterpret_cast<const int *>(smem + L.ids)[i];
             const float w = reinterpret_cast<const float *>(smem + L.probs)[i];
             p.ids[i] = id;
@@ -922,7 +943,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1) ll_moe_up_kernel(const __grid_
 
     // Tiles of ch channels (at most 8 gated, 16 not): as many rounds over the warps as the widest tile
     // needs, and ch as small as keeps that number, so that the warps' shares are even.
-    const int ch_max = p.gated ? 8 : 16, G = (int)gridDim.x * kMoeWarps, me = (int)blockIdx.x * kMoeWarps + warp;
+    const int ch_max = p.gated ? 8 : 16, G = (int)gridDim.x * WARPS, me = (int)blockIdx.x * WARPS + warp;
     const int all = na * F;  // at most LL_MOE_MAX_ROWS LL_MOE_MAX_TOPK LL_MOE_MAX_DIM = 2^25
     const int slots = (all + ch_max * G - 1) / (ch_max * G) * G;
     int ch = min(ch_max, (all + slots - 1) / slots);
@@ -943,8 +964,8 @@ __global__ void __launch_bounds__(kMoeThreads, 1) ll_moe_up_kernel(const __grid_
         half = ch;
         have = min(ch, F - f0);
     };
-    const uint8_t *stages = smem + warp * (kMoeStages * kMoeStage);
-    MoeRing ring = {};
+    const uint8_t *stages = smem + warp * (STAGES * kMoeStage);
+    MoeRing<STAGES> ring = {};
     ring.base = smem_u32(stages);
     ring.shape(p.gated ? 2 * ch : ch);
     ring.grain = p.up_grain;
@@ -952,7 +973,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1) ll_moe_up_kernel(const __grid_
     ring.row_bytes = (int)row_bytes;
     // the rings' place still holds the logits' parts: the cluster's CTAs have read them
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-    for (int s = 0; s < kMoeStages; ++s)
+    for (int s = 0; s < STAGES; ++s)
         ring.feed(tile_at);
     using Src = std::conditional_t<STAGED, MoeTerms<X::NS, true>, X>;
     Src src;
@@ -1017,21 +1038,22 @@ __global__ void __launch_bounds__(kMoeThreads, 1) ll_moe_up_kernel(const __grid_
 
 // ---- kernel 2: down projection and the weighted sum ----
 template <int WT, int NSH, int NT>
-__global__ void __launch_bounds__(kMoeThreads, 1) ll_moe_down_kernel(const __grid_constant__ MoeParams p)
+__global__ void __launch_bounds__(32 * moe_warps(NT), 1) ll_moe_down_kernel(const __grid_constant__ MoeParams p)
 {
     using W = MoeW<WT>;
     extern __shared__ __align__(128) uint8_t moe_smem_raw[];
     uint8_t *smem = moe_smem_raw;
-    const MoeSmem L = moe_smem(p, false);
+    constexpr int WARPS = moe_warps(NT), THREADS = 32 * WARPS, STAGES = moe_stages(NT);
+    const MoeSmem L = moe_smem(p, false, WARPS);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const uint32_t *misc = reinterpret_cast<const uint32_t *>(smem + L.misc);
     float *part = reinterpret_cast<float *>(smem + L.part);  // [warp][row][16 channels]
-    for (int i = tid; i < kMoeWarps * p.rows * 16; i += kMoeThreads)
+    for (int i = tid; i < WARPS * p.rows * 16; i += THREADS)
         part[i] = 0.0f;
     griddep_wait();
     int *ids = reinterpret_cast<int *>(smem + L.ids);
     float *probs = reinterpret_cast<float *>(smem + L.probs);
-    for (int i = tid; i < p.rows * p.top_k; i += kMoeThreads) {
+    for (int i = tid; i < p.rows * p.top_k; i += THREADS) {
         ids[i] = __ldcg(p.ids + i);
         probs[i] = __ldcg(p.probs + i);
     }
@@ -1046,26 +1068,26 @@ __global__ void __launch_bounds__(kMoeThreads, 1) ll_moe_down_kernel(const __gri
     // The CTA's R channels and the picked experts are shared out over the warps as (expert, rs
     // channels), rs as large as leaves every warp something to do.
     int rs = R;
-    while (rs > 1 && (R + rs - 1) / rs * na < kMoeWarps)
+    while (rs > 1 && (R + rs - 1) / rs * na < WARPS)
         rs = (rs + 1) / 2;
     const int subs = (R + rs - 1) / rs, units = subs * na;
-    const int mine_n = units > warp ? (units - warp + kMoeWarps - 1) / kMoeWarps : 0;  // of this warp, per item
+    const int mine_n = units > warp ? (units - warp + WARPS - 1) / WARPS : 0;  // of this warp, per item
     const int first = (int)blockIdx.x * R, items = first < H ? (H - first + G * R - 1) / (G * R) : 0;
     auto tile_at = [&](int q, const uint8_t *&s0, const uint8_t *&s1, int &half, int &have) {
-        const int item = q / mine_n, u = warp + (q - item * mine_n) * kMoeWarps;
+        const int item = q / mine_n, u = warp + (q - item * mine_n) * WARPS;
         const int a = u / subs, r = (u - a * subs) * rs, n = first + item * G * R + r;
         s0 = s1 = p.wd + ((size_t)act_e[a] * H + min(n, H - 1)) * row_bytes;
         half = rs;
         have = min(min(rs, R - r), H - n);
     };
-    const uint8_t *stages = smem + warp * (kMoeStages * kMoeStage);
-    MoeRing ring = {};
+    const uint8_t *stages = smem + warp * (STAGES * kMoeStage);
+    MoeRing<STAGES> ring = {};
     ring.base = smem_u32(stages);
     ring.shape(rs);
     ring.grain = p.down_grain;
     ring.n = items * mine_n;
     ring.row_bytes = (int)row_bytes;
-    for (int s = 0; s < kMoeStages; ++s)
+    for (int s = 0; s < STAGES; ++s)
         ring.feed(tile_at);
     const MoeTerms<NSH, false> src = {reinterpret_cast<const uint8_t *>(p.hid), (size_t)p.hid_plane * 2,
                                       (uint32_t)p.hid_ld * 2u};
@@ -1073,7 +1095,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1) ll_moe_down_kernel(const __gri
     float *mine = part + warp * p.rows * 16;
     for (int item = 0; item < items; ++item) {
         const int n0 = first + item * G * R, n_rows = min(R, H - n0);
-        for (int u = warp; u < units; u += kMoeWarps) {
+        for (int u = warp; u < units; u += WARPS) {
             const int a = u / subs, rr = (u - a * subs) * rs;
             const int e = act_e[a], pos0 = act_off[a], cnt = act_off[a + 1] - pos0, ntc = (cnt + 7) >> 3;
             uint32_t hrow[NT];
@@ -1113,11 +1135,11 @@ __global__ void __launch_bounds__(kMoeThreads, 1) ll_moe_down_kernel(const __gri
             __syncwarp();  // another lane may add to the same place for the next expert
         }
         __syncthreads();
-        for (int i = tid; i < p.rows * 16; i += kMoeThreads) {
+        for (int i = tid; i < p.rows * 16; i += THREADS) {
             const int row = i >> 4, r = i & 15;
             float v = 0.0f;
 #pragma unroll
-            for (int w = 0; w < kMoeWarps; ++w) {
+            for (int w = 0; w < WARPS; ++w) {
                 v += part[w * p.rows * 16 + i];
                 part[w * p.rows * 16 + i] = 0.0f;
             }
@@ -1150,7 +1172,7 @@ int moe_x_bytes(const MoeParams &p)
 }
 
 // One kernel with its own dynamic shared memory; `cluster` CTAs per cluster (0: none).
-inline int moe_launch(const void *fn, bool *ready, MoeParams &p, int smem, int grid, int cluster, bool dependent,
+inline int moe_launch(const void *fn, bool *ready, MoeParams &p, int threads, int smem, int grid, int cluster, bool dependent,
                       int device, cudaStream_t st)
 {
     if (!__atomic_load_n(&ready[device], __ATOMIC_ACQUIRE)) {
@@ -1159,7 +1181,7 @@ inline int moe_launch(const void *fn, bool *ready, MoeParams &p, int smem, int g
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)grid);
-    cfg.blockDim = dim3(kMoeThreads);
+    cfg.blockDim = dim3((unsigned)threads);
     cfg.dynamicSmemBytes = (size_t)smem;
     cfg.stream = st;
     cudaLaunchAttribute at[2];
@@ -1184,12 +1206,12 @@ inline int moe_launch(const void *fn, bool *ready, MoeParams &p, int smem, int g
 }
 
 // Clusters of kernel 1 that the device holds at once, one CTA per SM.
-inline int moe_clusters(const void *fn, int *n)
+inline int moe_clusters(const void *fn, int threads, int *n)
 {
     LL_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kMoeSmemCap));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(kMoeCluster);
-    cfg.blockDim = dim3(kMoeThreads);
+    cfg.blockDim = dim3((unsigned)threads);
     cfg.dynamicSmemBytes = kMoeSmemCap;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
@@ -1222,19 +1244,19 @@ int launch_moe_typed(MoeParams &p, int device, cudaStream_t st)
     // one wave of clusters: a GPC whose SMs are not a multiple of the cluster leaves some out
     int clusters = __atomic_load_n(&cluster_count[device], __ATOMIC_ACQUIRE);
     if (clusters == 0) {
-        LL_TRY(moe_clusters(up, &clusters));
+        LL_TRY(moe_clusters(up, 32 * moe_warps(NT), &clusters));
         __atomic_store_n(&cluster_count[device], clusters, __ATOMIC_RELEASE);
     }
-    LL_TRY(moe_launch(up, up_ready, p, moe_smem(p, true).total + (STAGED ? moe_x_bytes<WT, XT>(p) : 0),
+    LL_TRY(moe_launch(up, up_ready, p, 32 * moe_warps(NT), moe_smem(p, true, moe_warps(NT)).total + (STAGED ? moe_x_bytes<WT, XT>(p) : 0),
                       clusters * kMoeCluster, kMoeCluster, false, device, st));
-    return moe_launch(down, down_ready, p, moe_smem(p, false).total, std::min(sms, p.hidden), 0, true, device, st);
+    return moe_launch(down, down_ready, p, 32 * moe_warps(NT), moe_smem(p, false, moe_warps(NT)).total, std::min(sms, p.hidden), 0, true, device, st);
 }
 
 // Up to 8 rows whose terms fit beside the rings take the kernel that stages x.
 template <int WT, int XT>
 int launch_moe_rows(MoeParams &p, int device, cudaStream_t st)
 {
-    if (p.rows <= 8 && moe_smem(p, true).total + moe_x_bytes<WT, XT>(p) <= kMoeSmemCap)
+    if (p.rows <= 8 && moe_smem(p, true, moe_warps(1)).total + moe_x_bytes<WT, XT>(p) <= kMoeSmemCap)
         return launch_moe_typed<WT, XT, 1, true>(p, device, st);
     return launch_moe_typed<WT, XT, 4, false>(p, device, st);
 }
