@@ -37,21 +37,18 @@
 
 namespace llk {
 
-// Warps of a CTA and stages of a warp's ring: for up to 8 rows 8 warps, whose tiles are few; for more rows,
-// where every expert has work and a step takes longer, 16 with shorter rings (32 rows of 64 experts
-// 2048 x 1024 bf16: MOE_W16 us, MOE_W8 at 8 warps).
-__host__ __device__ constexpr int moe_warps(int nt)
+constexpr int kMoeWarps = 16;
+constexpr int kMoeThreads = 32 * kMoeWarps;
+constexpr int kMoeStages = 2;           // stages of a warp's ring
+// Warps that share a tile, each with a part of the columns: for up to 8 rows, where a T-row layer has few
+// tiles (one row of 8 experts of 1024 channels: 7 per SM), two; for more rows one.
+__host__ __device__ constexpr int moe_team(int nt)
 {
-    return nt == 1 ? 8 : 16;
-}
-__host__ __device__ constexpr int moe_stages(int nt)
-{
-    return nt == 1 ? 4 : 2;
+    return nt == 1 ? 2 : 1;
 }
 constexpr int kMoeCluster = 4;          // kernel 1
 constexpr int kMoeStage = 5120;         // bytes of a ring stage: 16 rows of 256 + 64, or fewer longer ones
-constexpr int kMoeRing = moe_warps(1) * moe_stages(1) * kMoeStage;
-static_assert(moe_warps(4) * moe_stages(4) == moe_warps(1) * moe_stages(1), "one size of the rings");
+constexpr int kMoeRing = kMoeWarps * kMoeStages * kMoeStage;
 constexpr int kMoeMaxPairs = LL_MOE_MAX_ROWS * LL_MOE_MAX_TOPK;
 
 struct MoeParams {
@@ -77,7 +74,7 @@ struct MoeParams {
 // ---- shared memory (byte offsets) ----
 // The warps' rings from 0; kernel 1's logits lie in the same place, read before the rings fill.
 struct MoeSmem {
-    int pairs, ids, probs, mask, act_e, act_off, misc, logits, part, x, total;
+    int pairs, ids, probs, mask, act_e, act_off, misc, logits, part, team, x, total;
 };
 
 __host__ __device__ inline int moe_up16(int v)
@@ -85,7 +82,7 @@ __host__ __device__ inline int moe_up16(int v)
     return (v + 15) & ~15;
 }
 
-__host__ __device__ inline MoeSmem moe_smem(const MoeParams &p, bool up, int warps)
+__host__ __device__ inline MoeSmem moe_smem(const MoeParams &p, bool up)
 {
     MoeSmem s;
     const int n = p.rows * p.top_k, picked = p.experts < n ? p.experts : n;
@@ -99,9 +96,10 @@ __host__ __device__ inline MoeSmem moe_smem(const MoeParams &p, bool up, int war
     s.act_off = o, o += moe_up16(2 * (picked + 1));
     s.logits = 0;
     s.part = moe_up16(4 * p.rows * p.experts);  // kernel 1: at most 32 + 64 KB with the logits
+    s.team = o, o += up ? kMoeWarps * 512 : 0;  // a team's sums on their way, two tiles'
     s.x = o;  // kernel 1: the rows of x, where they are staged
     if (!up)
-        s.part = o, o += warps * p.rows * 16 * 4;
+        s.part = o, o += kMoeWarps * p.rows * 16 * 4;
     s.total = o;
     return s;
 }
@@ -155,7 +153,7 @@ template <>
 struct MoeW<LL_W_BF16> {
     static constexpr int BYTES = 2, EP = 8;
     static constexpr bool PERM = false;
-    static __device__ __forceinline__ void widen(const uint4 &v, uint32_t (&o)[4])
+    static __device__ __forceinline__ void widen(const uint4 &v, uint32_t (&o)[4], uint32_t &)
     {
         o[0] = v.x, o[1] = v.y, o[2] = v.z, o[3] = v.w;
     }
@@ -172,7 +170,7 @@ struct MoeW<LL_W_I8> {
         const uint32_t p = prmt(w, 0x43434343u, sel);
         return bf16x2_sub(p & 0xff7fff7fu, p & 0xff80ff80u);
     }
-    static __device__ __forceinline__ void widen(const uint4 &v, uint32_t (&o)[8])
+    static __device__ __forceinline__ void widen(const uint4 &v, uint32_t (&o)[8], uint32_t &)
     {
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -191,26 +189,16 @@ struct MoeW<LL_W_F8> {
     // exponents' biases differ by 120; e4m3's subnormals become bf16's).  x is multiplied by
     // kMoeF8Up = 2^40 beforehand, so the sums carry 2^-80, far above fp32's underflow, and are
     // multiplied by kMoeF8Back at the end: 7 operations for 4 values, where the conversion
-    // instructions run at a fraction of the rate.  NaN (0x7f) would read as 480: looked for.
-    static __device__ __noinline__ uint32_t nan_in(uint32_t w, uint32_t o)  // bytes 0 and 2 of w
-    {
-        const uint32_t b0 = w & 0x7fu, b1 = (w >> 16) & 0x7fu;
-        return (b0 == 0x7fu ? 0x7fffu : o & 0xffffu) | (b1 == 0x7fu ? 0x7fff0000u : o & 0xffff0000u);
-    }
-    static __device__ __forceinline__ void widen(const uint4 &v, uint32_t (&o)[8])
+    // instructions run at a fraction of the rate.  NaN (0x7f) would read as 480: `nan` collects
+    // a mark (bit 7 of a byte) for it, and the row's sums become NaN at the tile's end.
+    static __device__ __forceinline__ void widen(const uint4 &v, uint32_t (&o)[8], uint32_t &nan)
     {
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-        uint32_t top = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             o[2 * i] = ((w[i] << 8) & 0x80008000u) | ((w[i] << 4) & 0x07f007f0u);  // bytes 0 and 2
             o[2 * i + 1] = (w[i] & 0x80008000u) | ((w[i] >> 4) & 0x07f007f0u);     // bytes 1 and 3
-            top |= (w[i] & 0x7f7f7f7fu) + 0x01010101u;  // bit 7 of a byte: it was 0x7f
-        }
-        if (top & 0x80808080u) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                o[i] = nan_in(w[i >> 1] >> (8 * (i & 1)), o[i]);
+            nan |= (w[i] & 0x7f7f7f7fu) + 0x01010101u;
         }
     }
 };
@@ -445,17 +433,62 @@ __device__ __forceinline__ void cp_async(uint32_t dst, const void *src, int n)
                      : "memory");
 }
 
+// A segment of a tile's rows (see MoeRing) in pieces of 16 bytes, 16 pieces (a half warp) of one row at a
+// time; zeros for rows that do not exist and from byte `end` of a row on.
+template <int GRAIN>
+__device__ __forceinline__ void moe_copy(uint32_t dst, int rows, int m, int half, int have, const uint8_t *s0,
+                                         const uint8_t *s1, int row_bytes, int off, int end)
+{
+    const int lane = threadIdx.x & 31, pl = (lane & 15) * 16, pitch = (256 << m) + 64;
+    dst += (uint32_t)pl;
+    constexpr int UN = GRAIN == 16 ? 2 : 1;
+#pragma unroll UN
+    for (int c = lane >> 4; c < rows << m; c += 2) {
+        const int r = c >> m, sub = (c - (r << m)) << 8, at = off + pl + sub;
+        const int h = r < half ? r : r - half;
+        const int n = h < have ? min(16, max(0, end - at)) : 0;
+        const uint8_t *src = n > 0 ? (r < half ? s0 : s1) + (size_t)h * (size_t)row_bytes + at : s0;
+        const uint32_t d = dst + (uint32_t)(r * pitch + sub);
+        if constexpr (GRAIN == 16) {
+            cp_async<16>(d, src, n);
+        } else if constexpr (GRAIN >= 4) {
+#pragma unroll
+            for (int i = 0; i < 16; i += GRAIN)
+                cp_async<GRAIN>(d + i, n > i ? src + i : s0, n > i ? GRAIN : 0);
+        } else {  // rows on odd addresses: by value
+            uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (i < n)
+                    w[i / 4] |= (uint32_t)__ldg(src + i) << (8 * (i % 4));
+            st_shared_v4(d, make_uint4(w[0], w[1], w[2], w[3]));
+        }
+    }
+}
+
+// Rows that do not start on 16 bytes: out of the way of the others' instructions.
+static __device__ __noinline__ void moe_copy_small(int grain, uint32_t dst, int rows, int m, int half, int have,
+                                                   const uint8_t *s0, const uint8_t *s1, int row_bytes, int off, int end)
+{
+    if (grain >= 8)
+        moe_copy<8>(dst, rows, m, half, have, s0, s1, row_bytes, off, end);
+    else if (grain >= 4)
+        moe_copy<4>(dst, rows, m, half, have, s0, s1, row_bytes, off, end);
+    else
+        moe_copy<1>(dst, rows, m, half, have, s0, s1, row_bytes, off, end);
+}
+
 // Tiles of `rows` rows come in segments of 256 << m bytes per row, m as large as 16 rows' 256 bytes
 // allow (a pitch of 64 mod 128 bytes, so that the 8 rows that a quarter of the warp reads do not
 // collide); rows that do not exist and what lies behind a row's end are zero.  The warp issues its
-// tiles' segments in order, STAGES ahead, one group of copies per segment (empty ones past the
+// tiles' segments in order, kMoeStages ahead, one group of copies per segment (empty ones past the
 // last, so that the count of groups tells which has landed).
-template <int STAGES>
 struct MoeRing {
     uint32_t base;  // shared-memory address of this warp's stages
     int rows, m, grain;
     int q, n;       // next tile to be copied, number of tiles
     int slot, off, row_bytes;
+    int step0, step1, begin, end;  // the steps and the bytes of a row that are this warp's
     const uint8_t *s0, *s1;  // first row of tile q, and first of its second half (rows half ..)
     int half, have;          // rows that exist: i < have, half + i < half + have
 
@@ -473,55 +506,35 @@ struct MoeRing {
         m = r > 8 ? 0 : r > 4 ? 1 : r > 2 ? 2 : r > 1 ? 3 : 4;
     }
 
-    // The segment in pieces of 16 bytes, 16 pieces (a half warp) of one row at a time.
-    template <int GRAIN>
-    __device__ __forceinline__ void copy()
+    // This warp's part of the columns: the i-th of TEAM, whole steps of 256 bytes.
+    template <int TEAM>
+    __device__ __forceinline__ void part(int bytes, int i)
     {
-        const int lane = threadIdx.x & 31, pl = (lane & 15) * 16;
-        const uint32_t dst = base + (uint32_t)(slot * kMoeStage + pl);
-        constexpr int UN = GRAIN == 16 ? 4 : 1;
-#pragma unroll UN
-        for (int c = lane >> 4; c < rows << m; c += 2) {
-            const int r = c >> m, at = off + pl + ((c - (r << m)) << 8);
-            const int h = r < half ? r : r - half;
-            const int n = h < have ? min(16, max(0, row_bytes - at)) : 0;
-            const uint8_t *src = n > 0 ? (r < half ? s0 : s1) + (size_t)h * (size_t)row_bytes + at : s0;
-            const uint32_t d = dst + (uint32_t)(r * pitch() + ((c - (r << m)) << 8));
-            if constexpr (GRAIN == 16) {
-                cp_async<16>(d, src, n);
-            } else if constexpr (GRAIN >= 4) {
-#pragma unroll
-                for (int i = 0; i < 16; i += GRAIN)
-                    cp_async<GRAIN>(d + i, n > i ? src + i : s0, n > i ? GRAIN : 0);
-            } else {  // rows on odd addresses: by value
-                uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (i < n)
-                        w[i / 4] |= (uint32_t)__ldg(src + i) << (8 * (i % 4));
-                st_shared_v4(d, make_uint4(w[0], w[1], w[2], w[3]));
-            }
-        }
+        row_bytes = bytes;
+        const int steps = (bytes + 255) >> 8, first = (steps + TEAM - 1) / TEAM;
+        step0 = min(steps, i * first);
+        step1 = min(steps, (i + 1) * first);
+        begin = off = step0 << 8;
+        end = min(bytes, step1 << 8);
+        if (step0 == step1)
+            n = 0;
     }
 
     template <class TileAt>
     __device__ __forceinline__ void feed(TileAt tile_at)
     {
         if (q < n) {
-            if (off == 0)
+            if (off == begin)
                 tile_at(q, s0, s1, half, have);
+            const uint32_t dst = base + (uint32_t)(slot * kMoeStage);
             if (grain >= 16)
-                copy<16>();
-            else if (grain >= 8)
-                copy<8>();
-            else if (grain >= 4)
-                copy<4>();
+                moe_copy<16>(dst, rows, m, half, have, s0, s1, row_bytes, off, end);
             else
-                copy<1>();
-            slot = slot + 1 == STAGES ? 0 : slot + 1;
+                moe_copy_small(grain, dst, rows, m, half, have, s0, s1, row_bytes, off, end);
+            slot = slot + 1 == kMoeStages ? 0 : slot + 1;
             off += seg();
-            if (off >= row_bytes) {
-                off = 0;
+            if (off >= end) {
+                off = begin;
                 ++q;
             }
         }
@@ -531,148 +544,128 @@ struct MoeRing {
     // The oldest segment has landed, for the whole warp.
     __device__ __forceinline__ void wait() const
     {
-        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+        asm volatile("cp.async.wait_group %0;" ::"n"(kMoeStages - 1) : "memory");
         __syncwarp();
     }
 };
 
-// 64 bytes (a piece of 16 per thread) of each of the tile's rows (r0 / r1: this thread's rows g and
-// g + 8 in the stage) against the n-tiles of x: d += W x.  PRE: the first n-tile's x is in b.
-template <int WT, int NT, bool PRE, class Src, int RAW>
-__device__ __forceinline__ void moe_piece(float (&d)[NT][4], const uint8_t *r0, const uint8_t *r1, int k, int ntc,
-                                          const Src &src, const uint32_t (&xrow)[NT], const uint4 (&b)[RAW])
-{
-    using W = MoeW<WT>;
-    constexpr int EP = W::EP, NS = Src::NS;
-    uint32_t a0[EP / 2], a1[EP / 2];
-    W::widen(*reinterpret_cast<const uint4 *>(r0), a0);
-    W::widen(*reinterpret_cast<const uint4 *>(r1), a1);
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        if (nt < ntc) {
-            uint32_t w[NS][EP / 2];
-            if (PRE && nt == 0) {
-                Src::template terms<EP, W::PERM>(b, w);
-            } else {
-                uint4 v[RAW];
-                src.template load<EP>(xrow[nt], k, v);
-                Src::template terms<EP, W::PERM>(v, w);
-            }
-#pragma unroll
-            for (int j = 0; j < EP / 4; ++j)
-#pragma unroll
-                for (int s = 0; s < NS; ++s)
-                    mma_bf16(d[nt], a0[2 * j], a1[2 * j], a0[2 * j + 1], a1[2 * j + 1], w[s][2 * j], w[s][2 * j + 1]);
-        }
-    }
-}
-
-// One tile: acc = (its rows) . x over all columns, in steps of 256 bytes of every row.  i0 / i1: places
-// of this thread's rows g and g + 8 in a stage; sc0 / sc1: their e4m3 scales by 128-column block.
-// Refills the ring as it goes.  The sums run on in the tensor instruction's accumulators, except that an e4m3 block's (its
-// scale) and an fp32 layer's (the instruction cuts off where fp32 would round) are added in fp32.
+// One tile: acc = (its rows) . x over this warp's columns, in steps of 128 bytes of every row.  i0 / i1:
+// places of this thread's rows g and g + 8 in a stage; sc0 / sc1: their e4m3 scales by 128-column
+// block.  Refills the ring as it goes.  The sums run on in the tensor instruction's accumulators,
+// except that an e4m3 block's (its scale) and an fp32 layer's (the instruction cuts off where fp32
+// would round) are added in fp32.  The loop is kept short: with 16 warps at different places in
+// it, a step unrolled to 24 KB of code waited for instructions half of the time.
 template <int WT, int NT, class Src, class TileAt>
-__device__ __forceinline__ void moe_tile(MoeRing<moe_stages(NT)> &r, const uint8_t *stages, int &slot, TileAt tile_at, int i0, int i1,
+__device__ __forceinline__ void moe_tile(MoeRing &r, const uint8_t *stages, int &slot, TileAt tile_at, int i0, int i1,
                                          int K, const float *sc0, const float *sc1, int ntc, const Src &src,
                                          const uint32_t (&xrow)[NT], float (&acc)[NT][4])
 {
     using W = MoeW<WT>;
-    constexpr int EP = W::EP, RAW = Src::template RAW<EP>, KS = 256 / W::BYTES;
-    // x from global memory is loaded a step ahead where the registers allow (64)
-    constexpr bool PRE = Src::GLOBAL && 4 * RAW * 4 <= 64;
-    constexpr bool FRESH = WT == LL_W_F8 || Src::NS == 3;
-    const int t = threadIdx.x & 3, steps = (K + KS - 1) / KS, blocks = (K + kF8Block - 1) / kF8Block;
-    uint4 b[4][RAW], bn[4][RAW];
-    float f[4] = {1.0f, 1.0f, 1.0f, 1.0f}, fn[4] = {1.0f, 1.0f, 1.0f, 1.0f};  // e4m3: rows g, g + 8 by half
-    // one n-tile: two chains of dependent tensor instructions, a step's halves; more: one, for the registers
-    constexpr int CH = NT == 1 ? 2 : 1;
-    float d[CH][NT][4];
+    constexpr int EP = W::EP, RAW = Src::template RAW<EP>, KS = 128 / W::BYTES, NS = Src::NS;
+    // x from global memory is loaded a step ahead where the registers allow (32)
+    constexpr bool PRE = Src::GLOBAL && 2 * RAW * 4 <= 32;
+    constexpr bool FRESH = WT == LL_W_F8 || NS == 3;
+    const int t = threadIdx.x & 3, steps = min(2 * r.step1, (K + KS - 1) / KS);
+    uint4 b[2][RAW], bn[2][RAW];
+    float f0 = 1.0f, f1 = 1.0f, n0 = 1.0f, n1 = 1.0f;  // e4m3: scales of rows g and g + 8
+    uint32_t nan0 = 0, nan1 = 0;
     auto load_step = [&](int st) {
         if constexpr (PRE)
 #pragma unroll
-            for (int pc = 0; pc < 4; ++pc)
+            for (int pc = 0; pc < 2; ++pc)
                 src.template load<EP>(xrow[0], st * KS + pc * 4 * EP + t * EP, bn[pc]);
         if constexpr (WT == LL_W_F8) {
-            const int j0 = 2 * st, j1 = min(2 * st + 1, blocks - 1);
-            fn[0] = __ldg(sc0 + j0);
-            fn[1] = __ldg(sc1 + j0);
-            fn[2] = __ldg(sc0 + j1);
-            fn[3] = __ldg(sc1 + j1);
+            n0 = __ldg(sc0 + st);
+            n1 = __ldg(sc1 + st);
         }
     };
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 4; ++i)
             acc[nt][i] = 0.0f;
-#pragma unroll
-            for (int h = 0; h < CH; ++h)
-                d[h][nt][i] = 0.0f;
-        }
-    load_step(0);
-    for (int st = 0; st < steps;) {
+    int st = 2 * r.step0;
+    if (st < steps)
+        load_step(st);
+    while (st < steps) {
         const uint8_t *at = stages + slot * kMoeStage + t * 16;
         const uint8_t *r0 = at + i0 * r.pitch(), *r1 = at + i1 * r.pitch();
-        const int end = min(steps, st + (1 << r.m));
+        const int end = min(steps, st + (2 << r.m));
         r.wait();
 #pragma unroll 1
         for (; st < end; ++st) {
             if constexpr (PRE)
 #pragma unroll
-                for (int pc = 0; pc < 4; ++pc)
+                for (int pc = 0; pc < 2; ++pc)
 #pragma unroll
                     for (int i = 0; i < RAW; ++i)
                         b[pc][i] = bn[pc][i];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                f[i] = fn[i];
+            f0 = n0;
+            f1 = n1;
             if (st + 1 < steps)
                 load_step(st + 1);  // on its way while this step is computed
+            float d[NT][4];
 #pragma unroll
-            for (int half = 0; half < 2; half += CH) {
-                if constexpr (FRESH)
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int h = 0; h < CH; ++h)
+                for (int i = 0; i < 4; ++i)
+                    d[nt][i] = FRESH ? 0.0f : acc[nt][i];
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt)
+            for (int pc = 0; pc < 2; ++pc) {
+                uint32_t a0[EP / 2], a1[EP / 2];
+                W::widen(*reinterpret_cast<const uint4 *>(r0 + 64 * pc), a0, nan0);
+                W::widen(*reinterpret_cast<const uint4 *>(r1 + 64 * pc), a1, nan1);
 #pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                d[h][nt][i] = 0.0f;
-#pragma unroll
-                for (int pc = 2 * half; pc < 2 * (half + CH); ++pc)
-                    moe_piece<WT, NT, PRE>(d[(pc >> 1) - half], r0 + 64 * pc, r1 + 64 * pc,
-                                           st * KS + pc * 4 * EP + t * EP, ntc, src, xrow, b[pc]);
-                if constexpr (FRESH)
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int h = 0; h < CH; ++h) {
-                            const float f0 = f[2 * (half + h)], f1 = f[2 * (half + h) + 1];
-                            acc[nt][0] = fmaf(d[h][nt][0], f0, acc[nt][0]);
-                            acc[nt][1] = fmaf(d[h][nt][1], f0, acc[nt][1]);
-                            acc[nt][2] = fmaf(d[h][nt][2], f1, acc[nt][2]);
-                            acc[nt][3] = fmaf(d[h][nt][3], f1, acc[nt][3]);
+                for (int nt = 0; nt < NT; ++nt) {
+                    if (nt < ntc) {
+                        uint32_t w[NS][EP / 2];
+                        if (PRE && nt == 0) {
+                            Src::template terms<EP, W::PERM>(b[pc], w);
+                        } else {
+                            uint4 v[RAW];
+                            src.template load<EP>(xrow[nt], st * KS + pc * 4 * EP + t * EP, v);
+                            Src::template terms<EP, W::PERM>(v, w);
                         }
+#pragma unroll
+                        for (int j = 0; j < EP / 4; ++j)
+#pragma unroll
+                            for (int s = 0; s < NS; ++s)
+                                mma_bf16(d[nt], a0[2 * j], a1[2 * j], a0[2 * j + 1], a1[2 * j + 1], w[s][2 * j],
+                                         w[s][2 * j + 1]);
+                    }
+                }
             }
-            r0 += 256;
-            r1 += 256;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                if constexpr (FRESH) {
+                    acc[nt][0] = fmaf(d[nt][0], f0, acc[nt][0]);
+                    acc[nt][1] = fmaf(d[nt][1], f0, acc[nt][1]);
+                    acc[nt][2] = fmaf(d[nt][2], f1, acc[nt][2]);
+                    acc[nt][3] = fmaf(d[nt][3], f1, acc[nt][3]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        acc[nt][i] = d[nt][i];
+                }
+            }
+            r0 += 128;
+            r1 += 128;
         }
         __syncwarp();  // every lane has read the stage
-        slot = slot + 1 == moe_stages(NT) ? 0 : slot + 1;
+        slot = slot + 1 == kMoeStages ? 0 : slot + 1;
         r.feed(tile_at);
     }
-    if constexpr (!FRESH)
+    if constexpr (WT == LL_W_F8) {
+        float s0 = kMoeF8Back, s1 = kMoeF8Back;
+        const uint32_t lanes = 0xfu << (threadIdx.x & 28);  // the four threads of a row
+        if (__ballot_sync(0xffffffffu, nan0 & 0x80808080u) & lanes)
+            s0 = __uint_as_float(0x7fc00000u);
+        if (__ballot_sync(0xffffffffu, nan1 & 0x80808080u) & lanes)
+            s1 = __uint_as_float(0x7fc00000u);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                acc[nt][i] = d[0][nt][i] + (CH == 2 ? d[CH - 1][nt][i] : 0.0f);
-    if constexpr (WT == LL_W_F8)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                acc[nt][i] *= kMoeF8Back;
+            acc[nt][0] *= s0, acc[nt][1] *= s0, acc[nt][2] *= s1, acc[nt][3] *= s1;
+    }
 }
 
 // This thread's pieces of the router's rows e0 and e1 (columns k0 .. k0 + 63) as bf16 terms.
@@ -712,7 +705,7 @@ __device__ __forceinline__ void moe_logits(const MoeParams &p, uint8_t *smem, co
     using X = MoeX<XT>;
     constexpr int EP = 8, KS = 64;
     const int tid = threadIdx.x, warp = tid >> 5, g = (tid & 31) >> 2, t = tid & 3;
-    constexpr int WARPS = moe_warps(NT);
+    constexpr int WARPS = kMoeWarps;
     const int mt_n = (p.experts + 15) / 16, ksub = mt_n >= WARPS ? 1 : WARPS / mt_n;
     const int tp = (p.rows + 7) / 8 * 8, ntc = tp / 8, H = p.hidden;
     const int rank = (int)cluster_ctarank();
@@ -724,7 +717,7 @@ __device__ __forceinline__ void moe_logits(const MoeParams &p, uint8_t *smem, co
             const int mt = u / ksub, ks = u - mt * ksub, sl = rank * ksub + ks;
             const uint32_t e0 = (uint32_t)min(mt * 16 + g, p.experts - 1), e1 = (uint32_t)min(mt * 16 + g + 8, p.experts - 1);
             float acc[NT][4] = {};
-#pragma unroll(NT == 1 ? 4 : 1)
+#pragma unroll(NT == 1 ? 2 : 1)
             for (int st = sl * steps / slices; st < (sl + 1) * steps / slices; ++st) {
                 uint4 xb[NT][2][X::template RAW<EP>];
 #pragma unroll
@@ -902,15 +895,15 @@ __device__ __forceinline__ void moe_stage_x(const MoeParams &p, uint8_t *to)
 // ---- kernel 1: router, choice, and the activations of the picked experts ----
 // NT n-tiles of 8 rows; STAGED: x in shared memory (else it is read from global memory as it goes).
 template <int WT, int XT, int NT, bool STAGED>
-__global__ void __launch_bounds__(32 * moe_warps(NT), 1) ll_moe_up_kernel(const __grid_constant__ MoeParams p)
+__global__ void __launch_bounds__(kMoeThreads, 1) ll_moe_up_kernel(const __grid_constant__ MoeParams p)
 {
     using W = MoeW<WT>;
     using X = MoeX<XT>;
     constexpr int NSH = XT == LL_T_F32 ? 3 : 2;  // bf16 terms of an activation
     extern __shared__ __align__(128) uint8_t moe_smem_raw[];
     uint8_t *smem = moe_smem_raw;
-    constexpr int WARPS = moe_warps(NT), THREADS = 32 * WARPS, STAGES = moe_stages(NT);
-    const MoeSmem L = moe_smem(p, true, WARPS);
+    constexpr int TEAM = moe_team(NT), TEAMS = kMoeWarps / TEAM;
+    const MoeSmem L = moe_smem(p, true);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const uint32_t *misc = reinterpret_cast<const uint32_t *>(smem + L.misc);
     griddep_wait();
@@ -924,7 +917,7 @@ __global__ void __launch_bounds__(32 * moe_warps(NT), 1) ll_moe_up_kernel(const 
         moe_pick<LL_MOE_MAX_EXPERTS / 32>(p, smem, L);
     const int n_pairs = p.rows * p.top_k;
     if (blockIdx.x == 0) {
-        for (int i = tid; i < n_pairs; i += THREADS) {
+        for (int i = tid; i < n_pairs; i += kMoeThreads) {
             const int id = reinterpret_cast<const int *>(smem + L.ids)[i];
             const float w = reinterpret_cast<const float *>(smem + L.probs)[i];
             p.ids[i] = id;
@@ -943,7 +936,7 @@ __global__ void __launch_bounds__(32 * moe_warps(NT), 1) ll_moe_up_kernel(const 
 
     // Tiles of ch channels (at most 8 gated, 16 not): as many rounds over the warps as the widest tile
     // needs, and ch as small as keeps that number, so that the warps' shares are even.
-    const int ch_max = p.gated ? 8 : 16, G = (int)gridDim.x * WARPS, me = (int)blockIdx.x * WARPS + warp;
+    const int ch_max = p.gated ? 8 : 16, G = (int)gridDim.x * TEAMS, me = (int)blockIdx.x * TEAMS + warp / TEAM;
     const int all = na * F;  // at most LL_MOE_MAX_ROWS LL_MOE_MAX_TOPK LL_MOE_MAX_DIM = 2^25
     const int slots = (all + ch_max * G - 1) / (ch_max * G) * G;
     int ch = min(ch_max, (all + slots - 1) / slots);
@@ -964,16 +957,16 @@ __global__ void __launch_bounds__(32 * moe_warps(NT), 1) ll_moe_up_kernel(const 
         half = ch;
         have = min(ch, F - f0);
     };
-    const uint8_t *stages = smem + warp * (STAGES * kMoeStage);
-    MoeRing<STAGES> ring = {};
+    const uint8_t *stages = smem + warp * (kMoeStages * kMoeStage);
+    MoeRing ring = {};
     ring.base = smem_u32(stages);
     ring.shape(p.gated ? 2 * ch : ch);
     ring.grain = p.up_grain;
     ring.n = hi - lo;
-    ring.row_bytes = (int)row_bytes;
+    ring.part<TEAM>((int)row_bytes, warp % TEAM);
     // the rings' place still holds the logits' parts: the cluster's CTAs have read them
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-    for (int s = 0; s < STAGES; ++s)
+    for (int s = 0; s < kMoeStages; ++s)
         ring.feed(tile_at);
     using Src = std::conditional_t<STAGED, MoeTerms<X::NS, true>, X>;
     Src src;
@@ -1003,6 +996,16 @@ __global__ void __launch_bounds__(32 * moe_warps(NT), 1) ll_moe_up_kernel(const 
         }
         float acc[NT][4];
         moe_tile<WT, NT>(ring, stages, slot, tile_at, i0, i1, H, sc0, sc1, ntc, src, xrow, acc);
+        if constexpr (TEAM == 2) {  // the second warp's sums to the first (NT is 1)
+            float4 *sums = reinterpret_cast<float4 *>(smem + L.team) + ((warp & ~1) + ((tile - lo) & 1)) * 32 + lane;
+            if (warp & 1)
+                *sums = make_float4(acc[0][0], acc[0][1], acc[0][2], acc[0][3]);
+            asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp >> 1)) : "memory");
+            if (warp & 1)
+                continue;
+            const float4 q = *sums;
+            acc[0][0] += q.x, acc[0][1] += q.y, acc[0][2] += q.z, acc[0][3] += q.w;
+        }
         float q0 = 1.0f, q1 = 1.0f;
         if constexpr (WT == LL_W_I8) {
             q0 = __ldg(p.sg + (size_t)e * F + c0);
@@ -1038,22 +1041,22 @@ __global__ void __launch_bounds__(32 * moe_warps(NT), 1) ll_moe_up_kernel(const 
 
 // ---- kernel 2: down projection and the weighted sum ----
 template <int WT, int NSH, int NT>
-__global__ void __launch_bounds__(32 * moe_warps(NT), 1) ll_moe_down_kernel(const __grid_constant__ MoeParams p)
+__global__ void __launch_bounds__(kMoeThreads, 1) ll_moe_down_kernel(const __grid_constant__ MoeParams p)
 {
     using W = MoeW<WT>;
     extern __shared__ __align__(128) uint8_t moe_smem_raw[];
     uint8_t *smem = moe_smem_raw;
-    constexpr int WARPS = moe_warps(NT), THREADS = 32 * WARPS, STAGES = moe_stages(NT);
-    const MoeSmem L = moe_smem(p, false, WARPS);
+    constexpr int TEAM = moe_team(NT), TEAMS = kMoeWarps / TEAM;
+    const MoeSmem L = moe_smem(p, false);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const uint32_t *misc = reinterpret_cast<const uint32_t *>(smem + L.misc);
     float *part = reinterpret_cast<float *>(smem + L.part);  // [warp][row][16 channels]
-    for (int i = tid; i < WARPS * p.rows * 16; i += THREADS)
+    for (int i = tid; i < kMoeWarps * p.rows * 16; i += kMoeThreads)
         part[i] = 0.0f;
     griddep_wait();
     int *ids = reinterpret_cast<int *>(smem + L.ids);
     float *probs = reinterpret_cast<float *>(smem + L.probs);
-    for (int i = tid; i < p.rows * p.top_k; i += THREADS) {
+    for (int i = tid; i < p.rows * p.top_k; i += kMoeThreads) {
         ids[i] = __ldcg(p.ids + i);
         probs[i] = __ldcg(p.probs + i);
     }
@@ -1068,26 +1071,26 @@ __global__ void __launch_bounds__(32 * moe_warps(NT), 1) ll_moe_down_kernel(cons
     // The CTA's R channels and the picked experts are shared out over the warps as (expert, rs
     // channels), rs as large as leaves every warp something to do.
     int rs = R;
-    while (rs > 1 && (R + rs - 1) / rs * na < WARPS)
+    while (rs > 1 && (R + rs - 1) / rs * na < TEAMS)
         rs = (rs + 1) / 2;
     const int subs = (R + rs - 1) / rs, units = subs * na;
-    const int mine_n = units > warp ? (units - warp + WARPS - 1) / WARPS : 0;  // of this warp, per item
+    const int team = warp / TEAM, mine_n = units > team ? (units - team + TEAMS - 1) / TEAMS : 0;  // of this team, per item
     const int first = (int)blockIdx.x * R, items = first < H ? (H - first + G * R - 1) / (G * R) : 0;
     auto tile_at = [&](int q, const uint8_t *&s0, const uint8_t *&s1, int &half, int &have) {
-        const int item = q / mine_n, u = warp + (q - item * mine_n) * WARPS;
+        const int item = q / mine_n, u = team + (q - item * mine_n) * TEAMS;
         const int a = u / subs, r = (u - a * subs) * rs, n = first + item * G * R + r;
         s0 = s1 = p.wd + ((size_t)act_e[a] * H + min(n, H - 1)) * row_bytes;
         half = rs;
         have = min(min(rs, R - r), H - n);
     };
-    const uint8_t *stages = smem + warp * (STAGES * kMoeStage);
-    MoeRing<STAGES> ring = {};
+    const uint8_t *stages = smem + warp * (kMoeStages * kMoeStage);
+    MoeRing ring = {};
     ring.base = smem_u32(stages);
     ring.shape(rs);
     ring.grain = p.down_grain;
     ring.n = items * mine_n;
-    ring.row_bytes = (int)row_bytes;
-    for (int s = 0; s < STAGES; ++s)
+    ring.part<TEAM>((int)row_bytes, warp % TEAM);
+    for (int s = 0; s < kMoeStages; ++s)
         ring.feed(tile_at);
     const MoeTerms<NSH, false> src = {reinterpret_cast<const uint8_t *>(p.hid), (size_t)p.hid_plane * 2,
                                       (uint32_t)p.hid_ld * 2u};
@@ -1095,7 +1098,7 @@ __global__ void __launch_bounds__(32 * moe_warps(NT), 1) ll_moe_down_kernel(cons
     float *mine = part + warp * p.rows * 16;
     for (int item = 0; item < items; ++item) {
         const int n0 = first + item * G * R, n_rows = min(R, H - n0);
-        for (int u = warp; u < units; u += WARPS) {
+        for (int u = team; u < units; u += TEAMS) {
             const int a = u / subs, rr = (u - a * subs) * rs;
             const int e = act_e[a], pos0 = act_off[a], cnt = act_off[a + 1] - pos0, ntc = (cnt + 7) >> 3;
             uint32_t hrow[NT];
@@ -1135,11 +1138,11 @@ __global__ void __launch_bounds__(32 * moe_warps(NT), 1) ll_moe_down_kernel(cons
             __syncwarp();  // another lane may add to the same place for the next expert
         }
         __syncthreads();
-        for (int i = tid; i < p.rows * 16; i += THREADS) {
+        for (int i = tid; i < p.rows * 16; i += kMoeThreads) {
             const int row = i >> 4, r = i & 15;
             float v = 0.0f;
 #pragma unroll
-            for (int w = 0; w < WARPS; ++w) {
+            for (int w = 0; w < kMoeWarps; ++w) {
                 v += part[w * p.rows * 16 + i];
                 part[w * p.rows * 16 + i] = 0.0f;
             }
@@ -1172,7 +1175,7 @@ int moe_x_bytes(const MoeParams &p)
 }
 
 // One kernel with its own dynamic shared memory; `cluster` CTAs per cluster (0: none).
-inline int moe_launch(const void *fn, bool *ready, MoeParams &p, int threads, int smem, int grid, int cluster, bool dependent,
+inline int moe_launch(const void *fn, bool *ready, MoeParams &p, int smem, int grid, int cluster, bool dependent,
                       int device, cudaStream_t st)
 {
     if (!__atomic_load_n(&ready[device], __ATOMIC_ACQUIRE)) {
@@ -1181,7 +1184,7 @@ inline int moe_launch(const void *fn, bool *ready, MoeParams &p, int threads, in
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)grid);
-    cfg.blockDim = dim3((unsigned)threads);
+    cfg.blockDim = dim3(kMoeThreads);
     cfg.dynamicSmemBytes = (size_t)smem;
     cfg.stream = st;
     cudaLaunchAttribute at[2];
@@ -1206,12 +1209,12 @@ inline int moe_launch(const void *fn, bool *ready, MoeParams &p, int threads, in
 }
 
 // Clusters of kernel 1 that the device holds at once, one CTA per SM.
-inline int moe_clusters(const void *fn, int threads, int *n)
+inline int moe_clusters(const void *fn, int *n)
 {
     LL_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kMoeSmemCap));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(kMoeCluster);
-    cfg.blockDim = dim3((unsigned)threads);
+    cfg.blockDim = dim3(kMoeThreads);
     cfg.dynamicSmemBytes = kMoeSmemCap;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
@@ -1244,19 +1247,19 @@ int launch_moe_typed(MoeParams &p, int device, cudaStream_t st)
     // one wave of clusters: a GPC whose SMs are not a multiple of the cluster leaves some out
     int clusters = __atomic_load_n(&cluster_count[device], __ATOMIC_ACQUIRE);
     if (clusters == 0) {
-        LL_TRY(moe_clusters(up, 32 * moe_warps(NT), &clusters));
+        LL_TRY(moe_clusters(up, &clusters));
         __atomic_store_n(&cluster_count[device], clusters, __ATOMIC_RELEASE);
     }
-    LL_TRY(moe_launch(up, up_ready, p, 32 * moe_warps(NT), moe_smem(p, true, moe_warps(NT)).total + (STAGED ? moe_x_bytes<WT, XT>(p) : 0),
+    LL_TRY(moe_launch(up, up_ready, p, moe_smem(p, true).total + (STAGED ? moe_x_bytes<WT, XT>(p) : 0),
                       clusters * kMoeCluster, kMoeCluster, false, device, st));
-    return moe_launch(down, down_ready, p, 32 * moe_warps(NT), moe_smem(p, false, moe_warps(NT)).total, std::min(sms, p.hidden), 0, true, device, st);
+    return moe_launch(down, down_ready, p, moe_smem(p, false).total, std::min(sms, p.hidden), 0, true, device, st);
 }
 
 // Up to 8 rows whose terms fit beside the rings take the kernel that stages x.
 template <int WT, int XT>
 int launch_moe_rows(MoeParams &p, int device, cudaStream_t st)
 {
-    if (p.rows <= 8 && moe_smem(p, true, moe_warps(1)).total + moe_x_bytes<WT, XT>(p) <= kMoeSmemCap)
+    if (p.rows <= 8 && moe_smem(p, true).total + moe_x_bytes<WT, XT>(p) <= kMoeSmemCap)
         return launch_moe_typed<WT, XT, 1, true>(p, device, st);
     return launch_moe_typed<WT, XT, 4, false>(p, device, st);
 }

@@ -235,6 +235,56 @@ def test_special_values_stay_in_their_rows(wtype):
 
 @pytest.mark.gpu
 @pytest.mark.timeout(300)
+@pytest.mark.parametrize("rows", [1, 12])
+def test_nan_weights_of_an_expert_reach_the_rows_that_picked_it(rows):
+    m = ll.MoE(256, 384, 4, 1, wtype=ll.W_F8)
+    layer = Layer(m, rows, router_scale=8.0)
+    layer.run()
+    ids = layer.ids.cpu().numpy()[:, 0]
+    clean = layer.y.float().cpu().numpy()[:rows]
+    e = int(ids[0])
+    layer.d["down"][e, 33, 200] = 0xFF  # one output channel
+    layer.run()
+    y = layer.y.float().cpu().numpy()[:rows]
+    hit = np.zeros_like(y, bool)
+    hit[ids == e, 33] = True
+    assert np.isnan(y[hit]).all() and np.array_equal(y[~hit], clean[~hit])
+    layer.d["gate"][e, 70, 5] = 0x7F    # one activation, so every output channel
+    layer.run()
+    y = layer.y.float().cpu().numpy()[:rows]
+    assert np.isnan(y[ids == e]).all() and np.array_equal(y[ids != e], clean[ids != e])
+
+
+@pytest.mark.gpu
+@pytest.mark.timeout(300)
+def test_every_e4m3_code_counts_exactly():
+    # gate weights that run through all codes, subnormal ones too, against a one-hot x: the activation is the
+    # weight itself; down is the identity, so y is the code's value times the scales
+    import torch
+
+    h = f = 256
+    m = ll.MoE(h, f, 1, 1, act=ll.ACT_IDENTITY, gated=False, wtype=ll.W_F8, x_type=ll.T_F32)
+    layer = Layer(m, 2)
+    codes = np.arange(256, dtype=np.uint8)
+    codes[[0x7F, 0xFF]] = 0
+    gate = np.zeros((1, f, h), np.uint8)
+    gate[0, :, 3], gate[0, :, 200] = codes, codes
+    down = np.zeros((1, h, f), np.uint8)
+    down[0, np.arange(h), np.arange(f)] = 0x38  # 1
+    layer.d["gate"].copy_(dev(gate))
+    layer.d["down"].copy_(dev(down))
+    layer.d["gate_scale"].fill_(0.5)
+    layer.d["down_scale"].fill_(2.0)
+    layer.xv.zero_()
+    layer.xv[0, 3] = 1.0
+    layer.xv[1, 200] = 1.0
+    layer.run()
+    y = layer.y.cpu().numpy()[:2]
+    assert np.array_equal(y[0], decode(codes).astype(np.float32)) and np.array_equal(y[1], y[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.timeout(300)
 @pytest.mark.parametrize("rows", [1, 20])
 def test_repeats_bit_for_bit_on_streams_and_in_graphs(rows):
     import torch
