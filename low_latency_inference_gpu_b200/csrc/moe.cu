@@ -104,11 +104,8 @@ int ll_moe_forward(const ll_moe_desc *d, const ll_moe_weights *w, const void *d_
         return LL_ERR_INVALID_ARG;
     }
     int dev = 0;
-    LL_CUDA_TRY(cudaGetDevice(&dev));
-    if (dev < 0 || dev >= kOpsMaxDevices) {
-        llh::set_error("%s: device index %d out of range", op, dev);
-        return LL_ERR_INVALID_ARG;
-    }
+    unsigned *status = nullptr;
+    LL_TRY(llh::ops_status_word(&dev, &status));
     const size_t xa = (size_t)type_bytes(d->x_type), wa = d->wtype == LL_W_BF16 ? 2 : 1;
     LL_TRY(llh::check_device_ptr(op, "x", d_x, dev, xa));
     LL_TRY(llh::check_device_ptr(op, "y", d_y, dev, xa));
@@ -169,6 +166,8 @@ int ll_moe_forward(const ll_moe_desc *d, const ll_moe_weights *w, const void *d_
     p.hid_ld = wl.ld;
     p.user_ids = d_ids;
     p.user_probs = d_probs;
+    p.status = status;
+    p.wait_ns = kOpsWaitNs;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     return d->wtype == LL_W_BF16 ? launch_moe_bf16(p, dev, st)
            : d->wtype == LL_W_I8 ? launch_moe_i8(p, dev, st)

@@ -12,10 +12,9 @@
 // tensor memory; at these widths the memory is the bound and the warp-level instruction is at a
 // few per cent of its rate.
 // Every warp works alone: it takes whole tiles (up to 16 weight rows, all columns), copies their
-// rows into a ring of its own (asynchronous copies, stages of 4 KB, refilled as soon as
-// a stage is read) and keeps the tile's sums in registers.  Nothing is handed from warp to warp on
-// the way, so the warps drift apart and cover each other's latencies, and nothing is waited for
-// that could fail to come.
+// rows into a ring of its own (bulk copies, a row's segment each, stages of 4 KB, refilled as soon
+// as a stage is read) and keeps the tile's sums in registers.  Nothing is handed from warp to warp
+// on the way, so the warps drift apart and cover each other's latencies.
 //
 // Precision: weights are exact in bf16 (int8 and e4m3 too; their scales multiply fp32 sums).  x
 // and the activations a are split into bf16 terms that add up to the value: x in bf16 one, fp16
@@ -69,12 +68,14 @@ struct MoeParams {
     __nv_bfloat16 *hid;                 // workspace: planes [rows * top_k][hid_ld]
     long long hid_plane;
     int hid_ld;
+    unsigned *status;
+    unsigned long long wait_ns;
 };
 
 // ---- shared memory (byte offsets) ----
 // The warps' rings from 0; kernel 1's logits lie in the same place, read before the rings fill.
 struct MoeSmem {
-    int pairs, ids, probs, mask, act_e, act_off, misc, logits, part, team, x, total;
+    int bars, pairs, ids, probs, mask, act_e, act_off, misc, logits, part, team, x, total;
 };
 
 __host__ __device__ inline int moe_up16(int v)
@@ -87,7 +88,8 @@ __host__ __device__ inline MoeSmem moe_smem(const MoeParams &p, bool up)
     MoeSmem s;
     const int n = p.rows * p.top_k, picked = p.experts < n ? p.experts : n;
     int o = kMoeRing;
-    s.misc = o, o += 16;  // number of picked experts
+    s.bars = o, o += 8 * kMoeWarps * kMoeStages;
+    s.misc = o, o += 16;  // number of picked experts, fail flag
     s.pairs = o, o += moe_up16(2 * n);
     s.ids = o, o += moe_up16(4 * n);
     s.probs = o, o += moe_up16(4 * n);
@@ -480,11 +482,14 @@ static __device__ __noinline__ void moe_copy_small(int grain, uint32_t dst, int 
 
 // Tiles of `rows` rows come in segments of 256 << m bytes per row, m as large as 16 rows' 256 bytes
 // allow (a pitch of 64 mod 128 bytes, so that the 8 rows that a quarter of the warp reads do not
-// collide); rows that do not exist and what lies behind a row's end are zero.  The warp issues its
-// tiles' segments in order, kMoeStages ahead, one group of copies per segment (empty ones past the
-// last, so that the count of groups tells which has landed).
+// collide); what lies behind a row's end is zero up to a whole step.  The warp issues its tiles'
+// segments in order, kMoeStages ahead: bulk copies on a barrier per stage, or (rows that do not
+// start on 16 bytes) one group of small copies per segment, empty ones past the last, so that the
+// count of groups tells which has landed.
 struct MoeRing {
-    uint32_t base;  // shared-memory address of this warp's stages
+    uint32_t base, bars;  // shared-memory addresses of this warp's stages and of a barrier for each
+    uint32_t laps;        // of each stage's barrier, the phase that its next wait is for (a bit)
+    bool ok;              // no wait has run out
     int rows, m, grain;
     int q, n;       // next tile to be copied, number of tiles
     int slot, off, row_bytes;
@@ -527,10 +532,25 @@ struct MoeRing {
             if (off == begin)
                 tile_at(q, s0, s1, half, have);
             const uint32_t dst = base + (uint32_t)(slot * kMoeStage);
-            if (grain >= 16)
-                moe_copy<16>(dst, rows, m, half, have, s0, s1, row_bytes, off, end);
-            else
+            if (grain >= 16) {
+                // a row's segment per lane; a barrier of the stage counts the bytes
+                const int lane = threadIdx.x & 31, h = lane < half ? lane : lane - half, len = min(seg(), end - off);
+                const bool mine = lane < rows && h < have;
+                const int n_rows = __popc(__ballot_sync(0xffffffffu, mine));
+                const uint32_t bar = bars + 8u * (uint32_t)slot, d = dst + (uint32_t)(lane * pitch());
+                if (lane == 0)
+                    mbar_arrive_expect_tx(bar, (uint32_t)(len * n_rows));
+                __syncwarp();
+                if (mine)
+                    bulk_g2s(d, (lane < half ? s0 : s1) + (size_t)h * (size_t)row_bytes + off, (uint32_t)len, bar);
+                if (len & 255) {  // behind a row's last byte: zeros up to a whole step
+                    for (int i = len; lane < rows && i < ((len + 255) & ~255); i += 16)
+                        st_shared_v4(d + (uint32_t)i, make_uint4(0u, 0u, 0u, 0u));
+                    fence_proxy_async_shared();  // before a later segment's copy to the same place
+                }
+            } else {
                 moe_copy_small(grain, dst, rows, m, half, have, s0, s1, row_bytes, off, end);
+            }
             slot = slot + 1 == kMoeStages ? 0 : slot + 1;
             off += seg();
             if (off >= end) {
@@ -541,13 +561,50 @@ struct MoeRing {
         asm volatile("cp.async.commit_group;" ::: "memory");
     }
 
-    // The oldest segment has landed, for the whole warp.
-    __device__ __forceinline__ void wait() const
+    // The segment in stage `at` has landed, for the whole warp.
+    __device__ __forceinline__ void wait(const MoeParams &p, int at, volatile uint32_t *fail)
     {
-        asm volatile("cp.async.wait_group %0;" ::"n"(kMoeStages - 1) : "memory");
+        if (grain >= 16) {
+            if (ok)
+                ok = ops_wait_warp(bars + 8u * (uint32_t)at, (laps >> at) & 1u, p.wait_ns, fail, p.status, 6);
+            laps ^= 1u << at;
+        } else {
+            asm volatile("cp.async.wait_group %0;" ::"n"(kMoeStages - 1) : "memory");
+        }
         __syncwarp();
     }
+
+    // After a wait that ran out: what is still on its way lands (or a second passes for each stage) before the
+    // shared memory is given back.
+    __device__ __forceinline__ void drain(const MoeParams &p) const
+    {
+        if (ok || (threadIdx.x & 31) != 0)
+            return;
+        for (int i = 0; i < kMoeStages; ++i) {
+            const uint64_t t0 = globaltimer();
+            while (!mbar_try_wait(bars + 8u * (uint32_t)i, ((laps >> i) & 1u) ^ 1u) && globaltimer() - t0 < p.wait_ns) {
+            }
+        }
+    }
 };
+
+// This warp's ring (its stages are part of `stages`), barriers initialised; the caller synchronises.
+__device__ __forceinline__ MoeRing moe_ring(uint8_t *smem, const MoeSmem &L)
+{
+    const int warp = threadIdx.x >> 5;
+    MoeRing r = {};
+    r.base = smem_u32(smem) + (uint32_t)(warp * kMoeStages * kMoeStage);
+    r.bars = smem_u32(smem + L.bars) + (uint32_t)(warp * kMoeStages * 8);
+    r.ok = true;
+    if ((threadIdx.x & 31) == 0) {
+        for (int i = 0; i < kMoeStages; ++i)
+            mbar_init(r.bars + 8u * (uint32_t)i, 1);
+        fence_mbar_init_cluster();
+    }
+    if (threadIdx.x == 0)
+        *reinterpret_cast<uint32_t *>(smem + L.misc + 4) = 0;
+    return r;
+}
 
 // One tile: acc = (its rows) . x over this warp's columns, in steps of 128 bytes of every row.  i0 / i1:
 // places of this thread's rows g and g + 8 in a stage; sc0 / sc1: their e4m3 scales by 128-column
@@ -556,7 +613,8 @@ struct MoeRing {
 // would round) are added in fp32.  The loop is kept short: with 16 warps at different places in
 // it, a step unrolled to 24 KB of code waited for instructions half of the time.
 template <int WT, int NT, class Src, class TileAt>
-__device__ __forceinline__ void moe_tile(MoeRing &r, const uint8_t *stages, int &slot, TileAt tile_at, int i0, int i1,
+__device__ __forceinline__ void moe_tile(const MoeParams &p, MoeRing &r, volatile uint32_t *fail, const uint8_t *stages,
+                                         int &slot, TileAt tile_at, int i0, int i1,
                                          int K, const float *sc0, const float *sc1, int ntc, const Src &src,
                                          const uint32_t (&xrow)[NT], float (&acc)[NT][4])
 {
@@ -591,7 +649,7 @@ __device__ __forceinline__ void moe_tile(MoeRing &r, const uint8_t *stages, int 
         const uint8_t *at = stages + slot * kMoeStage + t * 16;
         const uint8_t *r0 = at + i0 * r.pitch(), *r1 = at + i1 * r.pitch();
         const int end = min(steps, st + (2 << r.m));
-        r.wait();
+        r.wait(p, slot, fail);
 #pragma unroll 1
         for (; st < end; ++st) {
             if constexpr (PRE)
@@ -905,7 +963,8 @@ __global__ void __launch_bounds__(kMoeThreads, 1) ll_moe_up_kernel(const __grid_
     constexpr int TEAM = moe_team(NT), TEAMS = kMoeWarps / TEAM;
     const MoeSmem L = moe_smem(p, true);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const uint32_t *misc = reinterpret_cast<const uint32_t *>(smem + L.misc);
+    volatile uint32_t *misc = reinterpret_cast<volatile uint32_t *>(smem + L.misc);
+    MoeRing ring = moe_ring(smem, L);
     griddep_wait();
     griddep_launch_dependents();
     if constexpr (STAGED)
@@ -958,14 +1017,13 @@ __global__ void __launch_bounds__(kMoeThreads, 1) ll_moe_up_kernel(const __grid_
         have = min(ch, F - f0);
     };
     const uint8_t *stages = smem + warp * (kMoeStages * kMoeStage);
-    MoeRing ring = {};
-    ring.base = smem_u32(stages);
     ring.shape(p.gated ? 2 * ch : ch);
     ring.grain = p.up_grain;
     ring.n = hi - lo;
     ring.part<TEAM>((int)row_bytes, warp % TEAM);
     // the rings' place still holds the logits' parts: the cluster's CTAs have read them
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    fence_proxy_async_shared();
     for (int s = 0; s < kMoeStages; ++s)
         ring.feed(tile_at);
     using Src = std::conditional_t<STAGED, MoeTerms<X::NS, true>, X>;
@@ -995,7 +1053,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1) ll_moe_up_kernel(const __grid_
             sc1 = (p.gated ? p.su : p.sg) + ((size_t)e * fb + c1 / kF8Block) * kb;
         }
         float acc[NT][4];
-        moe_tile<WT, NT>(ring, stages, slot, tile_at, i0, i1, H, sc0, sc1, ntc, src, xrow, acc);
+        moe_tile<WT, NT>(p, ring, misc + 1, stages, slot, tile_at, i0, i1, H, sc0, sc1, ntc, src, xrow, acc);
         if constexpr (TEAM == 2) {  // the second warp's sums to the first (NT is 1)
             float4 *sums = reinterpret_cast<float4 *>(smem + L.team) + ((warp & ~1) + ((tile - lo) & 1)) * 32 + lane;
             if (warp & 1)
@@ -1037,6 +1095,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1) ll_moe_up_kernel(const __grid_
                     put(c, f0 + g + 8, ops_act(v1, p.act));
             }
     }
+    ring.drain(p);
 }
 
 // ---- kernel 2: down projection and the weighted sum ----
@@ -1049,7 +1108,8 @@ __global__ void __launch_bounds__(kMoeThreads, 1) ll_moe_down_kernel(const __gri
     constexpr int TEAM = moe_team(NT), TEAMS = kMoeWarps / TEAM;
     const MoeSmem L = moe_smem(p, false);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const uint32_t *misc = reinterpret_cast<const uint32_t *>(smem + L.misc);
+    volatile uint32_t *misc = reinterpret_cast<volatile uint32_t *>(smem + L.misc);
+    MoeRing ring = moe_ring(smem, L);
     float *part = reinterpret_cast<float *>(smem + L.part);  // [warp][row][16 channels]
     for (int i = tid; i < kMoeWarps * p.rows * 16; i += kMoeThreads)
         part[i] = 0.0f;
@@ -1084,8 +1144,6 @@ __global__ void __launch_bounds__(kMoeThreads, 1) ll_moe_down_kernel(const __gri
         have = min(min(rs, R - r), H - n);
     };
     const uint8_t *stages = smem + warp * (kMoeStages * kMoeStage);
-    MoeRing ring = {};
-    ring.base = smem_u32(stages);
     ring.shape(rs);
     ring.grain = p.down_grain;
     ring.n = items * mine_n;
@@ -1115,7 +1173,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1) ll_moe_down_kernel(const __gri
                 sc1 = p.sd + ((size_t)e * hb + c1 / kF8Block) * kb;
             }
             float acc[NT][4];
-            moe_tile<WT, NT>(ring, stages, slot, tile_at, i0, i1, F, sc0, sc1, ntc, src, hrow, acc);
+            moe_tile<WT, NT>(p, ring, misc + 1, stages, slot, tile_at, i0, i1, F, sc0, sc1, ntc, src, hrow, acc);
             float q0 = 1.0f, q1 = 1.0f;
             if constexpr (WT == LL_W_I8) {
                 q0 = __ldg(p.sd + (size_t)e * H + c0);
@@ -1146,7 +1204,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1) ll_moe_down_kernel(const __gri
                 v += part[w * p.rows * 16 + i];
                 part[w * p.rows * 16 + i] = 0.0f;
             }
-            if (r < n_rows) {
+            if (misc[1] == 0 && r < n_rows) {
                 const size_t o = (size_t)row * p.ldy + n0 + r;
                 if (p.x_type == LL_T_F32)
                     static_cast<float *>(p.y)[o] = v;
@@ -1158,6 +1216,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1) ll_moe_down_kernel(const __gri
         }
         __syncthreads();
     }
+    ring.drain(p);
 }
 
 // Launches both kernels for one weight type (moe_bf16.cu, moe_i8.cu, moe_f8.cu).
