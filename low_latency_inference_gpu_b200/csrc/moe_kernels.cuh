@@ -99,9 +99,9 @@ __host__ __device__ inline MoeSmem moe_smem(const MoeParams &p, bool up)
     s.logits = 0;
     s.part = moe_up16(4 * p.rows * p.experts);  // kernel 1: at most 32 + 64 KB with the logits
     s.team = o, o += up ? kMoeWarps * 512 : 0;  // a team's sums on their way, two tiles'
-    s.x = o;  // kernel 1: the rows of x, where they are staged
     if (!up)
         s.part = o, o += kMoeWarps * p.rows * 16 * 4;
+    s.x = o;  // the rows of x (kernel 2: the activations) where they are staged
     s.total = o;
     return s;
 }
@@ -233,11 +233,32 @@ struct MoeX {
     int cols;
     bool vec;  // rows start on 16 bytes
 
+    // A thread's place in a row: pieces of EP values, 4 EP apart, from column k + t EP on.
+    struct At {
+        const uint8_t *row;
+        int k;
+    };
+    template <int EP>
+    __device__ __forceinline__ At at(uint32_t row, int k) const
+    {
+        return {base + row * row_bytes, k + (int)(threadIdx.x & 3) * EP};
+    }
+    template <int EP>
+    __device__ __forceinline__ void piece(const At &a, int i, uint4 (&v)[RAW<EP>]) const
+    {
+        load<EP>(a.row, a.k + i * 4 * EP, v);
+    }
+    template <int EP>
+    static __device__ __forceinline__ void next(At &a, int pieces)
+    {
+        a.k += pieces * 4 * EP;
+    }
+
     // Values k .. k + EP - 1 of a row, zero from column `cols` on.
     template <int EP>
-    __device__ __forceinline__ void load(uint32_t row, int k, uint4 (&v)[RAW<EP>]) const
+    __device__ __forceinline__ void load(const uint8_t *row, int k, uint4 (&v)[RAW<EP>]) const
     {
-        const uint8_t *p = base + row * row_bytes + (size_t)k * BYTES;
+        const uint8_t *p = row + (size_t)k * BYTES;
         const int n = cols - k;
         if (vec && n >= EP) {
 #pragma unroll
@@ -322,17 +343,29 @@ struct MoeTerms {
     size_t plane;  // bytes
     uint32_t pitch;
 
+    struct At {
+        const uint8_t *p;
+    };
     template <int EP>
-    __device__ __forceinline__ void load(uint32_t row, int k, uint4 (&v)[RAW<EP>]) const
+    __device__ __forceinline__ At at(uint32_t row, int k) const
     {
-        const uint8_t *p = base + (size_t)row * pitch + (size_t)k * 2;
+        return {base + (size_t)row * pitch + (size_t)(k + (int)(threadIdx.x & 3) * EP) * 2};
+    }
+    template <int EP>
+    __device__ __forceinline__ void piece(const At &a, int j, uint4 (&v)[RAW<EP>]) const
+    {
 #pragma unroll
-        for (int s = 0; s < NSP; ++s)
+        for (int s = 0; s < NSP; ++s) {
+            const uint4 *q = reinterpret_cast<const uint4 *>(a.p + s * plane + j * (8 * EP));
 #pragma unroll
-            for (int i = 0; i < EP / 8; ++i) {
-                const uint4 *q = reinterpret_cast<const uint4 *>(p + s * plane) + i;
-                v[s * (EP / 8) + i] = SMEM ? *q : __ldcg(q);
-            }
+            for (int i = 0; i < EP / 8; ++i)
+                v[s * (EP / 8) + i] = SMEM ? q[i] : __ldcg(q + i);
+        }
+    }
+    template <int EP>
+    static __device__ __forceinline__ void next(At &a, int pieces)
+    {
+        a.p += pieces * (8 * EP);
     }
 
     template <int EP, bool PERM>
@@ -362,7 +395,7 @@ __host__ __device__ constexpr int moe_x_pitch(int cols, int wbytes)
 }
 
 // ---- the lists of picked experts, from the ids in shared memory (all threads; rows <= 32) ----
-// act_e[a] = a-th picked expert (rising), its rows are pairs[act_off[a] .. act_off[a + 1]),
+// act_e[a] = a-th picked expert (rising, but for one row by its weight), its rows are pairs[act_off[a] .. act_off[a + 1]),
 // pair = row | slot << 8, rows rising.
 __device__ __forceinline__ void moe_lists(const MoeParams &p, uint8_t *smem, const MoeSmem &L)
 {
@@ -373,6 +406,19 @@ __device__ __forceinline__ void moe_lists(const MoeParams &p, uint8_t *smem, con
     uint16_t *act_off = reinterpret_cast<uint16_t *>(smem + L.act_off);
     uint16_t *pairs = reinterpret_cast<uint16_t *>(smem + L.pairs);
     uint32_t *misc = reinterpret_cast<uint32_t *>(smem + L.misc);
+    if (p.rows == 1) {  // the picked experts as they are
+        const int i = threadIdx.x;
+        if (i < n) {
+            act_e[i] = (uint16_t)ids[i];
+            pairs[i] = (uint16_t)(i << 8);
+        }
+        if (i <= n)
+            act_off[i] = (uint16_t)i;
+        if (i == 0)
+            misc[0] = (uint32_t)n;
+        __syncthreads();
+        return;
+    }
     for (int e = threadIdx.x; e < p.experts; e += blockDim.x)
         mask[e] = 0;
     __syncthreads();
@@ -606,35 +652,44 @@ __device__ __forceinline__ MoeRing moe_ring(uint8_t *smem, const MoeSmem &L)
     return r;
 }
 
-// One tile: acc = (its rows) . x over this warp's columns, in steps of 128 bytes of every row.  i0 / i1:
-// places of this thread's rows g and g + 8 in a stage; sc0 / sc1: their e4m3 scales by 128-column
-// block.  Refills the ring as it goes.  The sums run on in the tensor instruction's accumulators,
-// except that an e4m3 block's (its scale) and an fp32 layer's (the instruction cuts off where fp32
-// would round) are added in fp32.  The loop is kept short: with 16 warps at different places in
-// it, a step unrolled to 24 KB of code waited for instructions half of the time.
+// One tile: acc = (its rows) . x over this warp's columns, in steps of 128 bytes of every row, two at a
+// time (segments and x are zero up to a whole pair).  i0 / i1: places of this thread's rows g and
+// g + 8 in a stage; sc0 / sc1: their e4m3 scales by 128-column block.  Refills the ring as it goes.
+// The sums run on in the tensor instruction's accumulators, except that an e4m3 block's (its
+// scale) and an fp32 layer's (the instruction cuts off where fp32 would round) are added in fp32.
+// The loop is kept short: with 16 warps at different places in it, a body of 24 KB of code
+// waited for instructions half of the time.
 template <int WT, int NT, class Src, class TileAt>
 __device__ __forceinline__ void moe_tile(const MoeParams &p, MoeRing &r, volatile uint32_t *fail, const uint8_t *stages,
-                                         int &slot, TileAt tile_at, int i0, int i1,
-                                         int K, const float *sc0, const float *sc1, int ntc, const Src &src,
-                                         const uint32_t (&xrow)[NT], float (&acc)[NT][4])
+                                         int &slot, TileAt tile_at, int i0, int i1, int K, const float *sc0,
+                                         const float *sc1, int ntc, const Src &src, const uint32_t (&xrow)[NT],
+                                         float (&acc)[NT][4])
 {
     using W = MoeW<WT>;
     constexpr int EP = W::EP, RAW = Src::template RAW<EP>, KS = 128 / W::BYTES, NS = Src::NS;
-    // x from global memory is loaded a step ahead where the registers allow (32)
+    // x from global memory is loaded a step ahead where the registers allow (2 x 32)
     constexpr bool PRE = Src::GLOBAL && 2 * RAW * 4 <= 32;
     constexpr bool FRESH = WT == LL_W_F8 || NS == 3;
-    const int t = threadIdx.x & 3, steps = min(2 * r.step1, (K + KS - 1) / KS);
-    uint4 b[2][RAW], bn[2][RAW];
-    float f0 = 1.0f, f1 = 1.0f, n0 = 1.0f, n1 = 1.0f;  // e4m3: scales of rows g and g + 8
+    const int t = threadIdx.x & 3, last = (K + kF8Block - 1) / kF8Block - 1;
+    uint4 ba[PRE ? 2 : 1][RAW], bb[PRE ? 2 : 1][RAW];
+    float fa0 = 1.0f, fa1 = 1.0f, fb0 = 1.0f, fb1 = 1.0f;  // e4m3: scales of rows g and g + 8
     uint32_t nan0 = 0, nan1 = 0;
-    auto load_step = [&](int st) {
-        if constexpr (PRE)
+    typename Src::At x[NT], ahead;
 #pragma unroll
-            for (int pc = 0; pc < 2; ++pc)
-                src.template load<EP>(xrow[0], st * KS + pc * 4 * EP + t * EP, bn[pc]);
+    for (int nt = 0; nt < NT; ++nt)
+        x[nt] = src.template at<EP>(xrow[nt], 2 * r.step0 * KS);
+    ahead = x[0];
+    int blk = 2 * r.step0;
+    auto load_step = [&](uint4(&to)[PRE ? 2 : 1][RAW], float &f0, float &f1) {
+        if constexpr (PRE) {
+            src.template piece<EP>(ahead, 0, to[0]);
+            src.template piece<EP>(ahead, 1, to[1]);
+            Src::template next<EP>(ahead, 2);
+        }
         if constexpr (WT == LL_W_F8) {
-            n0 = __ldg(sc0 + st);
-            n1 = __ldg(sc1 + st);
+            f0 = __ldg(sc0 + min(blk, last));
+            f1 = __ldg(sc1 + min(blk, last));
+            ++blk;
         }
     };
 #pragma unroll
@@ -642,72 +697,68 @@ __device__ __forceinline__ void moe_tile(const MoeParams &p, MoeRing &r, volatil
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             acc[nt][i] = 0.0f;
-    int st = 2 * r.step0;
-    if (st < steps)
-        load_step(st);
-    while (st < steps) {
+    auto products = [&](float(&d)[NT][4], const uint8_t *r0, const uint8_t *r1, const uint4(&b)[PRE ? 2 : 1][RAW]) {
+#pragma unroll
+        for (int pc = 0; pc < 2; ++pc) {
+            uint32_t a0[EP / 2], a1[EP / 2];
+            W::widen(*reinterpret_cast<const uint4 *>(r0 + 64 * pc), a0, nan0);
+            W::widen(*reinterpret_cast<const uint4 *>(r1 + 64 * pc), a1, nan1);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                if (nt < ntc) {
+                    uint32_t w[NS][EP / 2];
+                    if (PRE && nt == 0) {
+                        Src::template terms<EP, W::PERM>(b[pc * PRE], w);
+                    } else {
+                        uint4 v[RAW];
+                        src.template piece<EP>(x[nt], pc, v);
+                        Src::template terms<EP, W::PERM>(v, w);
+                    }
+#pragma unroll
+                    for (int j = 0; j < EP / 4; ++j)
+#pragma unroll
+                        for (int s = 0; s < NS; ++s)
+                            mma_bf16(d[nt], a0[2 * j], a1[2 * j], a0[2 * j + 1], a1[2 * j + 1], w[s][2 * j],
+                                     w[s][2 * j + 1]);
+                }
+            }
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+            Src::template next<EP>(x[nt], 2);
+    };
+    auto step = [&](const uint8_t *r0, const uint8_t *r1, const uint4(&b)[PRE ? 2 : 1][RAW], float f0, float f1) {
+        if constexpr (FRESH) {
+            float d[NT][4] = {};
+            products(d, r0, r1, b);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                acc[nt][0] = fmaf(d[nt][0], f0, acc[nt][0]);
+                acc[nt][1] = fmaf(d[nt][1], f0, acc[nt][1]);
+                acc[nt][2] = fmaf(d[nt][2], f1, acc[nt][2]);
+                acc[nt][3] = fmaf(d[nt][3], f1, acc[nt][3]);
+            }
+        } else {
+            products(acc, r0, r1, b);
+        }
+    };
+    int st = r.step0;
+    if (st < r.step1)
+        load_step(ba, fa0, fa1);
+    while (st < r.step1) {
         const uint8_t *at = stages + slot * kMoeStage + t * 16;
         const uint8_t *r0 = at + i0 * r.pitch(), *r1 = at + i1 * r.pitch();
-        const int end = min(steps, st + (2 << r.m));
+        const int end = min(r.step1, st + (1 << r.m));
         r.wait(p, slot, fail);
 #pragma unroll 1
         for (; st < end; ++st) {
-            if constexpr (PRE)
-#pragma unroll
-                for (int pc = 0; pc < 2; ++pc)
-#pragma unroll
-                    for (int i = 0; i < RAW; ++i)
-                        b[pc][i] = bn[pc][i];
-            f0 = n0;
-            f1 = n1;
-            if (st + 1 < steps)
-                load_step(st + 1);  // on its way while this step is computed
-            float d[NT][4];
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    d[nt][i] = FRESH ? 0.0f : acc[nt][i];
-#pragma unroll
-            for (int pc = 0; pc < 2; ++pc) {
-                uint32_t a0[EP / 2], a1[EP / 2];
-                W::widen(*reinterpret_cast<const uint4 *>(r0 + 64 * pc), a0, nan0);
-                W::widen(*reinterpret_cast<const uint4 *>(r1 + 64 * pc), a1, nan1);
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    if (nt < ntc) {
-                        uint32_t w[NS][EP / 2];
-                        if (PRE && nt == 0) {
-                            Src::template terms<EP, W::PERM>(b[pc], w);
-                        } else {
-                            uint4 v[RAW];
-                            src.template load<EP>(xrow[nt], st * KS + pc * 4 * EP + t * EP, v);
-                            Src::template terms<EP, W::PERM>(v, w);
-                        }
-#pragma unroll
-                        for (int j = 0; j < EP / 4; ++j)
-#pragma unroll
-                            for (int s = 0; s < NS; ++s)
-                                mma_bf16(d[nt], a0[2 * j], a1[2 * j], a0[2 * j + 1], a1[2 * j + 1], w[s][2 * j],
-                                         w[s][2 * j + 1]);
-                    }
-                }
-            }
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                if constexpr (FRESH) {
-                    acc[nt][0] = fmaf(d[nt][0], f0, acc[nt][0]);
-                    acc[nt][1] = fmaf(d[nt][1], f0, acc[nt][1]);
-                    acc[nt][2] = fmaf(d[nt][2], f1, acc[nt][2]);
-                    acc[nt][3] = fmaf(d[nt][3], f1, acc[nt][3]);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        acc[nt][i] = d[nt][i];
-                }
-            }
-            r0 += 128;
-            r1 += 128;
+            load_step(bb, fb0, fb1);  // on its way while the step before is computed
+            step(r0, r1, ba, fa0, fa1);
+            if (st + 1 < r.step1)
+                load_step(ba, fa0, fa1);
+            step(r0 + 128, r1 + 128, bb, fb0, fb1);
+            r0 += 256;
+            r1 += 256;
         }
         __syncwarp();  // every lane has read the stage
         slot = slot + 1 == kMoeStages ? 0 : slot + 1;
@@ -738,8 +789,8 @@ __device__ __forceinline__ void moe_router_step(const MoeParams &p, uint32_t e0,
 #pragma unroll
     for (int pc = 0; pc < 2; ++pc) {
         const int k = k0 + pc * 32 + t * 8;
-        src.template load<8>(e0, k, v[pc][0]);
-        src.template load<8>(e1, k, v[pc][1]);
+        src.template load<8>(src.base + e0 * src.row_bytes, k, v[pc][0]);
+        src.template load<8>(src.base + e1 * src.row_bytes, k, v[pc][1]);
     }
 #pragma unroll
     for (int pc = 0; pc < 2; ++pc) {
@@ -757,8 +808,8 @@ __device__ __forceinline__ void moe_router_step(const MoeParams &p, uint32_t e0,
 }
 
 // ---- router: logits of every (row, expert), by the whole cluster ----
-template <int XT, int NT>
-__device__ __forceinline__ void moe_logits(const MoeParams &p, uint8_t *smem, const MoeSmem &L)
+template <int XT, int NT, class Meanwhile>
+__device__ __forceinline__ void moe_logits(const MoeParams &p, uint8_t *smem, const MoeSmem &L, Meanwhile meanwhile)
 {
     using X = MoeX<XT>;
     constexpr int EP = 8, KS = 64;
@@ -784,7 +835,7 @@ __device__ __forceinline__ void moe_logits(const MoeParams &p, uint8_t *smem, co
 #pragma unroll
                         for (int pc = 0; pc < 2; ++pc) {
                             const int k = st * KS + pc * 32 + t * EP;
-                            src.template load<EP>((uint32_t)min(nt * 8 + g, p.rows - 1), k, xb[nt][pc]);
+                            src.template load<EP>(src.base + (size_t)min(nt * 8 + g, p.rows - 1) * src.row_bytes, k, xb[nt][pc]);
                         }
                 uint32_t a0[2][3][EP / 2], a1[2][3][EP / 2];
                 if (p.router_f32)
@@ -829,24 +880,29 @@ __device__ __forceinline__ void moe_logits(const MoeParams &p, uint8_t *smem, co
         }
     }
     __syncwarp();
-    cluster_sync();
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    meanwhile();  // while the others come
+    __syncwarp();
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     float *logits = reinterpret_cast<float *>(smem + L.logits);
     const uint32_t pa = smem_u32(part);
-    for (int i = tid; i < tp * p.experts; i += 32 * WARPS) {
-        const int e = i / tp, row = i - e * tp;  // consecutive threads: consecutive words
+    const int n_out = p.rows * p.experts, stride = mt_n * 16 * tp;
+    for (int i = tid; i < n_out; i += 32 * WARPS) {
+        // consecutive threads: consecutive rows of an expert where there are several, so consecutive words
+        const int e = i / p.rows, row = i - e * p.rows;
+        const uint32_t at = pa + (uint32_t)(e * tp + row) * 4u;
         float v = 0.0f;
+#pragma unroll 4
         for (int ks = 0; ks < ksub; ++ks) {
-            const uint32_t at = pa + (uint32_t)(ks * mt_n * 16 * tp + i) * 4u;
             float q[kMoeCluster];
 #pragma unroll
             for (int r = 0; r < kMoeCluster; ++r)
-                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(q[r]) : "r"(mapa(at, (uint32_t)r)) : "memory");
+                asm("ld.shared::cluster.f32 %0, [%1];" : "=f"(q[r]) : "r"(mapa(at + (uint32_t)(ks * stride) * 4u, (uint32_t)r)));
 #pragma unroll
             for (int r = 0; r < kMoeCluster; ++r)
                 v += q[r];
         }
-        if (row < p.rows)
-            logits[row * p.experts + e] = v;
+        logits[row * p.experts + e] = v;
     }
     // the peers' partial sums are read; matched by the wait before the rings fill
     __syncwarp();
@@ -896,23 +952,41 @@ __device__ __forceinline__ void moe_pick(const MoeParams &p, uint8_t *smem, cons
                 sum += __shfl_xor_sync(0xffffffffu, sum, off);
         }
         uint32_t mine = 0;  // lane j: the j-th picked expert
-#pragma unroll 1
-        for (int j = 0; j < p.top_k; ++j) {
-            uint32_t best = 0u, at = 0xffffffffu;
+        if constexpr (PER <= 2) {
+            // an expert's place is the number of experts before it: by logit, of equal ones by index
+            int place[PER] = {};
+            for (int e = 0; e < p.experts; ++e) {
+                const uint32_t k = __shfl_sync(0xffffffffu, PER == 2 && e >= 32 ? key[PER - 1] : key[0], e & 31);
 #pragma unroll
-            for (int i = PER - 1; i >= 0; --i)
-                if (key[i] >= best && key[i] != 0u) {  // of equal keys the lowest index
-                    best = key[i];
-                    at = (uint32_t)(lane + 32 * i);
-                }
-            const uint32_t top_key = __reduce_max_sync(0xffffffffu, best);
-            at = __reduce_min_sync(0xffffffffu, best == top_key ? at : 0xffffffffu);
-            if (lane == j)
-                mine = at;
+                for (int i = 0; i < PER; ++i)
+                    place[i] += k > key[i] || (k == key[i] && e < lane + 32 * i) ? 1 : 0;
+            }
+            uint32_t *slots = reinterpret_cast<uint32_t *>(ids + row * p.top_k);
 #pragma unroll
             for (int i = 0; i < PER; ++i)
-                if (at == (uint32_t)(lane + 32 * i))
-                    key[i] = 0u;
+                if (lane + 32 * i < p.experts && place[i] < p.top_k)
+                    slots[place[i]] = (uint32_t)(lane + 32 * i);
+            __syncwarp();
+            mine = lane < p.top_k ? slots[lane] : 0u;
+        } else {
+#pragma unroll 1
+            for (int j = 0; j < p.top_k; ++j) {
+                uint32_t best = 0u, at = 0xffffffffu;
+#pragma unroll
+                for (int i = PER - 1; i >= 0; --i)
+                    if (key[i] >= best && key[i] != 0u) {  // of equal keys the lowest index
+                        best = key[i];
+                        at = (uint32_t)(lane + 32 * i);
+                    }
+                const uint32_t top_key = __reduce_max_sync(0xffffffffu, best);
+                at = __reduce_min_sync(0xffffffffu, best == top_key ? at : 0xffffffffu);
+                if (lane == j)
+                    mine = at;
+#pragma unroll
+                for (int i = 0; i < PER; ++i)
+                    if (at == (uint32_t)(lane + 32 * i))
+                        key[i] = 0u;
+            }
         }
         const float ex = lane < p.top_k ? expf(lg[mine] - top) : 0.0f;
         if (p.renorm) {
@@ -940,7 +1014,7 @@ __device__ __forceinline__ void moe_stage_x(const MoeParams &p, uint8_t *to)
     for (int i = threadIdx.x; i < p.rows * chunks; i += (int)blockDim.x) {
         const int row = i / chunks, c = i - row * chunks;
         uint4 v[X::template RAW<8>];
-        src.template load<8>((uint32_t)row, c * 8, v);
+        src.template load<8>(src.base + (size_t)row * src.row_bytes, c * 8, v);
         uint32_t w[X::NS][4];
         X::template terms<8, W::PERM>(v, w);
 #pragma unroll
@@ -967,9 +1041,10 @@ __global__ void __launch_bounds__(kMoeThreads, 1) ll_moe_up_kernel(const __grid_
     MoeRing ring = moe_ring(smem, L);
     griddep_wait();
     griddep_launch_dependents();
-    if constexpr (STAGED)
-        moe_stage_x<WT, XT>(p, smem + L.x);
-    moe_logits<XT, NT>(p, smem, L);
+    moe_logits<XT, NT>(p, smem, L, [&] {
+        if constexpr (STAGED)
+            moe_stage_x<WT, XT>(p, smem + L.x);
+    });
     if (p.experts <= 64)
         moe_pick<2>(p, smem, L);
     else
@@ -1099,7 +1174,8 @@ __global__ void __launch_bounds__(kMoeThreads, 1) ll_moe_up_kernel(const __grid_
 }
 
 // ---- kernel 2: down projection and the weighted sum ----
-template <int WT, int NSH, int NT>
+// STAGED: the activations (all rows of all picked experts) in shared memory, else read from L2 as it goes.
+template <int WT, int NSH, int NT, bool STAGED>
 __global__ void __launch_bounds__(kMoeThreads, 1) ll_moe_down_kernel(const __grid_constant__ MoeParams p)
 {
     using W = MoeW<WT>;
@@ -1150,8 +1226,19 @@ __global__ void __launch_bounds__(kMoeThreads, 1) ll_moe_down_kernel(const __gri
     ring.part<TEAM>((int)row_bytes, warp % TEAM);
     for (int s = 0; s < kMoeStages; ++s)
         ring.feed(tile_at);
-    const MoeTerms<NSH, false> src = {reinterpret_cast<const uint8_t *>(p.hid), (size_t)p.hid_plane * 2,
-                                      (uint32_t)p.hid_ld * 2u};
+    MoeTerms<NSH, STAGED> src;
+    if constexpr (STAGED) {
+        const int pitch = moe_x_pitch(F, W::BYTES), chunks = p.hid_ld / 8, n = p.rows * p.top_k;
+        for (int i = tid; i < NSH * n * chunks; i += kMoeThreads) {
+            const int row = i / chunks, c = i - row * chunks, s = row / n;  // rows of all planes
+            *reinterpret_cast<uint4 *>(smem + L.x + (size_t)row * pitch + c * 16) =
+                __ldcg(reinterpret_cast<const uint4 *>(p.hid + (size_t)s * p.hid_plane + (size_t)(row - s * n) * p.hid_ld) + c);
+        }
+        __syncthreads();
+        src = {smem + L.x, (size_t)n * (size_t)pitch, (uint32_t)pitch};
+    } else {
+        src = {reinterpret_cast<const uint8_t *>(p.hid), (size_t)p.hid_plane * 2, (uint32_t)p.hid_ld * 2u};
+    }
     int slot = 0;
     float *mine = part + warp * p.rows * 16;
     for (int item = 0; item < items; ++item) {
@@ -1293,11 +1380,15 @@ inline int moe_clusters(const void *fn, int *n)
 template <int WT, int XT, int NT, bool STAGED>
 int launch_moe_typed(MoeParams &p, int device, cudaStream_t st)
 {
-    static bool up_ready[kOpsMaxDevices], down_ready[kOpsMaxDevices];
+    static bool up_ready[kOpsMaxDevices], down_ready[2][kOpsMaxDevices];
     static int sm_count[kOpsMaxDevices], cluster_count[kOpsMaxDevices];
     constexpr int NSH = XT == LL_T_F32 ? 3 : 2;
     const void *up = reinterpret_cast<const void *>(&ll_moe_up_kernel<WT, XT, NT, STAGED>);
-    const void *down = reinterpret_cast<const void *>(&ll_moe_down_kernel<WT, NSH, NT>);
+    const long long staged_h = moe_smem(p, false).total +
+                               (long long)NSH * p.rows * p.top_k * moe_x_pitch(p.inter, MoeW<WT>::BYTES);
+    const bool stage_h = NT == 1 && staged_h <= kMoeSmemCap;
+    const void *down = stage_h ? reinterpret_cast<const void *>(&ll_moe_down_kernel<WT, NSH, NT, NT == 1>)
+                               : reinterpret_cast<const void *>(&ll_moe_down_kernel<WT, NSH, NT, false>);
     int sms = __atomic_load_n(&sm_count[device], __ATOMIC_ACQUIRE);
     if (sms == 0) {
         LL_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
@@ -1311,7 +1402,7 @@ int launch_moe_typed(MoeParams &p, int device, cudaStream_t st)
     }
     LL_TRY(moe_launch(up, up_ready, p, moe_smem(p, true).total + (STAGED ? moe_x_bytes<WT, XT>(p) : 0),
                       clusters * kMoeCluster, kMoeCluster, false, device, st));
-    return moe_launch(down, down_ready, p, moe_smem(p, false).total, std::min(sms, p.hidden), 0, true, device, st);
+    return moe_launch(down, down_ready[stage_h], p, stage_h ? (int)staged_h : moe_smem(p, false).total, std::min(sms, p.hidden), 0, true, device, st);
 }
 
 // Up to 8 rows whose terms fit beside the rings take the kernel that stages x.
