@@ -658,12 +658,14 @@ __device__ __forceinline__ MoeRing moe_ring(uint8_t *smem, const MoeSmem &L)
 // The sums run on in the tensor instruction's accumulators, except that an e4m3 block's (its
 // scale) and an fp32 layer's (the instruction cuts off where fp32 would round) are added in fp32.
 // The loop is kept short: with 16 warps at different places in it, a body of 24 KB of code
-// waited for instructions half of the time.
-template <int WT, int NT, class Src, class TileAt>
+// waited for instructions half of the time.  NT: n-tiles that are computed (of NTA that have room);
+// an expert with up to 8 rows, nearly every one, takes the copy with NT = 1: in the other one the
+// instructions of the n-tiles that it lacks would be issued all the same, switched off one by one.
+template <int WT, int NT, int NTA, class Src, class TileAt>
 __device__ __forceinline__ void moe_tile(const MoeParams &p, MoeRing &r, volatile uint32_t *fail, const uint8_t *stages,
                                          int &slot, TileAt tile_at, int i0, int i1, int K, const float *sc0,
-                                         const float *sc1, int ntc, const Src &src, const uint32_t (&xrow)[NT],
-                                         float (&acc)[NT][4])
+                                         const float *sc1, int ntc, const Src &src, const uint32_t (&xrow)[NTA],
+                                         float (&out)[NTA][4])
 {
     using W = MoeW<WT>;
     constexpr int EP = W::EP, RAW = Src::template RAW<EP>, KS = 128 / W::BYTES, NS = Src::NS;
@@ -674,6 +676,7 @@ __device__ __forceinline__ void moe_tile(const MoeParams &p, MoeRing &r, volatil
     uint4 ba[PRE ? 2 : 1][RAW], bb[PRE ? 2 : 1][RAW];
     float fa0 = 1.0f, fa1 = 1.0f, fb0 = 1.0f, fb1 = 1.0f;  // e4m3: scales of rows g and g + 8
     uint32_t nan0 = 0, nan1 = 0;
+    float acc[NT][4];
     typename Src::At x[NT], ahead;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -705,7 +708,7 @@ __device__ __forceinline__ void moe_tile(const MoeParams &p, MoeRing &r, volatil
             W::widen(*reinterpret_cast<const uint4 *>(r1 + 64 * pc), a1, nan1);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                if (nt < ntc) {
+                if (NT == 1 || nt < ntc) {
                     uint32_t w[NS][EP / 2];
                     if (PRE && nt == 0) {
                         Src::template terms<EP, W::PERM>(b[pc * PRE], w);
@@ -775,6 +778,11 @@ __device__ __forceinline__ void moe_tile(const MoeParams &p, MoeRing &r, volatil
         for (int nt = 0; nt < NT; ++nt)
             acc[nt][0] *= s0, acc[nt][1] *= s0, acc[nt][2] *= s1, acc[nt][3] *= s1;
     }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            out[nt][i] = acc[nt][i];
 }
 
 // This thread's pieces of the router's rows e0 and e1 (columns k0 .. k0 + 63) as bf16 terms.
@@ -1128,7 +1136,10 @@ __global__ void __launch_bounds__(kMoeThreads, 1) ll_moe_up_kernel(const __grid_
             sc1 = (p.gated ? p.su : p.sg) + ((size_t)e * fb + c1 / kF8Block) * kb;
         }
         float acc[NT][4];
-        moe_tile<WT, NT>(p, ring, misc + 1, stages, slot, tile_at, i0, i1, H, sc0, sc1, ntc, src, xrow, acc);
+        if (NT == 1 || ntc == 1)
+            moe_tile<WT, 1, NT>(p, ring, misc + 1, stages, slot, tile_at, i0, i1, H, sc0, sc1, 1, src, xrow, acc);
+        else
+            moe_tile<WT, NT, NT>(p, ring, misc + 1, stages, slot, tile_at, i0, i1, H, sc0, sc1, ntc, src, xrow, acc);
         if constexpr (TEAM == 2) {  // the second warp's sums to the first (NT is 1)
             float4 *sums = reinterpret_cast<float4 *>(smem + L.team) + ((warp & ~1) + ((tile - lo) & 1)) * 32 + lane;
             if (warp & 1)
@@ -1159,7 +1170,9 @@ __global__ void __launch_bounds__(kMoeThreads, 1) ll_moe_up_kernel(const __grid_
             for (int i = lane; i < cnt * (p.hid_ld - F); i += 32)
                 put(i / (p.hid_ld - F), F + i % (p.hid_ld - F), 0.0f);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt) {
+            if (nt >= ntc)
+                break;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const int c = nt * 8 + 2 * t + j;  // column: one of the expert's rows of x
@@ -1169,6 +1182,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1) ll_moe_up_kernel(const __grid_
                 if (!p.gated && c < cnt && g + 8 < chs)
                     put(c, f0 + g + 8, ops_act(v1, p.act));
             }
+        }
     }
     ring.drain(p);
 }
@@ -1260,14 +1274,19 @@ __global__ void __launch_bounds__(kMoeThreads, 1) ll_moe_down_kernel(const __gri
                 sc1 = p.sd + ((size_t)e * hb + c1 / kF8Block) * kb;
             }
             float acc[NT][4];
-            moe_tile<WT, NT>(p, ring, misc + 1, stages, slot, tile_at, i0, i1, F, sc0, sc1, ntc, src, hrow, acc);
+            if (NT == 1 || ntc == 1)
+                moe_tile<WT, 1, NT>(p, ring, misc + 1, stages, slot, tile_at, i0, i1, F, sc0, sc1, 1, src, hrow, acc);
+            else
+                moe_tile<WT, NT, NT>(p, ring, misc + 1, stages, slot, tile_at, i0, i1, F, sc0, sc1, ntc, src, hrow, acc);
             float q0 = 1.0f, q1 = 1.0f;
             if constexpr (WT == LL_W_I8) {
                 q0 = __ldg(p.sd + (size_t)e * H + c0);
                 q1 = __ldg(p.sd + (size_t)e * H + c1);
             }
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int nt = 0; nt < NT; ++nt) {
+                if (nt >= ntc)
+                    break;
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     const int c = nt * 8 + 2 * t + j;
@@ -1280,6 +1299,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1) ll_moe_down_kernel(const __gri
                             mine[row * 16 + rr + g + 8] = fmaf(w, acc[nt][2 + j] * q1, mine[row * 16 + rr + g + 8]);
                     }
                 }
+            }
             __syncwarp();  // another lane may add to the same place for the next expert
         }
         __syncthreads();
