@@ -12,8 +12,8 @@
 // tensor memory; at these widths the memory is the bound and the warp-level instruction is at a
 // few per cent of its rate.
 // Every warp works alone: it takes whole tiles (up to 16 weight rows, all columns), copies their
-// rows into a ring of its own (bulk copies, a row's segment each, stages of 4 KB, refilled as soon
-// as a stage is read) and keeps the tile's sums in registers.  Nothing is handed from warp to warp
+// rows into a ring of its own (asynchronous copies, stages of 4 KB, refilled as soon as a stage is
+// read) and keeps the tile's sums in registers.  Nothing is handed from warp to warp
 // on the way, so the warps drift apart and cover each other's latencies.
 //
 // Precision: weights are exact in bf16 (int8 and e4m3 too; their scales multiply fp32 sums).  x
@@ -514,11 +514,36 @@ __device__ __forceinline__ void moe_copy(uint32_t dst, int rows, int m, int half
     }
 }
 
-// Rows that do not start on 16 bytes: out of the way of the others' instructions.
+// n whole segments (nothing of them behind a row's end), one row or two half rows at a time: four
+// instructions a copy.  m = 0 takes an even n.
+__device__ __forceinline__ void moe_copy_whole(uint32_t dst, int n, int m, const uint8_t *src, int row_bytes)
+{
+    const int lane = threadIdx.x & 31, hw = lane >> 4, pl = (lane & 15) * 16, pitch = (256 << m) + 64;
+    src += pl;
+    dst += (uint32_t)pl;
+    if (m == 0) {
+        src += (size_t)hw * (size_t)row_bytes;
+        dst += (uint32_t)(hw * pitch);
+#pragma unroll 4
+        for (int i = 0; i < n; i += 2, src += 2 * (size_t)row_bytes, dst += 2u * (uint32_t)pitch)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+    } else {
+        src += hw * 256;
+        dst += (uint32_t)(hw * 256);
+        for (int i = 0; i < n; ++i, src += (size_t)row_bytes, dst += (uint32_t)pitch)
+#pragma unroll 2
+            for (int j = 0; j < 256 << m; j += 512)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + (uint32_t)j), "l"(src + j) : "memory");
+    }
+}
+
+// Rows that do not start on 16 bytes, or end within the segment: out of the way of the others' instructions.
 static __device__ __noinline__ void moe_copy_small(int grain, uint32_t dst, int rows, int m, int half, int have,
                                                    const uint8_t *s0, const uint8_t *s1, int row_bytes, int off, int end)
 {
-    if (grain >= 8)
+    if (grain >= 16)
+        moe_copy<16>(dst, rows, m, half, have, s0, s1, row_bytes, off, end);
+    else if (grain >= 8)
         moe_copy<8>(dst, rows, m, half, have, s0, s1, row_bytes, off, end);
     else if (grain >= 4)
         moe_copy<4>(dst, rows, m, half, have, s0, s1, row_bytes, off, end);
@@ -529,13 +554,14 @@ static __device__ __noinline__ void moe_copy_small(int grain, uint32_t dst, int 
 // Tiles of `rows` rows come in segments of 256 << m bytes per row, m as large as 16 rows' 256 bytes
 // allow (a pitch of 64 mod 128 bytes, so that the 8 rows that a quarter of the warp reads do not
 // collide); what lies behind a row's end is zero up to a whole step.  The warp issues its tiles'
-// segments in order, kMoeStages ahead: bulk copies on a barrier per stage, or (rows that do not
-// start on 16 bytes) one group of small copies per segment, empty ones past the last, so that the
-// count of groups tells which has landed.
+// segments in order, kMoeStages ahead: bulk copies on a barrier per stage for up to 4 rows, else one
+// group of 16-byte (or smaller) copies per segment, empty ones past the last, so that the count of
+// groups tells which has landed.
 struct MoeRing {
     uint32_t base, bars;  // shared-memory addresses of this warp's stages and of a barrier for each
     uint32_t laps;        // of each stage's barrier, the phase that its next wait is for (a bit)
     bool ok;              // no wait has run out
+    bool bulk;            // up to 4 rows: bulk copies (a lane's takes 12 instructions, whatever its length)
     int rows, m, grain;
     int q, n;       // next tile to be copied, number of tiles
     int slot, off, row_bytes;
@@ -578,7 +604,7 @@ struct MoeRing {
             if (off == begin)
                 tile_at(q, s0, s1, half, have);
             const uint32_t dst = base + (uint32_t)(slot * kMoeStage);
-            if (grain >= 16) {
+            if (bulk) {
                 // a row's segment per lane; a barrier of the stage counts the bytes
                 const int lane = threadIdx.x & 31, h = lane < half ? lane : lane - half, len = min(seg(), end - off);
                 const bool mine = lane < rows && h < have;
@@ -594,6 +620,10 @@ struct MoeRing {
                         st_shared_v4(d + (uint32_t)i, make_uint4(0u, 0u, 0u, 0u));
                     fence_proxy_async_shared();  // before a later segment's copy to the same place
                 }
+            } else if (grain >= 16 && have >= half && off + seg() <= end && (m > 0 || (half & 1) == 0)) {
+                moe_copy_whole(dst, half, m, s0 + off, row_bytes);
+                if (rows > half)
+                    moe_copy_whole(dst + (uint32_t)(half * pitch()), half, m, s1 + off, row_bytes);
             } else {
                 moe_copy_small(grain, dst, rows, m, half, have, s0, s1, row_bytes, off, end);
             }
@@ -610,7 +640,7 @@ struct MoeRing {
     // The segment in stage `at` has landed, for the whole warp.
     __device__ __forceinline__ void wait(const MoeParams &p, int at, volatile uint32_t *fail)
     {
-        if (grain >= 16) {
+        if (bulk) {
             if (ok)
                 ok = ops_wait_warp(bars + 8u * (uint32_t)at, (laps >> at) & 1u, p.wait_ns, fail, p.status, 6);
             laps ^= 1u << at;
@@ -1102,6 +1132,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1) ll_moe_up_kernel(const __grid_
     const uint8_t *stages = smem + warp * (kMoeStages * kMoeStage);
     ring.shape(p.gated ? 2 * ch : ch);
     ring.grain = p.up_grain;
+    ring.bulk = ring.grain >= 16 && ring.rows <= 4;
     ring.n = hi - lo;
     ring.part<TEAM>((int)row_bytes, warp % TEAM);
     // the rings' place still holds the logits' parts: the cluster's CTAs have read them
@@ -1236,6 +1267,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1) ll_moe_down_kernel(const __gri
     const uint8_t *stages = smem + warp * (kMoeStages * kMoeStage);
     ring.shape(rs);
     ring.grain = p.down_grain;
+    ring.bulk = ring.grain >= 16 && ring.rows <= 4;
     ring.n = items * mine_n;
     ring.part<TEAM>((int)row_bytes, warp % TEAM);
     for (int s = 0; s < kMoeStages; ++s)
