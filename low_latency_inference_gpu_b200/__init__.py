@@ -18,6 +18,7 @@ Reference mapping (mamedov-ma/low_latency_inference_gpu):
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 from dataclasses import dataclass
 from typing import List, Optional, Sequence
@@ -675,16 +676,19 @@ def dense_mbyv_packed(Wcm_ptr: int, bpad_ptr: int, x_ptr: int, y_ptr: int, M: in
 def quantize_fp8(x_ptr: int, x_type: int, rows: int, dim: int, q_ptr: int, s_ptr: int, ldx: int = 0, ldq: int = 0,
                  pow2: bool = False, stream: int = 0):
     """Rows of x (T_F32, T_BF16 or T_F16) to e4m3 bytes and one fp32 scale per row and 128 columns (ll_quantize_fp8)."""
-    _check(lib().ll_quantize_fp8(x_ptr or None, x_type, rows, dim, ldx, int(pow2), q_ptr or None, ldq, s_ptr or None,
-                                 stream or None))
+    rc = lib().ll_quantize_fp8(x_ptr, x_type, rows, dim, ldx, pow2, q_ptr, ldq, s_ptr, stream)
+    if rc:
+        _check(rc)
 
 
 def dense_fp8(W_ptr: int, sw_ptr: int, b_ptr: int, x_ptr: int, sx_ptr: int, y_ptr: int, rows: int, M: int, K: int,
               act: int = ACT_IDENTITY, y_type: int = T_F32, sy_ptr: int = 0, ldw: int = 0, ldx: int = 0, ldy: int = 0,
               stream: int = 0):
     """y = act(W x + b) on e4m3 operands with block scales (ll_dense_fp8); y_type T_F8 needs sy_ptr."""
-    _check(lib().ll_dense_fp8(W_ptr or None, sw_ptr or None, b_ptr or None, x_ptr or None, sx_ptr or None,
-                              y_ptr or None, sy_ptr or None, y_type, rows, M, K, ldw, ldx, ldy, act, stream or None))
+    rc = lib().ll_dense_fp8(W_ptr, sw_ptr, b_ptr, x_ptr, sx_ptr, y_ptr, sy_ptr, y_type, rows, M, K, ldw, ldx, ldy, act,
+                            stream)
+    if rc:
+        _check(rc)
 
 
 def ops_check(stream: int = 0):
@@ -696,7 +700,7 @@ def ops_check(stream: int = 0):
 MOE_MAX_ROWS, MOE_MAX_EXPERTS, MOE_MAX_TOPK, MOE_MAX_DIM = 32, 256, 16, 65536
 
 
-@dataclass
+@dataclass(frozen=True)
 class MoE:
     """Description of a mixture-of-experts layer (ll_moe_desc)."""
     hidden: int
@@ -710,12 +714,13 @@ class MoE:
     router_type: int = T_BF16
     renormalize: bool = True
 
+    @functools.cached_property
     def desc(self) -> MoEDesc:
         return MoEDesc(self.hidden, self.inter, self.n_experts, self.top_k, self.act, int(self.gated), self.wtype,
                        self.x_type, self.router_type, int(self.renormalize))
 
 
-@dataclass
+@dataclass(frozen=True)
 class MoEWeights:
     """Device pointers of a layer's matrices and scales (ll_moe_weights); 0 where there is none."""
     router: int
@@ -726,24 +731,26 @@ class MoEWeights:
     up_scale: int = 0
     down_scale: int = 0
 
+    @functools.cached_property
     def struct(self) -> MoEWeightsStruct:
-        return MoEWeightsStruct(self.router or None, self.gate or None, self.up or None, self.down or None,
-                                self.gate_scale or None, self.up_scale or None, self.down_scale or None)
+        return MoEWeightsStruct(self.router, self.gate, self.up, self.down, self.gate_scale, self.up_scale,
+                                self.down_scale)
 
 
 def moe_workspace_bytes(moe: MoE, rows: int) -> int:
     """Bytes of device memory that moe_forward needs beside its operands for up to `rows` rows."""
     n = ctypes.c_size_t()
-    _check(lib().ll_moe_workspace_bytes(ctypes.byref(moe.desc()), rows, ctypes.byref(n)))
+    _check(lib().ll_moe_workspace_bytes(ctypes.byref(moe.desc), rows, ctypes.byref(n)))
     return n.value
 
 
 def moe_forward(moe: MoE, weights: MoEWeights, x_ptr: int, y_ptr: int, rows: int, work_ptr: int, work_bytes: int,
                 ids_ptr: int = 0, probs_ptr: int = 0, ldx: int = 0, ldy: int = 0, stream: int = 0):
     """One mixture-of-experts layer for up to MOE_MAX_ROWS rows (ll_moe_forward), device pointers."""
-    _check(lib().ll_moe_forward(ctypes.byref(moe.desc()), ctypes.byref(weights.struct()), x_ptr or None, ldx,
-                                y_ptr or None, ldy, rows, ids_ptr or None, probs_ptr or None, work_ptr or None,
-                                work_bytes, stream or None))
+    rc = lib().ll_moe_forward(moe.desc, weights.struct, x_ptr, ldx, y_ptr, ldy, rows, ids_ptr, probs_ptr, work_ptr,
+                              work_bytes, stream)
+    if rc:
+        _check(rc)
 
 
 def plan_net(net: Net, W=None, b=None, scales=None, opts: Optional[EngineOpts] = None, want_images: bool = False):

@@ -13,6 +13,8 @@ Tolerances, per output, from the sums of magnitudes (A_v = sum |a| |b| of each p
 The picked experts must be a top_k up to t_l: any expert left out has a logit at most 2 t_l above
 one that was picked; the reference continues with the device's choice.
 """
+import dataclasses
+
 import numpy as np
 import pytest
 
@@ -61,7 +63,7 @@ def test_refuses_arguments():
     refused(ll.moe_forward, bad, m, w, 16, 16, 1, 256, big, ldy=63)
     assert "workspace" in refused(ll.moe_forward, bad, m, w, 16, 16, 1, 256, ll.moe_workspace_bytes(m, 1) - 1)
     for name in ("router", "gate", "up", "down"):
-        refused(ll.moe_forward, bad, m, ll.MoEWeights(**{**w.__dict__, name: 0}), 16, 16, 1, 256, big)
+        refused(ll.moe_forward, bad, m, dataclasses.replace(w, **{name: 0}), 16, 16, 1, 256, big)
     for t in (ll.W_I8, ll.W_F8):
         refused(ll.moe_forward, bad, desc(wtype=t), w, 16, 16, 1, 256, big)
     ll.moe_forward(m, w, 0, 0, 0, 0, 0)  # no rows: nothing to do
