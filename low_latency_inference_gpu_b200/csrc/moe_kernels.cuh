@@ -730,7 +730,9 @@ __device__ __forceinline__ void moe_tile(const MoeParams &p, MoeRing &r, volatil
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             acc[nt][i] = 0.0f;
-    auto products = [&](float(&d)[NT][4], const uint8_t *r0, const uint8_t *r1, const uint4(&b)[PRE ? 2 : 1][RAW]) {
+    // d: the products of the first terms of x, e: those of the others (FRESH; else the same sums)
+    auto products = [&](float(&d)[NT][4], float(&e)[NT][4], const uint8_t *r0, const uint8_t *r1,
+                        const uint4(&b)[PRE ? 2 : 1][RAW]) {
 #pragma unroll
         for (int pc = 0; pc < 2; ++pc) {
             uint32_t a0[EP / 2], a1[EP / 2];
@@ -751,8 +753,8 @@ __device__ __forceinline__ void moe_tile(const MoeParams &p, MoeRing &r, volatil
                     for (int j = 0; j < EP / 4; ++j)
 #pragma unroll
                         for (int s = 0; s < NS; ++s)
-                            mma_bf16(d[nt], a0[2 * j], a1[2 * j], a0[2 * j + 1], a1[2 * j + 1], w[s][2 * j],
-                                     w[s][2 * j + 1]);
+                            mma_bf16(s == 0 ? d[nt] : e[nt], a0[2 * j], a1[2 * j], a0[2 * j + 1], a1[2 * j + 1],
+                                     w[s][2 * j], w[s][2 * j + 1]);
                 }
             }
         }
@@ -761,9 +763,20 @@ __device__ __forceinline__ void moe_tile(const MoeParams &p, MoeRing &r, volatil
             Src::template next<EP>(x[nt], 2);
     };
     auto step = [&](const uint8_t *r0, const uint8_t *r1, const uint4(&b)[PRE ? 2 : 1][RAW], float f0, float f1) {
-        if constexpr (FRESH) {
+        if constexpr (NS == 3) {
+            // fp32: the large products apart from the small ones, so that fewer cuts fall on the large sums
+            float d[NT][4] = {}, e[NT][4] = {};
+            products(d, e, r0, r1, b);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                acc[nt][0] = fmaf(d[nt][0] + e[nt][0], f0, acc[nt][0]);
+                acc[nt][1] = fmaf(d[nt][1] + e[nt][1], f0, acc[nt][1]);
+                acc[nt][2] = fmaf(d[nt][2] + e[nt][2], f1, acc[nt][2]);
+                acc[nt][3] = fmaf(d[nt][3] + e[nt][3], f1, acc[nt][3]);
+            }
+        } else if constexpr (FRESH) {
             float d[NT][4] = {};
-            products(d, r0, r1, b);
+            products(d, d, r0, r1, b);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 acc[nt][0] = fmaf(d[nt][0], f0, acc[nt][0]);
@@ -772,7 +785,7 @@ __device__ __forceinline__ void moe_tile(const MoeParams &p, MoeRing &r, volatil
                 acc[nt][3] = fmaf(d[nt][3], f1, acc[nt][3]);
             }
         } else {
-            products(acc, r0, r1, b);
+            products(acc, acc, r0, r1, b);
         }
     };
     int st = r.step0;
