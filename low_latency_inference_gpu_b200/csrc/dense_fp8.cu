@@ -827,14 +827,17 @@ __global__ void __launch_bounds__(kDlThreads, 1) ll_dense_fp8_large_kernel(const
                 for (int i = 0; i < 4; ++i)
                     f[i] = fx[i] * fw[i];
                 load_scales(kb0 + 4);
-                for (int i = 0; i < 4 && kb0 + i < p.nkb; ++i, ++g) {
-                    const int b = g & 1;
-                    if (!ops_wait_warp(b_accf(b), (g / 2) & 1, p.wait_ns, fail, p.status, 4)) {
-                        ok = false;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (kb0 + i >= p.nkb)
                         break;
-                    }
+                    const int b = g & 1;
+                    ok = ops_wait_warp(b_accf(b), (g / 2) & 1, p.wait_ns, fail, p.status, 4);
+                    if (!ok)
+                        break;
+                    ++g;
                     tc_fence_after();
-                    const float s = i == 0 ? f[0] : i == 1 ? f[1] : i == 2 ? f[2] : f[3];
+                    const float s = f[i];
                     const uint32_t at = tq + (uint32_t)(b * kDlN);
                     uint32_t v0[32], v1[32];
                     tc_ld_32cols_async(at, v0);

@@ -137,7 +137,7 @@ __device__ __forceinline__ void split_pair(float a, float b, uint32_t (&w)[NS])
 __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1)
 {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, "
         "%2, %3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -1006,6 +1006,7 @@ __device__ __forceinline__ void moe_pick(const MoeParams &p, uint8_t *smem, cons
         if constexpr (PER <= 2) {
             // an expert's place is the number of experts before it: by logit, of equal ones by index
             int place[PER] = {};
+#pragma unroll 8
             for (int e = 0; e < p.experts; ++e) {
                 const uint32_t k = __shfl_sync(0xffffffffu, PER == 2 && e >= 32 ? key[PER - 1] : key[0], e & 31);
 #pragma unroll
