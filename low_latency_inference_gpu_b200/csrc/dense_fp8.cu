@@ -65,16 +65,6 @@ __device__ __forceinline__ void tc_ld_16cols(uint32_t taddr, float (&v)[16])
         v[i] = __uint_as_float(r[i]);
 }
 
-__device__ __forceinline__ float4 ld_cluster_v4(uint32_t cluster_addr)
-{
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-                 : "r"(cluster_addr)
-                 : "memory");
-    return v;
-}
-
 // Four consecutive outputs of row `row` from channel m on; a warp holds one row's 128 channels of
 // one tile (lane l: 4 l ..), so the e4m3 output's group maximum is a warp reduction.
 __device__ __forceinline__ void store_y4(const DenseF8Params &p, long long row, int m, float (&v)[4], int mtile)
@@ -165,6 +155,10 @@ struct DsSmem {
     static constexpr bool OWN_PART = NT <= 32;
     static_assert(OWN_PART || NT * 512 <= STAGES * STAGE, "the sums fit the ring");
     static_assert(ALLOC <= 227 * 1024, "shared memory");
+    // CTAs that fit an SM together find tensor memory together: a cluster never holds some of it while
+    // another one waits for it on the next SM.
+    static_assert(2 * TMEM_COLS <= 512 || 2 * ALLOC > 227 * 1024, "tensor memory for the CTAs that fit");
+    static_assert(3 * ALLOC > 227 * 1024, "at most two CTAs fit");
 };
 
 __device__ __forceinline__ void cluster_arrive()

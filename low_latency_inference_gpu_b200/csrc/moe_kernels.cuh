@@ -48,7 +48,6 @@ __host__ __device__ constexpr int moe_team(int nt)
 constexpr int kMoeCluster = 4;          // kernel 1
 constexpr int kMoeStage = 5120;         // bytes of a ring stage: 16 rows of 256 + 64, or fewer longer ones
 constexpr int kMoeRing = kMoeWarps * kMoeStages * kMoeStage;
-constexpr int kMoeMaxPairs = LL_MOE_MAX_ROWS * LL_MOE_MAX_TOPK;
 
 struct MoeParams {
     const void *x;
@@ -948,7 +947,10 @@ __device__ __forceinline__ void moe_logits(const MoeParams &p, uint8_t *smem, co
             float q[kMoeCluster];
 #pragma unroll
             for (int r = 0; r < kMoeCluster; ++r)
-                asm("ld.shared::cluster.f32 %0, [%1];" : "=f"(q[r]) : "r"(mapa(at + (uint32_t)(ks * stride) * 4u, (uint32_t)r)));
+                asm volatile("ld.shared::cluster.f32 %0, [%1];"
+                             : "=f"(q[r])
+                             : "r"(mapa(at + (uint32_t)(ks * stride) * 4u, (uint32_t)r))
+                             : "memory");
 #pragma unroll
             for (int r = 0; r < kMoeCluster; ++r)
                 v += q[r];

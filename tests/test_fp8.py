@@ -414,6 +414,66 @@ def test_dense_repeats_bit_for_bit_on_streams_and_in_graphs(rows):
 
 @pytest.mark.gpu
 @pytest.mark.timeout(300)
+@pytest.mark.parametrize("rows", [2, 3500])
+def test_dense_behind_copies_and_other_launches(rows):
+    # the few-row kernel sets itself up beside the launch before it: what that one writes is seen all the same,
+    # behind a copy, a kernel of torch, the quantiser and another dense layer, eager and captured
+    import torch
+
+    c = DenseCase(rows, 384, 640, seed=9)
+    want, _ = c.run(ll.ACT_IDENTITY, ll.T_F32)
+    good = {k: c.d[k].clone() for k in ("x", "sx", "w", "sw", "b")}
+    y, sy = want.clone(), torch.empty(1, device="cuda")
+    other = DenseCase(5, 128, 256, seed=10)
+    oy, _ = other.run(ll.ACT_IDENTITY, ll.T_F32)
+
+    def sequence():
+        for k in good:  # copies
+            c.d[k].copy_(good[k])
+        c.run(ll.ACT_IDENTITY, ll.T_F32, y=y, sy=sy)
+        c.d["sx"].mul_(2.0)  # a kernel of torch
+        c.run(ll.ACT_IDENTITY, ll.T_F32, y=y, sy=sy)
+        c.d["sx"].mul_(0.5)
+        other.run(ll.ACT_IDENTITY, ll.T_F32, y=oy, sy=sy)
+        c.run(ll.ACT_IDENTITY, ll.T_F32, y=y, sy=sy)
+
+    for _ in range(3):
+        for k in ("x", "w", "sx"):
+            c.d[k].zero_()
+        y[:rows].fill_(-1.0)
+        sequence()
+        assert torch.equal(y[:rows], want[:rows])
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        sequence()
+    for _ in range(3):
+        for k in ("x", "w", "sx"):
+            c.d[k].zero_()
+        g.replay()
+        assert torch.equal(y[:rows], want[:rows])
+    ll.ops_check()
+
+
+@pytest.mark.gpu
+@pytest.mark.timeout(300)
+def test_silu_in_the_launch_per_layer_kernels():
+    M, K = 70, 96
+    W = ll.fill_normal(M * K, 0.0, 0.2, 1).reshape(M, K)
+    x, b = ll.fill_normal(K, 0.0, 1.0, 2), ll.fill_normal(M, 0.0, 1.0, 3)
+    v = W.astype(np.float64) @ x + b
+    tol = 1.1 * (np.abs(W) @ np.abs(x) + np.abs(b)) * (K + 2) * 2.0 ** -24 + np.abs(v) * 2.0 ** -20
+    dW, dWc, db, dx = dev(W), dev(ll.pack_rm_to_kmajor_padded(W, 96)), dev(ll.pack_bias_padded(b, 96)), dev(x)
+    for i in range(2):
+        y = dev(np.zeros(M, np.float32))
+        if i == 0:
+            ll.dense_warp_rm(dW.data_ptr(), db.data_ptr(), dx.data_ptr(), y.data_ptr(), M, K, ll.ACT_SILU)
+        else:
+            ll.dense_mbyv_packed(dWc.data_ptr(), db.data_ptr(), dx.data_ptr(), y.data_ptr(), M, K, ll.ACT_SILU)
+        assert np.all(np.abs(y.cpu().numpy() - v / (1 + np.exp(-v))) <= tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.timeout(300)
 def test_refuses_memory_of_the_host():
     import torch
 
