@@ -929,6 +929,16 @@ __device__ __forceinline__ void moe_logits(const MoeParams &p, uint8_t *smem, co
                 }
         }
     }
+    const int stride = mt_n * 16 * tp;
+    if (ksub > 1) {  // this CTA's parts first: the peers then read one word of each CTA
+        __syncthreads();
+        for (int i = tid; i < stride; i += 32 * WARPS) {
+            float v = part[i];
+            for (int ks = 1; ks < ksub; ++ks)
+                v += part[ks * stride + i];
+            part[i] = v;
+        }
+    }
     __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     meanwhile();  // while the others come
@@ -936,25 +946,18 @@ __device__ __forceinline__ void moe_logits(const MoeParams &p, uint8_t *smem, co
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     float *logits = reinterpret_cast<float *>(smem + L.logits);
     const uint32_t pa = smem_u32(part);
-    const int n_out = p.rows * p.experts, stride = mt_n * 16 * tp;
+    const int n_out = p.rows * p.experts;
     for (int i = tid; i < n_out; i += 32 * WARPS) {
         // consecutive threads: consecutive rows of an expert where there are several, so consecutive words
         const int e = i / p.rows, row = i - e * p.rows;
         const uint32_t at = pa + (uint32_t)(e * tp + row) * 4u;
-        float v = 0.0f;
-#pragma unroll 4
-        for (int ks = 0; ks < ksub; ++ks) {
-            float q[kMoeCluster];
+        float q[kMoeCluster], v = 0.0f;
 #pragma unroll
-            for (int r = 0; r < kMoeCluster; ++r)
-                asm volatile("ld.shared::cluster.f32 %0, [%1];"
-                             : "=f"(q[r])
-                             : "r"(mapa(at + (uint32_t)(ks * stride) * 4u, (uint32_t)r))
-                             : "memory");
+        for (int r = 0; r < kMoeCluster; ++r)
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(q[r]) : "r"(mapa(at, (uint32_t)r)) : "memory");
 #pragma unroll
-            for (int r = 0; r < kMoeCluster; ++r)
-                v += q[r];
-        }
+        for (int r = 0; r < kMoeCluster; ++r)
+            v += q[r];
         logits[row * p.experts + e] = v;
     }
     // the peers' partial sums are read; matched by the wait before the rings fill
@@ -1251,6 +1254,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1) ll_moe_down_kernel(const __gri
     for (int i = tid; i < kMoeWarps * p.rows * 16; i += kMoeThreads)
         part[i] = 0.0f;
     griddep_wait();
+    griddep_launch_dependents();
     int *ids = reinterpret_cast<int *>(smem + L.ids);
     float *probs = reinterpret_cast<float *>(smem + L.probs);
     for (int i = tid; i < p.rows * p.top_k; i += kMoeThreads) {
@@ -1389,8 +1393,8 @@ int moe_x_bytes(const MoeParams &p)
 }
 
 // One kernel with its own dynamic shared memory; `cluster` CTAs per cluster (0: none).
-inline int moe_launch(const void *fn, bool *ready, MoeParams &p, int smem, int grid, int cluster, bool dependent,
-                      int device, cudaStream_t st)
+inline int moe_launch(const void *fn, bool *ready, MoeParams &p, int smem, int grid, int cluster, int device,
+                      cudaStream_t st)
 {
     if (!__atomic_load_n(&ready[device], __ATOMIC_ACQUIRE)) {
         LL_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kMoeSmemCap));
@@ -1410,11 +1414,10 @@ inline int moe_launch(const void *fn, bool *ready, MoeParams &p, int smem, int g
         at[n].val.clusterDim.z = 1;
         ++n;
     }
-    if (dependent) {
-        at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        at[n].val.programmaticStreamSerializationAllowed = 1;
-        ++n;
-    }
+    // its CTAs may take their places as the launch before it leaves, and wait there for its end
+    at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
     cfg.attrs = at;
     cfg.numAttrs = (unsigned)n;
     void *args[] = {&p};
@@ -1469,8 +1472,9 @@ int launch_moe_typed(MoeParams &p, int device, cudaStream_t st)
         __atomic_store_n(&cluster_count[device], clusters, __ATOMIC_RELEASE);
     }
     LL_TRY(moe_launch(up, up_ready, p, moe_smem(p, true).total + (STAGED ? moe_x_bytes<WT, XT>(p) : 0),
-                      clusters * kMoeCluster, kMoeCluster, false, device, st));
-    return moe_launch(down, down_ready[stage_h], p, stage_h ? (int)staged_h : moe_smem(p, false).total, std::min(sms, p.hidden), 0, true, device, st);
+                      clusters * kMoeCluster, kMoeCluster, device, st));
+    return moe_launch(down, down_ready[stage_h], p, stage_h ? (int)staged_h : moe_smem(p, false).total,
+                      std::min(sms, p.hidden), 0, device, st);
 }
 
 // Up to 8 rows whose terms fit beside the rings take the kernel that stages x.
