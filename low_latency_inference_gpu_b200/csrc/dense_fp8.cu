@@ -184,7 +184,7 @@ __device__ __forceinline__ void ds_finish(const DenseF8Params &p, const float *p
     float bias[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-        bias[i] = p.bias && m + i < p.M ? __ldg(p.bias + m + i) : 0.0f;
+        bias[i] = p.bias && m + i < p.M ? p.bias[m + i] : 0.0f;
     const int mine = (int)min((long long)(NT - rank + SPLITS - 1) / SPLITS,
                               (p.rows - t0 - rank + SPLITS - 1) / SPLITS);  // rows c = rank + SPLITS slot that exist
     for (int slot = warp; slot < mine; slot += kDsThreads / 32) {
@@ -254,7 +254,9 @@ __global__ void __launch_bounds__(kDsThreads, 1) ll_dense_fp8_kernel(const __gri
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = misc[0];
-    griddep_wait();  // operands, scales and outputs belong to the launches before until here
+    // Operands, scales and outputs belong to the launches before until here; so they are read by plain loads,
+    // not by those for data that stays as it is for a whole kernel.
+    griddep_wait();
     griddep_launch_dependents();
     if (splits > 1 && L::OWN_PART)
         cluster_arrive();  // this CTA runs: its shared memory may be written to
@@ -311,7 +313,7 @@ __global__ void __launch_bounds__(kDsThreads, 1) ll_dense_fp8_kernel(const __gri
                 float f[kDsScaleKb];
 #pragma unroll
                 for (int jj = 0; jj < kDsScaleKb; ++jj)
-                    f[jj] = jj < n ? __ldg(sw + j + jj) : 0.0f;
+                    f[jj] = jj < n ? sw[j + jj] : 0.0f;
                 __syncwarp();
 #pragma unroll
                 for (int c0 = 0; c0 < NT; c0 += 32) {  // a row's blocks per lane, all loads at once
@@ -321,7 +323,7 @@ __global__ void __launch_bounds__(kDsThreads, 1) ll_dense_fp8_kernel(const __gri
                     float v[kDsScaleKb];
 #pragma unroll
                     for (int jj = 0; jj < kDsScaleKb; ++jj)
-                        v[jj] = c < NT && row < p.rows && jj < n ? __ldg(px + jj) : 0.0f;
+                        v[jj] = c < NT && row < p.rows && jj < n ? px[jj] : 0.0f;
                     if (c < NT)
 #pragma unroll
                         for (int jj = 0; jj < kDsScaleKb; ++jj)
@@ -422,7 +424,7 @@ __global__ void __launch_bounds__(kDsThreads, 1) ll_dense_fp8_kernel(const __gri
 // persistent cluster of two CTAs per pair), lane = row, 128 rows per CTA.  Each CTA loads its
 // rows of x and half of the tile's channels; the 2-SM instruction reads the other half from the
 // peer, so an SM's shared memory takes in 32 KB and gives 32 KB per K block of 512 tensor cycles,
-// just its 128 bytes a cycle (a 128 x 256 tile of one SM wants 192 and ran at 2.3 PFLOP/s).
+// just its 128 bytes a cycle (a 128 x 256 tile of one SM wants 192).
 // A K block's way out is 32 K values per CTA from TMEM and as many multiply-adds by the block's
 // scales (one factor per thread: sx of its row times sw of its 128 channels), beside the tensor
 // cores' work on the next block.

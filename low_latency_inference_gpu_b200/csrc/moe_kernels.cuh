@@ -12,9 +12,15 @@
 // tensor memory; at these widths the memory is the bound and the warp-level instruction is at a
 // few per cent of its rate.
 // Every warp works alone: it takes whole tiles (up to 16 weight rows, all columns), copies their
-// rows into a ring of its own (asynchronous copies, stages of 4 KB, refilled as soon as a stage is
-// read) and keeps the tile's sums in registers.  Nothing is handed from warp to warp
-// on the way, so the warps drift apart and cover each other's latencies.
+// rows into a ring of its own (asynchronous copies, two stages of 256 bytes of each row, refilled as
+// soon as a stage is read) and keeps the tile's sums in registers.  Nothing is handed from warp to
+// warp on the way, so the warps drift apart and cover each other's latencies.  For up to 8 rows two
+// warps share a tile, half of its columns each, as there are few tiles then.
+// Measured back to back in a graph, both kernels: 32 rows, 8 of 64 gated experts 2048 -> 1024 in bf16
+// (794 MB of weights) 235 us, 3.4 TB/s, where streaming them without the products takes 163: the
+// widths of a copy (256 bytes of a row) and the issue slots of copies and fragments hold it there.
+// One row, 8 of 64 e4m3 experts (50 MB) 32 us and 2 of 8 bf16 experts 1024 -> 512 16 us, of which
+// kernel 1 spends 7 to 10 on logits and choice before its first weight arrives: latency.
 //
 // Precision: weights are exact in bf16 (int8 and e4m3 too; their scales multiply fp32 sums).  x
 // and the activations a are split into bf16 terms that add up to the value: x in bf16 one, fp16
@@ -262,7 +268,7 @@ struct MoeX {
         if (vec && n >= EP) {
 #pragma unroll
             for (int i = 0; i < RAW<EP>; ++i)
-                v[i] = __ldg(reinterpret_cast<const uint4 *>(p) + i);
+                v[i] = reinterpret_cast<const uint4 *>(p)[i];
         } else {
 #pragma unroll 1
             for (int i = 0; i < RAW<EP>; ++i) {
@@ -271,8 +277,8 @@ struct MoeX {
                 for (int j = 0; j < 16 / BYTES; ++j)
                     if (i * (16 / BYTES) + j < n) {
                         const uint32_t one = BYTES == 4
-                                                 ? __ldg(reinterpret_cast<const uint32_t *>(p) + 4 * i + j)
-                                                 : (uint32_t)__ldg(reinterpret_cast<const uint16_t *>(p) + 8 * i + j);
+                                                 ? reinterpret_cast<const uint32_t *>(p)[4 * i + j]
+                                                 : (uint32_t)reinterpret_cast<const uint16_t *>(p)[8 * i + j];
                         w[j * BYTES / 4] |= one << (8 * (j * BYTES % 4));
                     }
                 const uint4 t = make_uint4(w[0], w[1], w[2], w[3]);
@@ -386,7 +392,7 @@ __host__ __device__ constexpr int moe_cols(int cols, int wbytes)
     return (cols + 256 / wbytes - 1) / (256 / wbytes) * (256 / wbytes);
 }
 
-// Bytes between rows of x in shared memory (8-byte types: the 16-byte pieces that a quarter of the
+// Bytes between rows of x in shared memory (8-bit types: the 16-byte pieces that a quarter of the
 // warp reads are 32 bytes apart in a row and 16 from row to row; bf16: 16 and 64).
 __host__ __device__ constexpr int moe_x_pitch(int cols, int wbytes)
 {
@@ -507,7 +513,7 @@ __device__ __forceinline__ void moe_copy(uint32_t dst, int rows, int m, int half
 #pragma unroll
             for (int i = 0; i < 16; ++i)
                 if (i < n)
-                    w[i / 4] |= (uint32_t)__ldg(src + i) << (8 * (i % 4));
+                    w[i / 4] |= (uint32_t)src[i] << (8 * (i % 4));
             st_shared_v4(d, make_uint4(w[0], w[1], w[2], w[3]));
         }
     }
@@ -719,8 +725,8 @@ __device__ __forceinline__ void moe_tile(const MoeParams &p, MoeRing &r, volatil
             Src::template next<EP>(ahead, 2);
         }
         if constexpr (WT == LL_W_F8) {
-            f0 = __ldg(sc0 + min(blk, last));
-            f1 = __ldg(sc1 + min(blk, last));
+            f0 = sc0[min(blk, last)];
+            f1 = sc1[min(blk, last)];
             ++blk;
         }
     };
@@ -1096,6 +1102,8 @@ __global__ void __launch_bounds__(kMoeThreads, 1) ll_moe_up_kernel(const __grid_
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     volatile uint32_t *misc = reinterpret_cast<volatile uint32_t *>(smem + L.misc);
     MoeRing ring = moe_ring(smem, L);
+    // What the launches before wrote is read from here on, by plain loads: those for data that stays as it is
+    // for a whole kernel may return what was there at its start.
     griddep_wait();
     griddep_launch_dependents();
     moe_logits<XT, NT>(p, smem, L, [&] {
@@ -1202,8 +1210,8 @@ __global__ void __launch_bounds__(kMoeThreads, 1) ll_moe_up_kernel(const __grid_
         }
         float q0 = 1.0f, q1 = 1.0f;
         if constexpr (WT == LL_W_I8) {
-            q0 = __ldg(p.sg + (size_t)e * F + c0);
-            q1 = __ldg((p.gated ? p.su : p.sg) + (size_t)e * F + c1);
+            q0 = p.sg[(size_t)e * F + c0];
+            q1 = (p.gated ? p.su : p.sg)[(size_t)e * F + c1];
         }
         // An activation into its planes, in the order that kernel 2 wants; behind the last one zeros up
         // to a whole step.
@@ -1332,8 +1340,8 @@ __global__ void __launch_bounds__(kMoeThreads, 1) ll_moe_down_kernel(const __gri
                 moe_tile<WT, NT, NT>(p, ring, misc + 1, stages, slot, tile_at, i0, i1, F, sc0, sc1, ntc, src, hrow, acc);
             float q0 = 1.0f, q1 = 1.0f;
             if constexpr (WT == LL_W_I8) {
-                q0 = __ldg(p.sd + (size_t)e * H + c0);
-                q1 = __ldg(p.sd + (size_t)e * H + c1);
+                q0 = p.sd[(size_t)e * H + c0];
+                q1 = p.sd[(size_t)e * H + c1];
             }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {

@@ -65,8 +65,8 @@ __device__ __forceinline__ float ops_act_fast(float v, int act)
     return ops_act(v, act);
 }
 
-// Bounded waits on a barrier of this CTA, by one thread or a whole warp.  The timer is read only after
-// some looks that failed: reading it takes about a microsecond, more than most of these waits.
+// Bounded waits on a barrier of this CTA, by one thread or a whole warp.  Most end within the first
+// looks, which read no timer and keep the loop short.
 __device__ __forceinline__ bool ops_try_wait(uint32_t bar, uint32_t parity)
 {
     uint32_t done;
