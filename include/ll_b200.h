@@ -453,7 +453,8 @@ void ll_quantize_fp8_blocks(const float *W, int m, int k, uint8_t *q, float *s);
  * ll_quantize_fp8 would make it of the fp32 result (the next layer's input), its scales in
  * d_sy [rows][ceil(M/128)].  ldw, ldx (bytes) and ldy (elements): row strides, 0 = dense; the rows
  * of W and x start on 16 bytes, so ldw and ldx are multiples of 16.  What lies beyond column K of
- * a row is not used.  rows = 0 does nothing.  Returns launch errors; ll_ops_check reports a device-side one.
+ * a row is not used.  rows = 0 does nothing.  The buffers do not overlap.  Returns launch errors;
+ * ll_ops_check reports a device-side one.
  */
 int ll_dense_fp8(const uint8_t *d_W, const float *d_sw, const float *d_b, const uint8_t *d_x, const float *d_sx,
                  void *d_y, float *d_sy, int y_type, int rows, int M, int K, int64_t ldw, int64_t ldx, int64_t ldy,
@@ -479,7 +480,9 @@ int ll_ops_check(void *stream);
  * rows <= LL_MOE_MAX_ROWS, 0 does nothing.  All sums are fp32; the weights are used exactly, x exactly,
  * the activations with 16 bits or more (24 when x is fp32).  d_ids / d_probs [rows][top_k]
  * (NULL to skip) receive the picked experts, largest logit first, and their weights.  A NaN logit
- * ranks below every number.
+ * ranks below every number.  A row with an infinity or NaN, or an expert with NaN weights, touches no
+ * row but its own and those that picked it.  e4m3 experts take values of x and activations up to 2^87,
+ * larger ones overflow.  y may be x; otherwise no buffer overlaps another.
  * d_work: work_bytes >= ll_moe_workspace_bytes(desc, rows), 256-byte aligned device memory that no
  * other call may use at the same time (calls one after another on a stream may share it); it needs
  * no initialisation.  Keeps nothing, allocates nothing, can be captured; as for ll_dense_fp8 every

@@ -13,6 +13,8 @@ Reference mapping (mamedov-ma/low_latency_inference_gpu):
                        src/bench_custom_warp_e2e.cu)
   * ``CublasMLP``   -- cuBLAS SGEMM chain (src/bench_cublas_mlp_graph.cu,
                        src/bench_persistent_cublas_mlp.cu)
+  * ``quantize_fp8``, ``dense_fp8``, ``moe_forward`` -- e4m3 layers and layers of experts on device
+                       pointers (no reference counterpart)
   * ``fill_normal`` -- host_init (src/bench_cublas_mlp.cu:37-43)
 """
 from __future__ import annotations

@@ -373,3 +373,46 @@ def test_a_layer_of_experts_and_an_output_layer(rows):
     x, w = dequant_rows(qn, sn), dequant_blocks(wq, sw)
     tol = (np.abs(x) @ np.abs(w).T) * (128 + 3 + 11) * U
     assert np.all(np.abs(out.cpu().numpy() - x @ w.T) <= tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.timeout(300)
+@pytest.mark.parametrize("rows,wtype,x_type", [(1, ll.W_BF16, ll.T_BF16), (4, ll.W_F8, ll.T_F16), (32, ll.W_I8, ll.T_F32)])
+def test_layers_in_a_row_write_over_their_input(rows, wtype, x_type):
+    """A chain of layers, each with y = x and one workspace: a launch that sets itself up beside the one before
+    it reads what that one wrote, eager and captured (the same results as with a synchronise after each)."""
+    import torch
+
+    m = ll.MoE(256, 128, 16, 2, wtype=wtype, x_type=x_type)
+    layers = [Layer(m, rows, seed=20 + 40 * i) for i in range(3)]
+    x = layers[0].xv
+    first = x.clone()
+    for l in layers:
+        l.xv, l.y, l.work = x, x, layers[0].work
+
+    def chain(wait):
+        x.copy_(first)
+        seen = []
+        for _ in range(2):
+            for l in layers:
+                l.run()
+                if wait:
+                    torch.cuda.synchronize()
+                seen.append((l.ids.clone(), x.clone()))
+        return seen
+
+    want = chain(True)
+    assert torch.isfinite(x).all() and not torch.equal(x, first)
+    for _ in range(5):
+        for a, b in zip(want, chain(False)):
+            assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        x.copy_(first)
+        for _ in range(2):
+            for l in layers:
+                l.run()
+    for _ in range(5):
+        g.replay()
+        assert torch.equal(x, want[-1][1])
+    ll.ops_check()
