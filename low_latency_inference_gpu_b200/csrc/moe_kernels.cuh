@@ -864,76 +864,62 @@ __device__ __forceinline__ void moe_router_step(const MoeParams &p, uint32_t e0,
 }
 
 // ---- router: logits of every (row, expert), by the whole cluster ----
-template <int XT, int NT, class Meanwhile>
+// A warp takes 16 experts x 8 rows over a part of the columns; one such product in the code, however many
+// rows there are: its first pass waits for every instruction of it to come from memory.
+template <int XT, class Meanwhile>
 __device__ __forceinline__ void moe_logits(const MoeParams &p, uint8_t *smem, const MoeSmem &L, Meanwhile meanwhile)
 {
     using X = MoeX<XT>;
     constexpr int EP = 8, KS = 64;
     const int tid = threadIdx.x, warp = tid >> 5, g = (tid & 31) >> 2, t = tid & 3;
     constexpr int WARPS = kMoeWarps;
-    const int mt_n = (p.experts + 15) / 16, ksub = mt_n >= WARPS ? 1 : WARPS / mt_n;
     const int tp = (p.rows + 7) / 8 * 8, ntc = tp / 8, H = p.hidden;
+    const int mt_n = (p.experts + 15) / 16, units = mt_n * ntc, ksub = units >= WARPS ? 1 : WARPS / units;
     const int rank = (int)cluster_ctarank();
     float *part = reinterpret_cast<float *>(smem + L.part);
     const int steps = (H + KS - 1) / KS, slices = kMoeCluster * ksub;
     const X src = {static_cast<const uint8_t *>(p.x), (size_t)p.ldx * X::BYTES, H, p.x_vec != 0};
-    {
-        for (int u = warp; u < mt_n * ksub; u += WARPS) {
-            const int mt = u / ksub, ks = u - mt * ksub, sl = rank * ksub + ks;
-            const uint32_t e0 = (uint32_t)min(mt * 16 + g, p.experts - 1), e1 = (uint32_t)min(mt * 16 + g + 8, p.experts - 1);
-            float acc[NT][4] = {};
-#pragma unroll(NT == 1 ? 2 : 1)
-            for (int st = sl * steps / slices; st < (sl + 1) * steps / slices; ++st) {
-                uint4 xb[NT][2][X::template RAW<EP>];
+    for (int u = warp; u < units * ksub; u += WARPS) {
+        const int ks = u / units, v = u - ks * units, mt = v / ntc, nt = v - mt * ntc, sl = rank * ksub + ks;
+        const uint32_t e0 = (uint32_t)min(mt * 16 + g, p.experts - 1), e1 = (uint32_t)min(mt * 16 + g + 8, p.experts - 1);
+        const uint8_t *row = src.base + (size_t)min(nt * 8 + g, p.rows - 1) * src.row_bytes;
+        float acc[4] = {};
+#pragma unroll 2
+        for (int st = sl * steps / slices; st < (sl + 1) * steps / slices; ++st) {
+            uint4 xb[2][X::template RAW<EP>];
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-                    if (nt < ntc)
+            for (int pc = 0; pc < 2; ++pc)
+                src.template load<EP>(row, st * KS + pc * 32 + t * EP, xb[pc]);
+            uint32_t a0[2][3][EP / 2], a1[2][3][EP / 2];
+            if (p.router_f32)
+                moe_router_step<LL_T_F32, 3>(p, e0, e1, st * KS, a0, a1);
+            else
+                moe_router_step<LL_T_BF16, 1>(p, e0, e1, st * KS, a0, a1);
+            float part4[4] = {};  // each step from zero, then added in fp32
 #pragma unroll
-                        for (int pc = 0; pc < 2; ++pc) {
-                            const int k = st * KS + pc * 32 + t * EP;
-                            src.template load<EP>(src.base + (size_t)min(nt * 8 + g, p.rows - 1) * src.row_bytes, k, xb[nt][pc]);
-                        }
-                uint32_t a0[2][3][EP / 2], a1[2][3][EP / 2];
-                if (p.router_f32)
-                    moe_router_step<LL_T_F32, 3>(p, e0, e1, st * KS, a0, a1);
-                else
-                    moe_router_step<LL_T_BF16, 1>(p, e0, e1, st * KS, a0, a1);
+            for (int pc = 0; pc < 2; ++pc) {
+                uint32_t b[X::NS][EP / 2];
+                X::template terms<EP, false>(xb[pc], b);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-                    if (nt < ntc) {
-                        float part4[4] = {};  // each step from zero, then added in fp32
+                for (int ra = 0; ra < 3; ++ra)
+                    if (ra == 0 || p.router_f32) {
 #pragma unroll
-                        for (int pc = 0; pc < 2; ++pc) {
-                            uint32_t b[X::NS][EP / 2];
-                            X::template terms<EP, false>(xb[nt][pc], b);
+                        for (int s = 0; s < X::NS; ++s)
 #pragma unroll
-                            for (int ra = 0; ra < 3; ++ra)
-                                if (ra == 0 || p.router_f32) {
-#pragma unroll
-                                    for (int s = 0; s < X::NS; ++s)
-#pragma unroll
-                                        for (int j = 0; j < EP / 4; ++j)
-                                            mma_bf16(part4, a0[pc][ra][2 * j], a1[pc][ra][2 * j],
-                                                     a0[pc][ra][2 * j + 1], a1[pc][ra][2 * j + 1], b[s][2 * j],
-                                                     b[s][2 * j + 1]);
-                                }
-                        }
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            acc[nt][i] += part4[i];
+                            for (int j = 0; j < EP / 4; ++j)
+                                mma_bf16(part4, a0[pc][ra][2 * j], a1[pc][ra][2 * j], a0[pc][ra][2 * j + 1],
+                                         a1[pc][ra][2 * j + 1], b[s][2 * j], b[s][2 * j + 1]);
                     }
             }
-            float *o = part + (size_t)(ks * mt_n + mt) * 16 * tp;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-                if (nt < ntc) {
-                    const int c = nt * 8 + 2 * t;
-                    o[g * tp + c] = acc[nt][0];
-                    o[g * tp + c + 1] = acc[nt][1];
-                    o[(g + 8) * tp + c] = acc[nt][2];
-                    o[(g + 8) * tp + c + 1] = acc[nt][3];
-                }
+            for (int i = 0; i < 4; ++i)
+                acc[i] += part4[i];
         }
+        float *o = part + (size_t)(ks * mt_n + mt) * 16 * tp + nt * 8 + 2 * t;
+        o[g * tp] = acc[0];
+        o[g * tp + 1] = acc[1];
+        o[(g + 8) * tp] = acc[2];
+        o[(g + 8) * tp + 1] = acc[3];
     }
     const int stride = mt_n * 16 * tp;
     if (ksub > 1) {  // this CTA's parts first: the peers then read one word of each CTA
@@ -982,7 +968,9 @@ __device__ __forceinline__ uint32_t order_key(float v)
 }
 
 // ---- the top_k experts of each row and their weights (one warp per row) ----
-template <int PER>  // experts per lane
+// PER experts per lane.  COUNT: an expert's place is counted, 64 steps that wait for nothing (a row alone);
+// else the largest is taken top_k times, fewer instructions where every warp has rows in turn.
+template <int PER, bool COUNT>
 __device__ __forceinline__ void moe_pick(const MoeParams &p, uint8_t *smem, const MoeSmem &L)
 {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -1014,7 +1002,8 @@ __device__ __forceinline__ void moe_pick(const MoeParams &p, uint8_t *smem, cons
                 sum += __shfl_xor_sync(0xffffffffu, sum, off);
         }
         uint32_t mine = 0;  // lane j: the j-th picked expert
-        if constexpr (PER <= 2) {
+        if constexpr (COUNT) {
+            static_assert(PER <= 2, "two keys per lane");
             // an expert's place is the number of experts before it: by logit, of equal ones by index
             int place[PER] = {};
 #pragma unroll 8
@@ -1106,14 +1095,14 @@ __global__ void __launch_bounds__(kMoeThreads, 1) ll_moe_up_kernel(const __grid_
     // for a whole kernel may return what was there at its start.
     griddep_wait();
     griddep_launch_dependents();
-    moe_logits<XT, NT>(p, smem, L, [&] {
+    moe_logits<XT>(p, smem, L, [&] {
         if constexpr (STAGED)
             moe_stage_x<WT, XT>(p, smem + L.x);
     });
     if (p.experts <= 64)
-        moe_pick<2>(p, smem, L);
+        moe_pick<2, NT == 1>(p, smem, L);
     else
-        moe_pick<LL_MOE_MAX_EXPERTS / 32>(p, smem, L);
+        moe_pick<LL_MOE_MAX_EXPERTS / 32, false>(p, smem, L);
     const int n_pairs = p.rows * p.top_k;
     if (blockIdx.x == 0) {
         for (int i = tid; i < n_pairs; i += kMoeThreads) {
