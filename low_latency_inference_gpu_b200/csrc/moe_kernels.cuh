@@ -835,8 +835,8 @@ __device__ __forceinline__ void moe_tile(const MoeParams &p, MoeRing &r, volatil
 
 // This thread's pieces of the router's rows e0 and e1 (columns k0 .. k0 + 63) as bf16 terms.
 template <int RT, int NR>
-__device__ __forceinline__ void moe_router_step(const MoeParams &p, uint32_t e0, uint32_t e1, int k0, uint32_t (&a0)[2][3][4],
-                                                uint32_t (&a1)[2][3][4])
+__device__ __forceinline__ void moe_router_step(const MoeParams &p, uint32_t e0, uint32_t e1, int k0, uint32_t (&a0)[2][NR][4],
+                                                uint32_t (&a1)[2][NR][4])
 {
     using R = MoeX<RT>;
     const R src = {static_cast<const uint8_t *>(p.router), (size_t)p.hidden * R::BYTES, p.hidden, p.router_vec != 0};
@@ -864,8 +864,9 @@ __device__ __forceinline__ void moe_router_step(const MoeParams &p, uint32_t e0,
 }
 
 // ---- router: logits of every (row, expert), by the whole cluster ----
-// A warp takes 16 experts x 8 rows over a part of the columns; one such product in the code, however many
-// rows there are: its first pass waits for every instruction of it to come from memory.
+// A warp takes 16 experts x 8 rows over a part of the columns.  One such product in the code, however many
+// rows there are, and its loop not unrolled: its first pass waits for every instruction of it to come from
+// memory (32 rows of 64 experts 2048 x 1024: 229 us unrolled twice, 225 not; one row of 8: 16.2, 15.7).
 template <int XT, class Meanwhile>
 __device__ __forceinline__ void moe_logits(const MoeParams &p, uint8_t *smem, const MoeSmem &L, Meanwhile meanwhile)
 {
@@ -879,48 +880,51 @@ __device__ __forceinline__ void moe_logits(const MoeParams &p, uint8_t *smem, co
     float *part = reinterpret_cast<float *>(smem + L.part);
     const int steps = (H + KS - 1) / KS, slices = kMoeCluster * ksub;
     const X src = {static_cast<const uint8_t *>(p.x), (size_t)p.ldx * X::BYTES, H, p.x_vec != 0};
-    for (int u = warp; u < units * ksub; u += WARPS) {
-        const int ks = u / units, v = u - ks * units, mt = v / ntc, nt = v - mt * ntc, sl = rank * ksub + ks;
-        const uint32_t e0 = (uint32_t)min(mt * 16 + g, p.experts - 1), e1 = (uint32_t)min(mt * 16 + g + 8, p.experts - 1);
-        const uint8_t *row = src.base + (size_t)min(nt * 8 + g, p.rows - 1) * src.row_bytes;
-        float acc[4] = {};
-#pragma unroll 2
-        for (int st = sl * steps / slices; st < (sl + 1) * steps / slices; ++st) {
-            uint4 xb[2][X::template RAW<EP>];
+    // one copy for each type of the router, of which a launch fetches one
+    auto products = [&](auto type) {
+        constexpr int RT = decltype(type)::value, NR = RT == LL_T_F32 ? 3 : 1;
+        for (int u = warp; u < units * ksub; u += WARPS) {
+            const int ks = u / units, v = u - ks * units, mt = v / ntc, nt = v - mt * ntc, sl = rank * ksub + ks;
+            const uint32_t e0 = (uint32_t)min(mt * 16 + g, p.experts - 1), e1 = (uint32_t)min(mt * 16 + g + 8, p.experts - 1);
+            const uint8_t *row = src.base + (size_t)min(nt * 8 + g, p.rows - 1) * src.row_bytes;
+            float acc[4] = {};
+#pragma unroll 1
+            for (int st = sl * steps / slices; st < (sl + 1) * steps / slices; ++st) {
+                uint4 xb[2][X::template RAW<EP>];
 #pragma unroll
-            for (int pc = 0; pc < 2; ++pc)
-                src.template load<EP>(row, st * KS + pc * 32 + t * EP, xb[pc]);
-            uint32_t a0[2][3][EP / 2], a1[2][3][EP / 2];
-            if (p.router_f32)
-                moe_router_step<LL_T_F32, 3>(p, e0, e1, st * KS, a0, a1);
-            else
-                moe_router_step<LL_T_BF16, 1>(p, e0, e1, st * KS, a0, a1);
-            float part4[4] = {};  // each step from zero, then added in fp32
+                for (int pc = 0; pc < 2; ++pc)
+                    src.template load<EP>(row, st * KS + pc * 32 + t * EP, xb[pc]);
+                uint32_t a0[2][NR][EP / 2], a1[2][NR][EP / 2];
+                moe_router_step<RT, NR>(p, e0, e1, st * KS, a0, a1);
+                float part4[4] = {};  // each step from zero, then added in fp32
 #pragma unroll
-            for (int pc = 0; pc < 2; ++pc) {
-                uint32_t b[X::NS][EP / 2];
-                X::template terms<EP, false>(xb[pc], b);
+                for (int pc = 0; pc < 2; ++pc) {
+                    uint32_t b[X::NS][EP / 2];
+                    X::template terms<EP, false>(xb[pc], b);
 #pragma unroll
-                for (int ra = 0; ra < 3; ++ra)
-                    if (ra == 0 || p.router_f32) {
+                    for (int ra = 0; ra < NR; ++ra)
 #pragma unroll
                         for (int s = 0; s < X::NS; ++s)
 #pragma unroll
                             for (int j = 0; j < EP / 4; ++j)
                                 mma_bf16(part4, a0[pc][ra][2 * j], a1[pc][ra][2 * j], a0[pc][ra][2 * j + 1],
                                          a1[pc][ra][2 * j + 1], b[s][2 * j], b[s][2 * j + 1]);
-                    }
-            }
+                }
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                acc[i] += part4[i];
+                for (int i = 0; i < 4; ++i)
+                    acc[i] += part4[i];
+            }
+            float *o = part + (size_t)(ks * mt_n + mt) * 16 * tp + nt * 8 + 2 * t;
+            o[g * tp] = acc[0];
+            o[g * tp + 1] = acc[1];
+            o[(g + 8) * tp] = acc[2];
+            o[(g + 8) * tp + 1] = acc[3];
         }
-        float *o = part + (size_t)(ks * mt_n + mt) * 16 * tp + nt * 8 + 2 * t;
-        o[g * tp] = acc[0];
-        o[g * tp + 1] = acc[1];
-        o[(g + 8) * tp] = acc[2];
-        o[(g + 8) * tp + 1] = acc[3];
-    }
+    };
+    if (p.router_f32)
+        products(std::integral_constant<int, LL_T_F32>());
+    else
+        products(std::integral_constant<int, LL_T_BF16>());
     const int stride = mt_n * 16 * tp;
     if (ksub > 1) {  // this CTA's parts first: the peers then read one word of each CTA
         __syncthreads();
