@@ -128,6 +128,8 @@ __device__ __forceinline__ void store_y4(const DenseF8Params &p, long long row, 
 //     as their operands land and wait for nobody;
 //   * 4 stages of 18 KB at 16 rows, so that two CTAs fit an SM and the next launch's set-up
 //     (barriers, tensor memory, tensor maps) runs beside this one's end (programmatic dependent launch).
+// Back to back in a graph: 1 x 2048 x 2048 4.0 us, 32 x 4096 x 4096 with e4m3 output 7.2 (16.8 MB of weights, 2.4
+// TB/s), 256 x 2048 x 2048 8.2.
 //   warp 0     TMA producer (W box 16 KB + X box NT * 128 B per K block)
 //   warp 1     TMEM allocation; one lane issues the MMAs
 //   warps 2-5  lane = channel: TMEM -> registers, times the block's scales
@@ -425,6 +427,8 @@ __global__ void __launch_bounds__(kDsThreads, 1) ll_dense_fp8_kernel(const __gri
 // rows of x and half of the tile's channels; the 2-SM instruction reads the other half from the
 // peer, so an SM's shared memory takes in 32 KB and gives 32 KB per K block of 512 tensor cycles,
 // just its 128 bytes a cycle (a 128 x 256 tile of one SM wants 192).
+// 8192 x 4096 x 4096 with GELU and bf16 output: 167 us, 1647 TFLOP/s; without the store 137, and with the
+// instructions and loads alone 91, which twice the measured bf16 rate would do in 82.
 // A K block's way out is 32 K values per CTA from TMEM and as many multiply-adds by the block's
 // scales (one factor per thread: sx of its row times sw of its 128 channels), beside the tensor
 // cores' work on the next block.

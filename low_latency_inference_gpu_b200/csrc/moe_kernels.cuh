@@ -17,9 +17,9 @@
 // warp on the way, so the warps drift apart and cover each other's latencies.  For up to 8 rows two
 // warps share a tile, half of its columns each, as there are few tiles then.
 // Measured back to back in a graph, both kernels: 32 rows, 8 of 64 gated experts 2048 -> 1024 in bf16
-// (794 MB of weights) 235 us, 3.4 TB/s, where streaming them without the products takes 163: the
+// (794 MB of weights) 224 us, 3.5 TB/s, where streaming them without the products takes 163: the
 // widths of a copy (256 bytes of a row) and the issue slots of copies and fragments hold it there.
-// One row, 8 of 64 e4m3 experts (50 MB) 32 us and 2 of 8 bf16 experts 1024 -> 512 16 us, of which
+// One row, 8 of 64 e4m3 experts (50 MB) 31 us and 2 of 8 bf16 experts 1024 -> 512 15 us, of which
 // kernel 1 spends 7 to 10 on logits and choice before its first weight arrives: latency.
 //
 // Precision: weights are exact in bf16 (int8 and e4m3 too; their scales multiply fp32 sums).  x
