@@ -427,8 +427,10 @@ __global__ void __launch_bounds__(kDsThreads, 1) ll_dense_fp8_kernel(const __gri
 // rows of x and half of the tile's channels; the 2-SM instruction reads the other half from the
 // peer, so an SM's shared memory takes in 32 KB and gives 32 KB per K block of 512 tensor cycles,
 // just its 128 bytes a cycle (a 128 x 256 tile of one SM wants 192).
-// 8192 x 4096 x 4096 with GELU and bf16 output: 167 us, 1647 TFLOP/s; without the store 137, and with the
+// 8192 x 4096 x 4096 with GELU and bf16 output: 159 us, 1726 TFLOP/s; without the store 125, and with the
 // instructions and loads alone 91, which twice the measured bf16 rate would do in 82.
+// The loads from TMEM follow each other without a pause, across blocks too, each beside the multiply-adds of
+// the 32 columns before it (all of a block's loads and then its last sums: 167).
 // A K block's way out is 32 K values per CTA from TMEM and as many multiply-adds by the block's
 // scales (one factor per thread: sx of its row times sw of its 128 channels), beside the tensor
 // cores' work on the next block.
@@ -822,6 +824,11 @@ __global__ void __launch_bounds__(kDlThreads, 1) ll_dense_fp8_large_kernel(const
                 }
             };
             load_scales(0);
+            uint32_t v0[32], v1[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+                v1[i] = 0u;
+            float late = 0.0f;
             for (int kb0 = 0; kb0 < p.nkb && ok; kb0 += 4) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
@@ -839,16 +846,17 @@ __global__ void __launch_bounds__(kDlThreads, 1) ll_dense_fp8_large_kernel(const
                     tc_fence_after();
                     const float s = f[i];
                     const uint32_t at = tq + (uint32_t)(b * kDlN);
-                    uint32_t v0[32], v1[32];
                     tc_ld_32cols_async(at, v0);
-                    tc_ld_32cols_async(at + 32, v1);
+                    fma_32cols(acc + 96, v1, late);
                     tc_wait_ld_32(v0);
-                    tc_wait_ld_32(v1);
+                    tc_ld_32cols_async(at + 32, v1);
                     fma_32cols(acc, v0, s);
+                    tc_wait_ld_32(v1);
                     tc_ld_32cols_async(at + 64, v0);
                     fma_32cols(acc + 32, v1, s);
-                    tc_ld_32cols_async(at + 96, v1);
                     tc_wait_ld_32(v0);
+                    tc_ld_32cols_async(at + 96, v1);
+                    fma_32cols(acc + 64, v0, s);
                     tc_wait_ld_32(v1);
                     tc_fence_before();
                     __syncwarp();
@@ -858,10 +866,10 @@ __global__ void __launch_bounds__(kDlThreads, 1) ll_dense_fp8_large_kernel(const
                         else
                             mbar_arrive_remote_cta(mapa(b_acce(b), 0u));
                     }
-                    fma_32cols(acc + 64, v0, s);
-                    fma_32cols(acc + 96, v1, s);
+                    late = s;
                 }
             }
+            fma_32cols(acc + 96, v1, late);
             if (ok && c0 < p.M)
                 dl_store<YT>(p, out, acc, row0, c0);
         }
