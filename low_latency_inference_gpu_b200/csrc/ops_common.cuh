@@ -34,6 +34,15 @@ __device__ __forceinline__ float ops_act(float v, int act)
     return v;
 }
 
+// Coefficients of R below, from the tenth power down.
+__host__ __device__ constexpr float gelu_tail(int k)
+{
+    constexpr float c[11] = {1.846406121e-06f, -3.862410449e-05f, 3.623082885e-04f, -2.055361634e-03f, 8.110309020e-03f,
+                             -2.453368530e-02f, 6.132410467e-02f, -1.325876117e-01f, 2.499329448e-01f, -3.989378810e-01f,
+                             4.999999404e-01f};
+    return c[k];
+}
+
 // The activations for results that are rounded to 16 bits or fewer.  Off by less than 2^-21 |v|, where
 // that rounding takes 2^-11 of the result or more, at a third of the instructions:
 //   gelu  v Phi(v), Phi(-a) = exp(-a^2 / 2) R(a): R, the smooth factor of the normal tail (half the
@@ -44,17 +53,10 @@ __device__ __forceinline__ float ops_act_fast(float v, int act)
 {
     if (act == LL_ACT_GELU) {
         const float a = fabsf(v), b = fminf(a, 5.5f);
-        float r = 1.846406121e-06f;
-        r = fmaf(r, b, -3.862410449e-05f);
-        r = fmaf(r, b, 3.623082885e-04f);
-        r = fmaf(r, b, -2.055361634e-03f);
-        r = fmaf(r, b, 8.110309020e-03f);
-        r = fmaf(r, b, -2.453368530e-02f);
-        r = fmaf(r, b, 6.132410467e-02f);
-        r = fmaf(r, b, -1.325876117e-01f);
-        r = fmaf(r, b, 2.499329448e-01f);
-        r = fmaf(r, b, -3.989378810e-01f);
-        r = fmaf(r, b, 4.999999404e-01f);
+        float r = gelu_tail(0);
+#pragma unroll
+        for (int k = 1; k < 11; ++k)
+            r = fmaf(r, b, gelu_tail(k));
         float e;  // exp(-a^2 / 2) = 2^(-a^2 log2(e) / 2)
         asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(a * a * -0.72134752044448170f));
         const float tail = e * r;
@@ -63,6 +65,64 @@ __device__ __forceinline__ float ops_act_fast(float v, int act)
     if (act == LL_ACT_SILU)
         return __fdividef(v, 1.0f + __expf(-v));
     return ops_act(v, act);
+}
+
+// Two fp32 values in a register pair.
+__device__ __forceinline__ uint64_t f2_pack(float a, float b)
+{
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 f2_unpack(uint64_t v)
+{
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// gelu of ops_act_fast, N values in pairs: the same steps in fewer instructions.  8192 x 4096 x 4096 of
+// ll_dense_fp8 takes 156 us with it and 159 with single values (146 with relu).
+template <int N>
+__device__ __forceinline__ void ops_gelu_fast(float (&v)[N])
+{
+    uint64_t b[N / 2], r[N / 2];
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+        b[i] = f2_pack(fminf(fabsf(v[2 * i]), 5.5f), fminf(fabsf(v[2 * i + 1]), 5.5f));
+        r[i] = f2_pack(gelu_tail(0), gelu_tail(0));
+    }
+#pragma unroll
+    for (int k = 1; k < 11; ++k) {
+        const uint64_t ck = f2_pack(gelu_tail(k), gelu_tail(k));
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i)
+            r[i] = f2_fma(r[i], b[i], ck);
+    }
+    const uint64_t half = f2_pack(-0.72134752044448170f, -0.72134752044448170f);
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+        const uint64_t w = f2_pack(v[2 * i], v[2 * i + 1]);
+        const float2 q = f2_unpack(f2_mul(f2_mul(w, w), half));
+        float2 e;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(q.x));
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(q.y));
+        const uint64_t tail = f2_mul(f2_pack(e.x, e.y), r[i]);
+        const float2 t = f2_unpack(tail);
+        v[2 * i] = v[2 * i] * (v[2 * i] > 0.0f ? 1.0f - t.x : t.x);
+        v[2 * i + 1] = v[2 * i + 1] * (v[2 * i + 1] > 0.0f ? 1.0f - t.y : t.y);
+    }
 }
 
 // Bounded waits on a barrier of this CTA, by one thread or a whole warp.  Most end within the first
