@@ -453,8 +453,8 @@ void ll_quantize_fp8_blocks(const float *W, int m, int k, uint8_t *q, float *s);
  * ll_quantize_fp8 would make it of the fp32 result (the next layer's input), its scales in
  * d_sy [rows][ceil(M/128)].  ldw, ldx (bytes) and ldy (elements): row strides, 0 = dense; the rows
  * of W and x start on 16 bytes, so ldw and ldx are multiples of 16.  What lies beyond column K of
- * a row is not used.  rows = 0 does nothing.  The buffers do not overlap.  Returns launch errors;
- * ll_ops_check reports a device-side one.
+ * a row is not used.  rows = 0 does nothing, more than 65535 * 128 are refused.  The buffers do not
+ * overlap.  Returns launch errors; ll_ops_check reports a device-side one.
  */
 int ll_dense_fp8(const uint8_t *d_W, const float *d_sw, const float *d_b, const uint8_t *d_x, const float *d_sx,
                  void *d_y, float *d_sy, int y_type, int rows, int M, int K, int64_t ldw, int64_t ldx, int64_t ldy,

@@ -203,6 +203,25 @@ def test_moe(wtype, x_type, case):
 
 @pytest.mark.gpu
 @pytest.mark.timeout(300)
+@pytest.mark.parametrize("wtype,x_type", [(ll.W_BF16, ll.T_BF16), (ll.W_F8, ll.T_F32), (ll.W_I8, ll.T_F16)])
+@pytest.mark.parametrize("rows,hidden,inter,experts,top_k,gated", [
+    (8, 4096, 72, 4, 2, True),     # few rows whose x fits no shared memory
+    (2, 72, 9000, 3, 3, True),     # nor their activations
+    (1, 48, 24, 256, 16, False),   # one row, the most experts and picks
+    (1, 65536, 8, 2, 1, True),     # the widest rows
+    (1, 8, 65536, 2, 2, False),
+    (1, 1, 1, 1, 1, True),
+    (32, 1, 1, 3, 2, False),
+])
+def test_borders(wtype, x_type, rows, hidden, inter, experts, top_k, gated):
+    layer = Layer(ll.MoE(hidden, inter, experts, top_k, gated=gated, wtype=wtype, x_type=x_type), rows, seed=3)
+    layer.run()
+    ll.ops_check()
+    layer.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.timeout(300)
 def test_ties_go_to_the_lower_index():
     m = ll.MoE(128, 64, 12, 5)
     layer = Layer(m, 4)
