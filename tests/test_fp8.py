@@ -380,6 +380,36 @@ def test_dense_special_values():
 
 @pytest.mark.gpu
 @pytest.mark.timeout(300)
+@pytest.mark.parametrize("act", [ll.ACT_GELU, ll.ACT_SILU, ll.ACT_RELU])
+@pytest.mark.parametrize("y_type", [ll.T_F32, ll.T_BF16, ll.T_F16, ll.T_F8])
+def test_dense_many_rows_every_activation(act, y_type):
+    c = DenseCase(1290, 2048, 384, seed=31)
+    y, sy = c.run(act, y_type)
+    ll.ops_check()
+    c.check(act, y_type, y, sy)
+
+
+@pytest.mark.gpu
+@pytest.mark.timeout(300)
+@pytest.mark.parametrize("act", [ll.ACT_IDENTITY, ll.ACT_GELU])
+@pytest.mark.parametrize("y_type", [ll.T_F32, ll.T_BF16])
+def test_dense_many_rows_special_values(act, y_type):
+    c = DenseCase(1290, 2048, 384, seed=32)
+    plain, _ = c.run(act, y_type)
+    plain = plain.float().cpu().numpy()[:1290]
+    c.d["x"][3, 5] = 0x7F                       # NaN: its row
+    c.d["sx"][700, 1] = float("nan")            # a scale: its row
+    c.d["w"][2000, 17] = 0x7F                   # NaN: its channel
+    y, _ = c.run(act, y_type)
+    y = y.float().cpu().numpy()[:1290]
+    assert np.isnan(y[[3, 700]]).all() and np.isnan(y[:, 2000]).all()
+    rows, cols = np.delete(np.arange(1290), [3, 700]), np.delete(np.arange(2048), 2000)
+    assert np.array_equal(y[np.ix_(rows, cols)], plain[np.ix_(rows, cols)])
+    ll.ops_check()
+
+
+@pytest.mark.gpu
+@pytest.mark.timeout(300)
 @pytest.mark.parametrize("rows", [1, 40, 700, 3500])
 def test_dense_repeats_bit_for_bit_on_streams_and_in_graphs(rows):
     import torch
