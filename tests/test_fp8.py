@@ -562,3 +562,42 @@ def test_an_e4m3_net_layer_after_layer(rows):
     y_ref = h_got @ dequant_blocks(*qs[1]).T
     a = np.abs(h_got) @ np.abs(dequant_blocks(*qs[1])).T
     assert np.all(np.abs(y.cpu().numpy() - y_ref) <= a * (128 + 4 + 11) * 2.0 ** -23)
+
+
+@pytest.mark.gpu
+@pytest.mark.timeout(300)
+@pytest.mark.parametrize("rows,M", [(1, 4096), (256, 8192)])  # the few-row kernel, the many-row one
+@pytest.mark.parametrize("y_type", [ll.T_F32, ll.T_BF16, ll.T_F16])
+def test_gelu_keeps_its_digits_for_negative_values(rows, M, y_type):
+    # Weights of zero, so that the activation's argument is the bias, exactly.  Bounds relative to the result:
+    #   fp32: the exponent -v^2 / 2 has two roundings, 2^-24 of it each, so v^2 2^-23 / 2 in the tail; the rest
+    #         (a polynomial's fit and its nine roundings, the approximate quotient and power, three products)
+    #         within 6 units 2^-23, which also cover the other half of v^2;
+    #   16 bits: the tail is good to 2^-16.5 up to |v| = 6.5 and 2^-14.2 beyond; two more operations add 2^-23;
+    #         then half a step of rounding, of fp16's lowest octave 2^-25.
+    from math import erfc
+
+    import torch
+
+    v = np.concatenate([np.linspace(-12.5, 8, M - 64), -np.exp2(np.linspace(-30, 3, 64))]).astype(np.float32)
+    K = 16
+    c = DenseCase(rows, M, K)
+    c.d["w"].zero_()
+    c.d["b"] = dev(v)
+    y, _ = c.run(ll.ACT_GELU, y_type)
+    ll.ops_check()
+    v = v.astype(np.float64)
+    ref = 0.5 * v * np.vectorize(erfc)(v * -np.sqrt(0.5))
+    if y_type == ll.T_F32:
+        tol = np.abs(ref) * (v * v + 6) * 2.0 ** -23
+    else:
+        tol = np.abs(ref) * (np.where(np.abs(v) <= 6.5, 2.0 ** -16.5, 2.0 ** -14.2) + 2.0 ** -22) * 1.01
+        tol += np.abs(ref) * (2.0 ** -8 if y_type == ll.T_BF16 else 2.0 ** -11) + (y_type == ll.T_F16) * 2.0 ** -25
+    got = y[:rows].double().cpu().numpy()
+    assert torch.equal(y[0], y[rows - 1])
+    off = np.abs(got - ref)
+    assert np.all(off <= tol), (v[np.argmax(np.max(off - tol, 0))], np.max(off / np.maximum(tol, 1e-300)))
+    big = DenseCase(rows, M, K, bias=False)
+    big.d["w"].zero_()
+    big.d["b"] = dev(np.full(M, np.inf, np.float32))
+    assert np.all(big.run(ll.ACT_GELU, y_type)[0][:rows].float().cpu().numpy() == np.inf)
