@@ -199,7 +199,7 @@ __device__ __forceinline__ void ds_finish(const DenseF8Params &p, const float *p
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             v[i] += bias[i];
-            v[i] = p.y_type == LL_T_F32 ? ops_act(v[i], p.act) : ops_act_fast(v[i], p.act);
+            v[i] = ops_act(v[i], p.act);
         }
         store_y4(p, t0 + rank + SPLITS * slot, m, v, mtile);
     }
@@ -520,6 +520,8 @@ __device__ __forceinline__ void fma_32cols(float *acc, const uint32_t (&v)[32], 
 template <int YT, int ACT>
 __device__ __forceinline__ void dl_store_64cols(const DenseF8Params &p, uint8_t *out, float *acc, long long row0, int c0)
 {
+    // an e4m3 result is the fp32 one, quantised: the same activation, so that the two agree in every byte
+    constexpr bool HALF = YT == LL_T_BF16 || YT == LL_T_F16;
     const int lane = threadIdx.x & 31, j = lane & 7, c = c0 + 8 * j, have = p.M - c;
     auto piece = [&](int r, int i) {  // 16 pieces of a row: two stretches of 8
         return reinterpret_cast<float4 *>(out + r * 256 + (i >> 3) * 128 + (((i ^ r) & 7) << 4));
@@ -544,12 +546,12 @@ __device__ __forceinline__ void dl_store_64cols(const DenseF8Params &p, uint8_t 
 #pragma unroll
             for (int e = 0; e < 8; ++e)
                 v[e] += bias[e];
-            if constexpr (YT != LL_T_F32 && ACT == LL_ACT_GELU) {
+            if constexpr (HALF && ACT == LL_ACT_GELU) {
                 ops_gelu_fast(v);
             } else {
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                    v[e] = YT == LL_T_F32 ? ops_act(v[e], ACT) : ops_act_fast(v[e], ACT);
+                    v[e] = HALF ? ops_act_fast(v[e], ACT) : ops_act(v[e], ACT);
             }
             if constexpr (YT == LL_T_F8) {
                 *piece(r, 2 * j) = make_float4(v[0], v[1], v[2], v[3]);
@@ -583,7 +585,7 @@ __device__ __forceinline__ void dl_store_64cols(const DenseF8Params &p, uint8_t 
             for (int e = 0; e < 8; ++e) {
                 float *at = reinterpret_cast<float *>(piece(r, 2 * j + (e >> 2))) + (e & 3);
                 float v = *at + (p.bias && e < have ? __ldg(p.bias + c + e) : 0.0f);
-                v = YT == LL_T_F32 ? ops_act(v, ACT) : ops_act_fast(v, ACT);
+                v = HALF ? ops_act_fast(v, ACT) : ops_act(v, ACT);
                 const long long o = (row0 + r) * p.ldy + c + e;
                 if constexpr (YT == LL_T_F8) {
                     *at = e < have ? v : 0.0f;

@@ -57,7 +57,7 @@ __device__ __forceinline__ float ops_act(float v, int act)
     if (act == LL_ACT_GELU)
         return ops_gelu(v);
     if (act == LL_ACT_SILU)
-        return v / (1.0f + expf(-v));
+        return v / __fadd_rn(1.0f, expf(-v));  // no step is fused with another one, wherever this is compiled
     return v;
 }
 

@@ -601,3 +601,26 @@ def test_gelu_keeps_its_digits_for_negative_values(rows, M, y_type):
     big.d["w"].zero_()
     big.d["b"] = dev(np.full(M, np.inf, np.float32))
     assert np.all(big.run(ll.ACT_GELU, y_type)[0][:rows].float().cpu().numpy() == np.inf)
+
+
+@pytest.mark.gpu
+@pytest.mark.timeout(300)
+@pytest.mark.parametrize("rows,M,K", [
+    (1, 130, 300), (20, 520, 900), (150, 2000, 520), (1100, 1500, 300),  # few rows: tiles of 16, 32 and 128, split or not
+    (1290, 2048, 384), (2500, 1030, 700)])                               # many rows
+@pytest.mark.parametrize("act", [ll.ACT_IDENTITY, ll.ACT_RELU, ll.ACT_GELU, ll.ACT_SILU])
+def test_e4m3_result_is_the_fp32_result_quantised(rows, M, K, act):
+    # byte for byte, scales too: the bias spreads the values over the activations' whole range
+    import torch
+
+    c = DenseCase(rows, M, K, seed=41)
+    c.d["b"] = dev(np.linspace(-13.0, 6.0, M).astype(np.float32)[np.argsort(np.arange(M) * 7919 % M, kind="stable")])
+    f, _ = c.run(act, ll.T_F32)
+    q, s = c.run(act, ll.T_F8)
+    want_q = torch.full_like(q, 99)
+    want_s = torch.empty_like(s)
+    ll.quantize_fp8(f.data_ptr(), ll.T_F32, rows, M, want_q.data_ptr(), want_s.data_ptr(),
+                    stream=torch.cuda.current_stream().cuda_stream)
+    ll.ops_check()
+    assert torch.equal(s, want_s)
+    assert torch.equal(q, want_q)
