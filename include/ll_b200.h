@@ -463,6 +463,10 @@ int ll_dense_fp8(const uint8_t *d_W, const float *d_sw, const float *d_b, const 
  * LL_OK, or LL_ERR_DEVICE_FAULT when a bounded device-side wait ran out since the last check (the
  * outputs of the calls since then are not to be used; the word is cleared). */
 int ll_ops_check(void *stream);
+/* Bound on every device-side wait of those two in calls from now on, in the whole process (a captured call
+ * keeps the one it was captured with): 1 s at first, at most 60 s.  With 0 every wait gives up at once
+ * and the calls fail on the device: for a program that tests what it does then. */
+int ll_ops_set_wait_limit(uint64_t ns);
 
 /*
  * Mixture-of-experts layer for a few rows, in two kernels (no counterpart in the reference, whose

@@ -64,6 +64,7 @@ EXPORTED_SYMBOLS = [
     "ll_weights_save", "ll_weights_load", "ll_weights_net", "ll_weights_arrays", "ll_weights_free",
     "ll_submit_many", "ll_engine_bench_ring", "ll_engine_bench_ring_mt",
     "ll_quantize_fp8", "ll_quantize_fp8_blocks", "ll_dense_fp8", "ll_ops_check",
+    "ll_ops_set_wait_limit",
     "ll_moe_workspace_bytes", "ll_moe_forward",
 ]
 MAX_LAYERS = 24
@@ -247,6 +248,7 @@ def _sig(lib):
                                         ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int,
                                         _vp]),
         "ll_ops_check": (ctypes.c_int, [_vp]),
+        "ll_ops_set_wait_limit": (ctypes.c_int, [ctypes.c_uint64]),
         "ll_moe_workspace_bytes": (ctypes.c_int, [P(MoEDesc), ctypes.c_int, P(ctypes.c_size_t)]),
         "ll_moe_forward": (ctypes.c_int, [P(MoEDesc), P(MoEWeightsStruct), _vp, ctypes.c_int64, _vp, ctypes.c_int64,
                                           ctypes.c_int, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
@@ -696,6 +698,11 @@ def dense_fp8(W_ptr: int, sw_ptr: int, b_ptr: int, x_ptr: int, sx_ptr: int, y_pt
 def ops_check(stream: int = 0):
     """Raise if a device-side wait of dense_fp8 or moe_forward ran out since the last check (ll_ops_check)."""
     _check(lib().ll_ops_check(stream or None))
+
+
+def ops_set_wait_limit(ns: int = 1_000_000_000):
+    """Bound on the device-side waits of later dense_fp8 and moe_forward calls; 0 makes them fail (ll_ops_set_wait_limit)."""
+    _check(lib().ll_ops_set_wait_limit(ns))
 
 
 # ---- mixture-of-experts layer ----

@@ -195,6 +195,13 @@ int ops_status_word(int *device, unsigned **word)
     return LL_OK;
 }
 
+static unsigned long long g_wait_ns = llk::kOpsWaitNs;
+
+unsigned long long ops_wait_ns()
+{
+    return __atomic_load_n(&g_wait_ns, __ATOMIC_RELAXED);
+}
+
 int check_device_ptr(const char *op, const char *what, const void *p, int device, size_t align)
 {
     if ((reinterpret_cast<uintptr_t>(p) & (align - 1)) != 0) {
@@ -255,6 +262,16 @@ int ll_quantize_fp8(const void *d_x, int x_type, int rows, int dim, int64_t ldx,
     else
         llk::launch_quantize<__half>(d_x, ldx, rows, dim, pow2_scales != 0, d_q, ldq, d_s, st);
     LL_CUDA_TRY(cudaGetLastError());
+    return LL_OK;
+}
+
+int ll_ops_set_wait_limit(uint64_t ns)
+{
+    if (ns > llk::kOpsMaxWaitNs) {
+        llh::set_error("ll_ops_set_wait_limit: at most %llu ns (%llu)", llk::kOpsMaxWaitNs, (unsigned long long)ns);
+        return LL_ERR_INVALID_ARG;
+    }
+    __atomic_store_n(&llh::g_wait_ns, (unsigned long long)ns, __ATOMIC_RELAXED);
     return LL_OK;
 }
 

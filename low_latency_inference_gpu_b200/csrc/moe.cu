@@ -167,7 +167,7 @@ int ll_moe_forward(const ll_moe_desc *d, const ll_moe_weights *w, const void *d_
     p.user_ids = d_ids;
     p.user_probs = d_probs;
     p.status = status;
-    p.wait_ns = kOpsWaitNs;
+    p.wait_ns = llh::ops_wait_ns();
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     return d->wtype == LL_W_BF16 ? launch_moe_bf16(p, dev, st)
            : d->wtype == LL_W_I8 ? launch_moe_i8(p, dev, st)

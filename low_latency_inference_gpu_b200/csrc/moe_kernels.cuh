@@ -565,7 +565,8 @@ static __device__ __noinline__ void moe_copy_small(int grain, uint32_t dst, int 
 struct MoeRing {
     uint32_t base, bars;  // shared-memory addresses of this warp's stages and of a barrier for each
     uint32_t laps;        // of each stage's barrier, the phase that its next wait is for (a bit)
-    bool ok;              // no wait has run out
+    uint32_t out;         // stages whose bulk copies were issued and not yet waited for (a bit)
+    bool ok;              // no wait has run out; from then on nothing is issued or waited for
     bool bulk;            // up to 4 rows: bulk copies (a lane's takes 12 instructions, whatever its length)
     int rows, m, grain;
     int q, n;       // next tile to be copied, number of tiles
@@ -605,7 +606,7 @@ struct MoeRing {
     template <class TileAt>
     __device__ __forceinline__ void feed(TileAt tile_at)
     {
-        if (q < n) {
+        if (q < n && ok) {
             if (off == begin)
                 tile_at(q, s0, s1, half, have);
             const uint32_t dst = base + (uint32_t)(slot * kMoeStage);
@@ -617,6 +618,7 @@ struct MoeRing {
                 const uint32_t bar = bars + 8u * (uint32_t)slot, d = dst + (uint32_t)(lane * pitch());
                 if (lane == 0)
                     mbar_arrive_expect_tx(bar, (uint32_t)(len * n_rows));
+                out |= 1u << slot;
                 __syncwarp();
                 if (mine)
                     bulk_g2s(d, (lane < half ? s0 : s1) + (size_t)h * (size_t)row_bytes + off, (uint32_t)len, bar);
@@ -646,26 +648,29 @@ struct MoeRing {
     __device__ __forceinline__ void wait(const MoeParams &p, int at, volatile uint32_t *fail)
     {
         if (bulk) {
-            if (ok)
+            if (ok) {
                 ok = ops_wait_warp(bars + 8u * (uint32_t)at, (laps >> at) & 1u, p.wait_ns, fail, p.status, 6);
-            laps ^= 1u << at;
+                if (ok) {
+                    laps ^= 1u << at;
+                    out &= ~(1u << at);
+                }
+            }
         } else {
             asm volatile("cp.async.wait_group %0;" ::"n"(kMoeStages - 1) : "memory");
         }
         __syncwarp();
     }
 
-    // After a wait that ran out: what is still on its way lands (or a second passes for each stage) before the
-    // shared memory is given back.
-    __device__ __forceinline__ void drain(const MoeParams &p) const
+    // After a wait that ran out: what is still on its way lands (or kOpsDrainNs pass) before the shared memory
+    // is given back.
+    __device__ __forceinline__ void drain() const
     {
         if (ok || (threadIdx.x & 31) != 0)
             return;
-        for (int i = 0; i < kMoeStages; ++i) {
-            const uint64_t t0 = globaltimer();
-            while (!mbar_try_wait(bars + 8u * (uint32_t)i, ((laps >> i) & 1u) ^ 1u) && globaltimer() - t0 < p.wait_ns) {
-            }
-        }
+        const uint64_t t0 = globaltimer();
+        for (int i = 0; i < kMoeStages; ++i)
+            if ((out >> i) & 1u)
+                ops_drain(bars + 8u * (uint32_t)i, (laps >> i) & 1u, t0);
     }
 };
 
@@ -1235,7 +1240,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1) ll_moe_up_kernel(const __grid_
             }
         }
     }
-    ring.drain(p);
+    ring.drain();
 }
 
 // ---- kernel 2: down projection and the weighted sum ----
@@ -1376,7 +1381,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1) ll_moe_down_kernel(const __gri
         }
         __syncthreads();
     }
-    ring.drain(p);
+    ring.drain();
 }
 
 // Launches both kernels for one weight type (moe_bf16.cu, moe_i8.cu, moe_f8.cu).

@@ -15,8 +15,10 @@ namespace llk {
 constexpr int kF8Block = LL_F8_BLOCK;   // columns (and weight rows) that share one scale
 constexpr float kF8Max = 448.0f;        // largest e4m3 value
 constexpr int kOpsMaxDevices = 64;
-// Bound on every device-side wait of the stateless operators.
-constexpr unsigned long long kOpsWaitNs = 1000ull * 1000 * 1000;
+// Bound on every device-side wait of the stateless operators (ll_ops_set_wait_limit changes it), and the longest
+// that a CTA which gave up stays for its own copies and products in flight: independent of the first.
+constexpr unsigned long long kOpsWaitNs = 1000ull * 1000 * 1000, kOpsMaxWaitNs = 60 * kOpsWaitNs;
+constexpr unsigned long long kOpsDrainNs = 2000ull * 1000 * 1000;
 
 __host__ __device__ constexpr int type_bytes(int t)
 {
@@ -144,7 +146,7 @@ __device__ __forceinline__ void ops_gelu_fast(float (&v)[N])
 }
 
 // Bounded waits on a barrier of this CTA, by one thread or a whole warp.  Most end within the first
-// looks, which read no timer and keep the loop short.
+// looks, which read no timer and keep the loop short.  A bound of 0 gives up without a look.
 __device__ __forceinline__ bool ops_try_wait(uint32_t bar, uint32_t parity)
 {
     uint32_t done;
@@ -158,24 +160,48 @@ __device__ __forceinline__ bool ops_try_wait(uint32_t bar, uint32_t parity)
     return done != 0u;
 }
 
+__device__ __forceinline__ void ops_give_up(volatile uint32_t *fail, unsigned *status, uint32_t role)
+{
+    *fail = 1u;
+    atomicOr(status, 1u | (role << 8));
+}
+
 __device__ __forceinline__ bool ops_wait(uint32_t bar, uint32_t parity, unsigned long long bound_ns,
                                          volatile uint32_t *fail, unsigned *status, uint32_t role)
 {
+    const int looks = bound_ns != 0 ? 64 : 0;
 #pragma unroll 1
-    for (int i = 0; i < 64; ++i)
+    for (int i = 0; i < looks; ++i)
         if (ops_try_wait(bar, parity))
             return true;
+    if (bound_ns == 0) {
+        ops_give_up(fail, status, role);
+        return false;
+    }
     return tc_wait(bar, parity, bound_ns, fail, status, role);
 }
 
 __device__ __forceinline__ bool ops_wait_warp(uint32_t bar, uint32_t parity, unsigned long long bound_ns,
                                               volatile uint32_t *fail, unsigned *status, uint32_t role)
 {
+    const int looks = bound_ns != 0 ? 64 : 0;
 #pragma unroll 1
-    for (int i = 0; i < 64; ++i)
+    for (int i = 0; i < looks; ++i)
         if (__all_sync(0xffffffffu, ops_try_wait(bar, parity)))
             return true;
+    if (bound_ns == 0) {
+        if ((threadIdx.x & 31) == 0)
+            ops_give_up(fail, status, role);
+        return false;
+    }
     return tc_wait_warp(bar, parity, bound_ns, fail, status, role);
+}
+
+// What a CTA that gave up still waits for: phase `parity` of `bar`, until kOpsDrainNs after t0.
+__device__ __forceinline__ void ops_drain(uint32_t bar, uint32_t parity, uint64_t t0)
+{
+    while (!mbar_try_wait(bar, parity) && globaltimer() - t0 < kOpsDrainNs) {
+    }
 }
 
 // One lane of a converged warp, the same one every time: true there.  With the warp converged around it the
@@ -275,6 +301,9 @@ namespace llh {
 // Device word that a stateless operator's kernel sets when a bounded wait runs out (one per GPU,
 // read and cleared by ll_ops_check).  Looked up once per device.
 int ops_status_word(int *device, unsigned **word);
+
+// The bound of device-side waits that calls from now on take.
+unsigned long long ops_wait_ns();
 
 // LL_OK when p is memory of the current device (managed memory included), aligned to `align` bytes.
 int check_device_ptr(const char *op, const char *what, const void *p, int device, size_t align);

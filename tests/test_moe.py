@@ -435,3 +435,53 @@ def test_layers_in_a_row_write_over_their_input(rows, wtype, x_type):
         g.replay()
         assert torch.equal(x, want[-1][1])
     ll.ops_check()
+
+
+def test_the_limit_of_waits_is_bounded():
+    refused(ll.ops_set_wait_limit, ll.LL_ERR_INVALID_ARG, 60_000_000_001)
+    ll.ops_set_wait_limit()
+
+
+@pytest.mark.gpu
+@pytest.mark.timeout(300)
+@pytest.mark.parametrize("rows,hidden,inter,experts,top_k,wtype,x_type", [
+    (1, 256, 128, 8, 2, ll.W_BF16, ll.T_BF16),     # bulk copies in both kernels: the up kernel's first wait gives up
+    (1, 1024, 512, 8, 2, ll.W_F8, ll.T_BF16),
+    (3, 512, 96, 4, 2, ll.W_I8, ll.T_F32),
+    (32, 384, 512, 40, 8, ll.W_BF16, ll.T_F16),    # in the down kernel alone
+])
+def test_a_wait_that_runs_out_is_reported_and_the_next_call_is_right(rows, hidden, inter, experts, top_k, wtype, x_type):
+    # with a limit of 0 every wait gives up with its copies in flight: they land before the kernel ends, the
+    # status says so, and the calls behind it on the same stream are as ever
+    import torch
+
+    layer = Layer(ll.MoE(hidden, inter, experts, top_k, wtype=wtype, x_type=x_type), rows, seed=5)
+    layer.run()
+    ll.ops_check()
+    layer.check()
+    want = layer.y.clone()
+    for _ in range(3):
+        ll.ops_set_wait_limit(0)
+        try:
+            layer.run()
+        finally:
+            ll.ops_set_wait_limit()
+        layer.run()
+        with pytest.raises(ll.LLError) as e:
+            ll.ops_check()
+        assert e.value.code == ll.LL_ERR_DEVICE_FAULT
+        assert torch.equal(layer.y, want)
+        ll.ops_check()
+
+
+@pytest.mark.gpu
+@pytest.mark.timeout(300)
+def test_rows_that_start_on_no_16_bytes_wait_for_no_barrier():
+    layer = Layer(ll.MoE(129, 65, 7, 3, x_type=ll.T_F32), 3, seed=6)
+    ll.ops_set_wait_limit(0)
+    try:
+        layer.run()
+    finally:
+        ll.ops_set_wait_limit()
+    ll.ops_check()
+    layer.check()
