@@ -173,6 +173,13 @@ __device__ __forceinline__ void cluster_wait()
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+__device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t cluster_addr)
+{
+    uint32_t v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(cluster_addr) : "memory");
+    return v;
+}
+
 __device__ __forceinline__ void st_cluster_f32(uint32_t cluster_addr, float v)
 {
     asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_addr), "f"(v) : "memory");
@@ -377,14 +384,6 @@ __global__ void __launch_bounds__(kDsThreads, 1) ll_dense_fp8_kernel(const __gri
                 st_cluster_f32(mapa(part + (uint32_t)((((c >> log2) << log2) + rank) * 512), (uint32_t)(c & mask)), acc[c]);
         }
     }
-    // A CTA that gave up leaves loads in flight: they land before its shared memory is given back.
-    if (warp == 0 && lane == 0 && *fail) {
-        for (int j = max(0, issued - S); j < issued; ++j) {
-            const uint64_t w0 = globaltimer();
-            while (!mbar_try_wait(b_full(j % S), (j / S) & 1) && globaltimer() - w0 < p.wait_ns) {
-            }
-        }
-    }
     __syncwarp();
     if (splits > 1 && warp < 2) {  // the producers' part of the barrier that the others have passed
         if (!L::OWN_PART)
@@ -398,13 +397,18 @@ __global__ void __launch_bounds__(kDsThreads, 1) ll_dense_fp8_kernel(const __gri
     } else {
         __syncthreads();
     }
-    if (warp == 1) {
-        if (*fail && lane == 0) {
-            const uint64_t w0 = globaltimer();
-            while (!mbar_try_wait(b_done, 0) && globaltimer() - w0 < p.wait_ns) {
-            }
-        }
+    // Every role has ended, so nobody gives up any more.  A CTA in which one did has loads and MMAs in flight: they
+    // end before its shared and tensor memory are given back.
+    if (*fail) {
+        const uint64_t w0 = globaltimer();
+        if (warp == 0 && lane == 0)
+            for (int j = max(0, issued - S); j < issued; ++j)
+                ops_drain(b_full(j % S), (j / S) & 1, w0);
+        if (warp == 1 && lane == 0)
+            ops_drain(b_done, 0, w0);
         __syncwarp();
+    }
+    if (warp == 1) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(L::TMEM_COLS)
                      : "memory");
@@ -730,11 +734,19 @@ __global__ void __launch_bounds__(kDlThreads, 1) ll_dense_fp8_large_kernel(const
     cluster_sync();  // both CTAs' barriers are initialised and their tensor memory allocated
     tc_fence_after();
     const uint32_t tmem = misc[0];
-    int issued = 0;
 
     if (warp < 4) {
         // 384 threads were launched with 168 registers each: 256 x 224 + 128 x 56 is just that
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        int issued = 0;  // producer: K blocks whose loads were started
+        auto load = [&](int s, int mt, int nt, int kb) {
+            if (lead)
+                mbar_arrive_expect_tx(b_full(s), 2 * kDlStage);  // both CTAs' loads land on this barrier
+            const uint32_t full = mapa(b_full(s), 0u);
+            tma_load_2d_pair(sbase + s * kDlStage, &p.tm_x, kb * kF8Block, (2 * mt + (int)rank) * kDlM, full);
+            tma_load_2d_pair(sbase + s * kDlStage + kDlM * kF8Block, &p.tm_w, kb * kF8Block,
+                             nt * kDlN + (int)rank * (kDlN / 2), full);
+        };
         if (warp == 0) {
             if (lane == 0) {
                 bool ok = true;
@@ -748,16 +760,13 @@ __global__ void __launch_bounds__(kDlThreads, 1) ll_dense_fp8_large_kernel(const
                             ok = false;
                             break;
                         }
-                        if (lead)
-                            mbar_arrive_expect_tx(b_full(s), 2 * kDlStage);  // both CTAs' loads land on this barrier
-                        const uint32_t full = mapa(b_full(s), 0u);
-                        tma_load_2d_pair(sbase + s * kDlStage, &p.tm_x, kb * kF8Block, (2 * mt + (int)rank) * kDlM, full);
-                        tma_load_2d_pair(sbase + s * kDlStage + kDlM * kF8Block, &p.tm_w, kb * kF8Block,
-                                         nt * kDlN + (int)rank * (kDlN / 2), full);
+                        load(s, mt, nt, kb);
                         ++issued;
                     }
                 }
+                misc[2] = (uint32_t)issued;
             }
+            __syncwarp();
         } else if (warp == 1) {
             if (lead) {  // the whole warp, so that the loop runs on uniform registers; one lane issues
                 constexpr uint32_t idesc = tc_idesc_e4m3_pair(kDlN);
@@ -795,6 +804,29 @@ __global__ void __launch_bounds__(kDlThreads, 1) ll_dense_fp8_large_kernel(const
                 __syncwarp();
             }
         }
+        tc_fence_before();
+        cluster_sync();  // every role of both CTAs has ended: nobody gives up any more
+        if (warp == 0 && lane == 0) {
+            const uint32_t peer = mapa(sbase + (uint32_t)kDlOffMisc, rank ^ 1u);
+            if (*fail || ld_cluster_u32(peer + 4u)) {
+                // The loads in flight land before the shared memory is given back.  CTA 0's barriers count both
+                // CTAs' bytes, so a CTA that stopped earlier than its peer first issues what it is behind:
+                // at most S blocks, each into a stage whose last MMAs had released the peer.
+                const int n = max(issued, (int)ld_cluster_u32(peer + 8u));
+                for (; issued < n; ++issued) {
+                    const int t = issued / p.nkb;
+                    int mt, nt;
+                    tile_at(pair + t * pairs, mt, nt);
+                    load(issued % S, mt, nt, issued - t * p.nkb);
+                }
+                const uint64_t w0 = globaltimer();
+                for (int j = max(0, n - S); lead && j < n; ++j)
+                    ops_drain(b_full(j % S), (j / S) & 1, w0);
+            }
+        }
+        if (warp == 1 && lane == 0)
+            ops_drain(b_done, 0, globaltimer());
+        __syncwarp();
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         const int quad = warp & 3, half = (warp - 4) >> 2, mblocks = (p.M + kF8Block - 1) / kF8Block;
@@ -882,25 +914,9 @@ __global__ void __launch_bounds__(kDlThreads, 1) ll_dense_fp8_large_kernel(const
             if (ok && c0 < p.M)
                 dl_store<YT>(p, out, acc, row0, c0);
         }
+        tc_fence_before();
+        cluster_sync();  // with the other warps' above
     }
-    if (lead && warp == 0 && lane == 0 && *fail) {  // both CTAs' loads in flight land before the shared memory is given back
-        for (int j = max(0, issued - S); j < issued; ++j) {
-            const uint64_t w0 = globaltimer();
-            while (!mbar_try_wait(b_full(j % S), (j / S) & 1) && globaltimer() - w0 < p.wait_ns) {
-            }
-        }
-    }
-    __syncwarp();
-    tc_fence_before();
-    __syncthreads();
-    if (warp == 1) {
-        if (lane == 0) {
-            const uint64_t w0 = globaltimer();
-            while (!mbar_try_wait(b_done, 0) && globaltimer() - w0 < p.wait_ns) {
-            }
-        }
-    }
-    __syncthreads();
     cluster_sync();  // the pair's MMAs are complete in both CTAs, and nobody arrives at the peer any more
     if (warp == 1) {
         tc_fence_after();
@@ -1047,7 +1063,7 @@ extern "C" int ll_dense_fp8(const uint8_t *d_W, const float *d_sw, const float *
     const int v4 = 4 * type_bytes(y_type);  // bytes of four outputs
     p.y_vec = (ldy % 4 == 0 && (reinterpret_cast<uintptr_t>(d_y) % v4) == 0) ? 1 : 0;
     p.status = status;
-    p.wait_ns = kOpsWaitNs;
+    p.wait_ns = llh::ops_wait_ns();
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     // Which kernel, measured in a graph on B200 (us; many-row kernel / few-row kernel at its best):
     //   32 tiles of 256 x 256 and more: 1024 x 2048 x 1024 12.6 / 13.2, 512 x 4096 x 4096 26 / 33,

@@ -624,3 +624,34 @@ def test_e4m3_result_is_the_fp32_result_quantised(rows, M, K, act):
     ll.ops_check()
     assert torch.equal(s, want_s)
     assert torch.equal(q, want_q)
+
+
+@pytest.mark.gpu
+@pytest.mark.timeout(300)
+@pytest.mark.parametrize("rows,M,K,y_type", [
+    (1, 16, 16, ll.T_F32), (1, 2048, 2048, ll.T_BF16),       # one block; two blocks in each of eight CTAs
+    (20, 512, 4096, ll.T_F8), (8, 300, 40000, ll.T_F32),     # as many blocks as stages and more
+    (1100, 1500, 1300, ll.T_F32),                            # tiles of 128 rows
+    (1290, 2048, 384, ll.T_BF16), (2560, 4096, 1024, ll.T_F8),  # pairs of SMs: within the first stages, and beyond
+])
+def test_a_wait_that_runs_out_is_reported_and_the_next_call_is_right(rows, M, K, y_type):
+    # with a limit of 0 every wait gives up: loads and products in flight end before the kernel does, the status
+    # says so, and the calls behind it are as ever
+    import torch
+
+    c = DenseCase(rows, M, K, seed=51)
+    want, want_s = c.run(ll.ACT_RELU, y_type)
+    ll.ops_check()
+    y, sy = want.clone(), want_s.clone()
+    for _ in range(3):
+        ll.ops_set_wait_limit(0)
+        try:
+            c.run(ll.ACT_RELU, y_type, y=y, sy=sy)
+        finally:
+            ll.ops_set_wait_limit()
+        c.run(ll.ACT_RELU, y_type, y=y, sy=sy)
+        with pytest.raises(ll.LLError) as e:
+            ll.ops_check()
+        assert e.value.code == ll.LL_ERR_DEVICE_FAULT
+        assert torch.equal(y, want) and torch.equal(sy, want_s)
+        ll.ops_check()
