@@ -459,9 +459,10 @@ void ll_quantize_fp8_blocks(const float *W, int m, int k, uint8_t *q, float *s);
 int ll_dense_fp8(const uint8_t *d_W, const float *d_sw, const float *d_b, const uint8_t *d_x, const float *d_sx,
                  void *d_y, float *d_sy, int y_type, int rows, int M, int K, int64_t ldw, int64_t ldx, int64_t ldy,
                  int act, void *stream);
-/* Synchronise `stream` and read the current device's status word of ll_dense_fp8 and ll_moe_forward:
- * LL_OK, or LL_ERR_DEVICE_FAULT when a bounded device-side wait ran out since the last check (the
- * outputs of the calls since then are not to be used; the word is cleared). */
+/* Synchronise `stream` and look whether a bounded device-side wait of ll_dense_fp8 or ll_moe_forward ran out on
+ * the current device, in any stream, since the calling thread's last check of this stream (ever, at its first):
+ * LL_ERR_DEVICE_FAULT if so, and the outputs of the calls on this stream since then are not to be used.  Every
+ * thread and stream is told of each failure; no check takes it from another one. */
 int ll_ops_check(void *stream);
 /* Bound on every device-side wait of those two in calls from now on, in the whole process (a captured call
  * keeps the one it was captured with): 1 s at first, at most 60 s.  With 0 every wait gives up at once

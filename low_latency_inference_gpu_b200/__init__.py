@@ -696,7 +696,8 @@ def dense_fp8(W_ptr: int, sw_ptr: int, b_ptr: int, x_ptr: int, sx_ptr: int, y_pt
 
 
 def ops_check(stream: int = 0):
-    """Raise if a device-side wait of dense_fp8 or moe_forward ran out since the last check (ll_ops_check)."""
+    """Raise if a device-side wait of dense_fp8 or moe_forward ran out since this thread's last check of the stream
+    (ll_ops_check)."""
     _check(lib().ll_ops_check(stream or None))
 
 

@@ -1037,7 +1037,7 @@ extern "C" int ll_dense_fp8(const uint8_t *d_W, const float *d_sw, const float *
     }
     int dev = 0;
     unsigned *status = nullptr;
-    LL_TRY(llh::ops_status_word(&dev, &status));
+    LL_TRY(llh::ops_status_words(&dev, &status));
     LL_TRY(llh::check_device_ptr(op, "W", d_W, dev, 16));
     LL_TRY(llh::check_device_ptr(op, "the scales of W", d_sw, dev, 4));
     LL_TRY(llh::check_device_ptr(op, "x", d_x, dev, 16));

@@ -170,13 +170,13 @@ void launch_quantize(const void *x, long long ldx, int rows, int dim, bool pow2,
         ll_quantize_fp8_kernel<T, false><<<grid, kQtThreads, 0, st>>>((const T *)x, ldx, dim, n, fd, q, ldq, s, pow2);
 }
 
-__device__ unsigned g_ops_status;  // see llh::ops_status_word
+__device__ unsigned g_ops_status[2];  // see llh::ops_status_words
 
 }  // namespace llk
 
 namespace llh {
 
-int ops_status_word(int *device, unsigned **word)
+int ops_status_words(int *device, unsigned **words)
 {
     static unsigned *at[llk::kOpsMaxDevices];  // racing first calls store the same address
     LL_CUDA_TRY(cudaGetDevice(device));
@@ -191,7 +191,7 @@ int ops_status_word(int *device, unsigned **word)
         p = static_cast<unsigned *>(v);
         __atomic_store_n(&at[*device], p, __ATOMIC_RELEASE);
     }
-    *word = p;
+    *words = p;
     return LL_OK;
 }
 
@@ -277,17 +277,36 @@ int ll_ops_set_wait_limit(uint64_t ns)
 
 int ll_ops_check(void *stream)
 {
+    // The device's count is never reset, so that no check takes a failure from another one; what each has told its
+    // caller is kept here, per thread, stream and device, once there is something to tell.
+    struct Told {
+        void *stream;
+        int device;
+        unsigned failures;
+    };
+    constexpr int kTold = 64;  // of more streams than these the oldest is told again
+    static thread_local Told told[kTold];
+    static thread_local unsigned n_told;
+
     int dev = 0;
-    unsigned *word = nullptr, v = 0;
-    LL_TRY(llh::ops_status_word(&dev, &word));
+    unsigned *words = nullptr, now[2] = {0, 0};
+    LL_TRY(llh::ops_status_words(&dev, &words));
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    LL_CUDA_TRY(cudaMemcpyAsync(&v, word, sizeof(v), cudaMemcpyDeviceToHost, st));
+    LL_CUDA_TRY(cudaMemcpyAsync(now, words, sizeof(now), cudaMemcpyDeviceToHost, st));
     LL_CUDA_TRY(cudaStreamSynchronize(st));
-    if (v == 0)
+    if (now[0] == 0)
         return LL_OK;
-    LL_CUDA_TRY(cudaMemsetAsync(word, 0, sizeof(v), st));
-    LL_CUDA_TRY(cudaStreamSynchronize(st));
-    llh::set_error("a device-side wait of ll_dense_fp8 or ll_moe_forward ran out (role %u)", (v >> 8) & 0xffu);
+    Told *t = nullptr;
+    for (unsigned i = 0; i < kTold && i < n_told && !t; ++i)
+        if (told[i].stream == stream && told[i].device == dev)
+            t = &told[i];
+    if (t && t->failures == now[0])
+        return LL_OK;
+    if (!t)
+        t = &told[n_told++ % kTold];
+    *t = {stream, dev, now[0]};
+    llh::set_error("a device-side wait of ll_dense_fp8 or ll_moe_forward ran out (%u in all, the last in role %u)", now[0],
+                   now[1]);
     return LL_ERR_DEVICE_FAULT;
 }
 

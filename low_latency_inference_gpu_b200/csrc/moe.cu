@@ -105,7 +105,7 @@ int ll_moe_forward(const ll_moe_desc *d, const ll_moe_weights *w, const void *d_
     }
     int dev = 0;
     unsigned *status = nullptr;
-    LL_TRY(llh::ops_status_word(&dev, &status));
+    LL_TRY(llh::ops_status_words(&dev, &status));
     const size_t xa = (size_t)type_bytes(d->x_type), wa = d->wtype == LL_W_BF16 ? 2 : 1;
     LL_TRY(llh::check_device_ptr(op, "x", d_x, dev, xa));
     LL_TRY(llh::check_device_ptr(op, "y", d_y, dev, xa));

@@ -160,41 +160,58 @@ __device__ __forceinline__ bool ops_try_wait(uint32_t bar, uint32_t parity)
     return done != 0u;
 }
 
+// status: how many waits ran out, never reset, and the role of the last one (llh::ops_status_words).
 __device__ __forceinline__ void ops_give_up(volatile uint32_t *fail, unsigned *status, uint32_t role)
 {
     *fail = 1u;
-    atomicOr(status, 1u | (role << 8));
+    atomicExch(status + 1, role);
+    atomicAdd(status, 1u);
 }
 
 __device__ __forceinline__ bool ops_wait(uint32_t bar, uint32_t parity, unsigned long long bound_ns,
                                          volatile uint32_t *fail, unsigned *status, uint32_t role)
 {
-    const int looks = bound_ns != 0 ? 64 : 0;
+    uint64_t t0 = 0;
 #pragma unroll 1
-    for (int i = 0; i < looks; ++i)
+    for (uint32_t it = 1; bound_ns != 0; ++it) {
         if (ops_try_wait(bar, parity))
             return true;
-    if (bound_ns == 0) {
-        ops_give_up(fail, status, role);
-        return false;
+        if ((it & 63u) == 0) {
+            if (*fail)  // another role of the CTA gave up
+                return false;
+            const uint64_t now = globaltimer();
+            if (t0 == 0)
+                t0 = now;
+            else if (now - t0 > bound_ns)
+                break;
+        }
     }
-    return tc_wait(bar, parity, bound_ns, fail, status, role);
+    ops_give_up(fail, status, role);
+    return false;
 }
 
+// Every lane looks for itself (so that what the phase guards is visible to each) and the verdict is the warp's.
 __device__ __forceinline__ bool ops_wait_warp(uint32_t bar, uint32_t parity, unsigned long long bound_ns,
                                               volatile uint32_t *fail, unsigned *status, uint32_t role)
 {
-    const int looks = bound_ns != 0 ? 64 : 0;
+    uint64_t t0 = 0;
 #pragma unroll 1
-    for (int i = 0; i < looks; ++i)
+    for (uint32_t it = 1; bound_ns != 0; ++it) {
         if (__all_sync(0xffffffffu, ops_try_wait(bar, parity)))
             return true;
-    if (bound_ns == 0) {
-        if ((threadIdx.x & 31) == 0)
-            ops_give_up(fail, status, role);
-        return false;
+        if ((it & 63u) == 0) {
+            if (__any_sync(0xffffffffu, *fail != 0u))
+                return false;
+            const uint64_t now = globaltimer();
+            if (t0 == 0)
+                t0 = now;
+            else if (__any_sync(0xffffffffu, now - t0 > bound_ns))
+                break;
+        }
     }
-    return tc_wait_warp(bar, parity, bound_ns, fail, status, role);
+    if ((threadIdx.x & 31) == 0)
+        ops_give_up(fail, status, role);
+    return false;
 }
 
 // What a CTA that gave up still waits for: phase `parity` of `bar`, until kOpsDrainNs after t0.
@@ -298,9 +315,9 @@ __device__ __forceinline__ uint32_t group_e4m3x4(const float *v, bool pow2, floa
 
 namespace llh {
 
-// Device word that a stateless operator's kernel sets when a bounded wait runs out (one per GPU,
-// read and cleared by ll_ops_check).  Looked up once per device.
-int ops_status_word(int *device, unsigned **word);
+// Device words in which a stateless operator's kernel counts the bounded waits that ran out, and notes the role
+// of the last one (one pair per GPU, never reset; read by ll_ops_check).  Looked up once per device.
+int ops_status_words(int *device, unsigned **words);
 
 // The bound of device-side waits that calls from now on take.
 unsigned long long ops_wait_ns();

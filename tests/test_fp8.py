@@ -655,3 +655,46 @@ def test_a_wait_that_runs_out_is_reported_and_the_next_call_is_right(rows, M, K,
         assert e.value.code == ll.LL_ERR_DEVICE_FAULT
         assert torch.equal(y, want) and torch.equal(sy, want_s)
         ll.ops_check()
+
+
+@pytest.mark.gpu
+@pytest.mark.timeout(300)
+def test_every_stream_and_thread_is_told_of_a_failure():
+    # a failure on stream b: the check of stream a takes nothing from b's, whichever comes first, nor from
+    # another thread's; each is told once
+    import threading
+
+    import torch
+
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    c = DenseCase(3, 128, 256, seed=61)
+    y, sy = c.run(ll.ACT_RELU, ll.T_F32)
+    torch.cuda.synchronize()
+
+    def told(stream):
+        try:
+            ll.ops_check(stream.cuda_stream)
+            return False
+        except ll.LLError as e:
+            assert e.code == ll.LL_ERR_DEVICE_FAULT
+            return True
+
+    def elsewhere(stream):
+        out = []
+        t = threading.Thread(target=lambda: out.extend((told(stream), told(stream))))
+        t.start()
+        t.join()
+        return out
+
+    for first, second in ((a, b), (b, a)):
+        ll.ops_set_wait_limit(0)
+        try:
+            c.run(ll.ACT_RELU, ll.T_F32, stream=b, y=y, sy=sy)
+        finally:
+            ll.ops_set_wait_limit()
+        b.synchronize()
+        assert told(first)
+        assert told(second)
+        assert elsewhere(b) == [True, False]
+        assert not told(first) and not told(second)
+    assert told(torch.cuda.default_stream()) and not told(torch.cuda.default_stream())
