@@ -72,7 +72,8 @@ __device__ __forceinline__ void load_all(const T *p, float (&v)[kQtPer])
 // least 2^-17 (relative) away from it; v / s differs from it by the rounding of s alone, one
 // factor for the whole group within 2^-24.  So where s is not exact, a factor of 1 +- 2^-20
 // towards the side on which that rounding puts the quotients decides the ties and changes nothing
-// else; where it is (or is the smallest scale), one correction step makes the quotient exact.
+// else; where it is, one correction step makes the quotient exact.  (Not for scales below kF8SmallScale, whose
+// residuals would be fp32's subnormal numbers: those groups go the way of fp32 values.)
 struct Scale16 {
     float s, inv, by;  // by: the reciprocal with the group's factor
     bool exact;
@@ -81,7 +82,7 @@ struct Scale16 {
 __device__ __forceinline__ Scale16 scale16(float amax, float s, float inv)
 {
     const float d = fmaf(-kF8Max, s, amax);  // exact: s is amax / 448 to 2^-24
-    const bool exact = d == 0.0f || s <= 0x1p-126f;
+    const bool exact = d == 0.0f;
     return {s, inv, exact ? inv : inv * (d > 0.0f ? 1.0f + 0x1p-20f : 1.0f - 0x1p-20f), exact};
 }
 
@@ -130,7 +131,7 @@ __global__ void __launch_bounds__(kQtThreads) ll_quantize_fp8_kernel(const T *__
     float sc, inv;
     e4m3_scale(amax, pow2, sc, inv);
     uint32_t o[kQtPer / 4];
-    if (sizeof(T) == 2 && !pow2) {
+    if (sizeof(T) == 2 && !pow2 && !(sc < kF8SmallScale && sc != 0.0f)) {
         const Scale16 f = scale16(amax, sc, inv);
 #pragma unroll
         for (int i = 0; i < kQtPer / 4; ++i)

@@ -14,6 +14,7 @@ namespace llk {
 
 constexpr int kF8Block = LL_F8_BLOCK;   // columns (and weight rows) that share one scale
 constexpr float kF8Max = 448.0f;        // largest e4m3 value
+constexpr float kF8SmallScale = 0x1p-60f;  // v - s times an e4m3 border may be subnormal well below this
 constexpr int kOpsMaxDevices = 64;
 // Bound on every device-side wait of the stateless operators (ll_ops_set_wait_limit changes it), and the longest
 // that a CTA which gave up stays for its own copies and products in flight: independent of the first.
@@ -254,12 +255,14 @@ __device__ __forceinline__ float e4m3_value(uint32_t code)
 
 // Of two neighbouring e4m3 codes (one byte each, of v's sign) the one nearest to the exact quotient v / s:
 // the sign of |v| - border * s, one fused operation, says on which side of the border (5 significant
-// bits, exact) the quotient lies; a tie goes to the even code.
+// bits, exact) the quotient lies; a tie goes to the even code.  Of a small scale both are lifted by a power of
+// two: among fp32's subnormal numbers the difference would be rounded to 0.
 __device__ __forceinline__ uint32_t nearer_e4m3(float v, float s, uint32_t a, uint32_t b)
 {
     const uint32_t lo = min(a, b) & 0x7fu, hi = max(a, b) & 0x7fu, sign = a & 0x80u;
     const float border = 0.5f * (e4m3_value(lo) + e4m3_value(hi));
-    const float side = fmaf(-border, s, fabsf(v));
+    const float lift = s < kF8SmallScale ? 1.0f / kF8SmallScale : 1.0f;
+    const float side = fmaf(-border, s * lift, fabsf(v) * lift);
     return sign | (side > 0.0f ? hi : side < 0.0f ? lo : lo + (lo & 1u));
 }
 

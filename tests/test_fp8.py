@@ -698,3 +698,40 @@ def test_every_stream_and_thread_is_told_of_a_failure():
         assert elsewhere(b) == [True, False]
         assert not told(first) and not told(second)
     assert told(torch.cuda.default_stream()) and not told(torch.cuda.default_stream())
+
+
+@pytest.mark.gpu
+@pytest.mark.timeout(300)
+@pytest.mark.parametrize("x_type", [ll.T_F32, ll.T_BF16])
+def test_quantize_ties_of_the_smallest_scales(x_type):
+    # groups whose scale is 2^-126 or little more: what separates a quotient from a border of two e4m3 values is
+    # below fp32's smallest number there, and still decides
+    rows = []
+    mids = (TABLE[:-1] + TABLE[1:]) / 2
+    if x_type == ll.T_F32:
+        sig = np.concatenate([1 + np.arange(1, 40) * 2.0 ** -23, np.linspace(1.0, 2.0, 25)])
+        for e in (-126, -125, -120, -110, -66, -60):
+            for g in sig:
+                s = np.float32(g * 2.0 ** e)
+                amax = np.float32(448.0 * s)
+                s = np.float32(amax / np.float32(448))
+                v = (mids * np.float64(s)).astype(np.float32)
+                v = np.concatenate([np.nextafter(v[:42], np.float32(0)), v[42:84], np.nextafter(v[84:], np.float32(1))])
+                rows.append(np.concatenate([v, [amax, -amax]]))
+    else:
+        for k in range(1, 37):  # the scales that are exact in 16 bits
+            for e in range(-126 - 5, -112):
+                s = k * 2.0 ** e
+                if s < 2.0 ** -126:
+                    continue
+                v = (mids * s).astype(np.float32)
+                u = v.view(np.uint32)
+                u += 0x7FFF + ((u >> 16) & 1)
+                u &= np.uint32(0xFFFF0000)
+                rows.append(np.concatenate([v, [448 * s, -448 * s]]))
+    x = np.stack(rows).astype(np.float32)
+    assert x.shape[1] == F8
+    q, s, x = run_quantize(x, x_type)
+    want_q, want_s = quantize_rows(x)
+    assert np.array_equal(s, want_s)
+    assert np.array_equal(decode(q), decode(want_q))
