@@ -151,7 +151,7 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1
 
 // Weight types: EP values in 16 bytes; widen() gives them as EP / 2 packed bf16 pairs times UNIT
 // (exact).  PERM: of every four values the pairs are (0, 2) and (1, 3), and x follows.
-constexpr float kMoeF8Up = 0x1p40f, kMoeF8Back = 0x1p80f;
+constexpr float kMoeF8Up = 0x1p64f, kMoeF8Back = 0x1p56f;  // 0x1p120f together
 
 template <int WT>
 struct MoeW;
@@ -194,10 +194,11 @@ struct MoeW<LL_W_F8> {
     static constexpr bool PERM = true;
     // Sign, exponent and significand moved to their bf16 places are the value times 2^-120 (the
     // exponents' biases differ by 120; e4m3's subnormals become bf16's).  x is multiplied by
-    // kMoeF8Up = 2^40 beforehand, so the sums carry 2^-80, far above fp32's underflow, and are
-    // multiplied by kMoeF8Back at the end: 7 operations for 4 values, where the conversion
-    // instructions run at a fraction of the rate.  NaN (0x7f) would read as 480: `nan` collects
-    // a mark (bit 7 of a byte) for it, and the row's sums become NaN at the tile's end.
+    // kMoeF8Up = 2^64 beforehand, so a block's sum carries 2^-56 and is multiplied by kMoeF8Back on its
+    // way to the others: x below 2^64 does not overflow in bf16, and sums from 2^-70 on are fp32's
+    // normal numbers.  7 operations for 4 values, where the conversion instructions run at a fraction
+    // of the rate.  NaN (0x7f) would read as 480: `nan` collects a mark (bit 7 of a byte) for it, and the
+    // row's sums become NaN at the tile's end.
     static __device__ __forceinline__ void widen(const uint4 &v, uint32_t (&o)[8], uint32_t &nan)
     {
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -310,8 +311,8 @@ struct MoeX {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     w[0][4 * i + j] = u[j];
-                    if constexpr (PERM)  // 0x5380: 2^40
-                        asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(w[0][4 * i + j]) : "r"(0x53805380u));
+                    if constexpr (PERM)  // 0x5f80: 2^64
+                        asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(w[0][4 * i + j]) : "r"(0x5f805f80u));
                 }
             } else {
 #pragma unroll
@@ -712,6 +713,7 @@ __device__ __forceinline__ void moe_tile(const MoeParams &p, MoeRing &r, volatil
     // x from global memory is loaded a step ahead where the registers allow (2 x 32)
     constexpr bool PRE = Src::GLOBAL && 2 * RAW * 4 <= 32;
     constexpr bool FRESH = WT == LL_W_F8 || NS == 3;
+    constexpr float back = WT == LL_W_F8 ? kMoeF8Back : 1.0f;
     const int t = threadIdx.x & 3, last = (K + kF8Block - 1) / kF8Block - 1;
     uint4 ba[PRE ? 2 : 1][RAW], bb[PRE ? 2 : 1][RAW];
     float fa0 = 1.0f, fa1 = 1.0f, fb0 = 1.0f, fb1 = 1.0f;  // e4m3: scales of rows g and g + 8
@@ -779,20 +781,20 @@ __device__ __forceinline__ void moe_tile(const MoeParams &p, MoeRing &r, volatil
             products(d, e, r0, r1, b);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                acc[nt][0] = fmaf(d[nt][0] + e[nt][0], f0, acc[nt][0]);
-                acc[nt][1] = fmaf(d[nt][1] + e[nt][1], f0, acc[nt][1]);
-                acc[nt][2] = fmaf(d[nt][2] + e[nt][2], f1, acc[nt][2]);
-                acc[nt][3] = fmaf(d[nt][3] + e[nt][3], f1, acc[nt][3]);
+                acc[nt][0] = fmaf((d[nt][0] + e[nt][0]) * back, f0, acc[nt][0]);
+                acc[nt][1] = fmaf((d[nt][1] + e[nt][1]) * back, f0, acc[nt][1]);
+                acc[nt][2] = fmaf((d[nt][2] + e[nt][2]) * back, f1, acc[nt][2]);
+                acc[nt][3] = fmaf((d[nt][3] + e[nt][3]) * back, f1, acc[nt][3]);
             }
         } else if constexpr (FRESH) {
             float d[NT][4] = {};
             products(d, d, r0, r1, b);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                acc[nt][0] = fmaf(d[nt][0], f0, acc[nt][0]);
-                acc[nt][1] = fmaf(d[nt][1], f0, acc[nt][1]);
-                acc[nt][2] = fmaf(d[nt][2], f1, acc[nt][2]);
-                acc[nt][3] = fmaf(d[nt][3], f1, acc[nt][3]);
+                acc[nt][0] = fmaf(d[nt][0] * back, f0, acc[nt][0]);
+                acc[nt][1] = fmaf(d[nt][1] * back, f0, acc[nt][1]);
+                acc[nt][2] = fmaf(d[nt][2] * back, f1, acc[nt][2]);
+                acc[nt][3] = fmaf(d[nt][3] * back, f1, acc[nt][3]);
             }
         } else {
             products(acc, acc, r0, r1, b);
@@ -821,7 +823,7 @@ __device__ __forceinline__ void moe_tile(const MoeParams &p, MoeRing &r, volatil
         r.feed(tile_at);
     }
     if constexpr (WT == LL_W_F8) {
-        float s0 = kMoeF8Back, s1 = kMoeF8Back;
+        float s0 = 1.0f, s1 = 1.0f;
         const uint32_t lanes = 0xfu << (threadIdx.x & 28);  // the four threads of a row
         if (__ballot_sync(0xffffffffu, nan0 & 0x80808080u) & lanes)
             s0 = __uint_as_float(0x7fc00000u);

@@ -485,3 +485,38 @@ def test_rows_that_start_on_no_16_bytes_wait_for_no_barrier():
         ll.ops_set_wait_limit()
     ll.ops_check()
     layer.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.timeout(300)
+@pytest.mark.parametrize("wtype", [ll.W_F8, ll.W_I8])
+@pytest.mark.parametrize("x_type", [ll.T_F32, ll.T_BF16])
+@pytest.mark.parametrize("rows", [1, 12])
+@pytest.mark.parametrize("scale,gated", [(1e-8, True), (2.0 ** -36, True), (2.0 ** -75, False), (2.0 ** 60, False)])
+def test_small_and_large_values_keep_their_digits(wtype, x_type, rows, scale, gated):
+    # one expert, so that the weight is 1; the bounds of the module's head, relative to the sums of magnitudes,
+    # without its absolute share: x of 1e-8 makes activations of 2^-54 through a gate and SiLU, of 2^-36 some 2^-72
+    h, f = 384, 256
+    act = ll.ACT_SILU if gated else ll.ACT_RELU
+    layer = Layer(ll.MoE(h, f, 1, 1, act, gated, wtype, x_type, ll.T_BF16), rows, seed=71)
+    layer.xv[:, :h] *= scale
+    layer.x = layer.xv[:, :h].double().cpu().numpy()
+    layer.run()
+    ll.ops_check()
+    ns, nsh = (3, 3) if x_type == ll.T_F32 else (1, 2)
+    w = {n: layer.w[n][0] for n in layer.w}
+    x = layer.x
+    g, tg = x @ w["gate"].T, (np.abs(x) @ np.abs(w["gate"]).T) * (ns * h + 40) * U
+    a, ta = act64(g, act), 1.13 * tg + 2.0 ** -20 * np.abs(g)
+    if gated:
+        u, tu = x @ w["up"].T, (np.abs(x) @ np.abs(w["up"]).T) * (ns * h + 40) * U
+        ta = ta * (np.abs(u) + tu) + np.abs(a) * tu
+        a = a * u
+        ta = ta + np.abs(a) * U
+    ta = ta + np.abs(a) * (2.0 ** -22 if nsh == 3 else 2.0 ** -16)
+    d = np.abs(w["down"])
+    y = a @ w["down"].T
+    tol = ta @ d.T + ((np.abs(a) + ta) @ d.T) * ((nsh * f + 40) * U + 2.0 ** -19)
+    tol = tol * 1.01 + np.abs(y) * ROUND[x_type]
+    off = np.abs(layer.y[:rows].double().cpu().numpy() - y)
+    assert np.all(off <= tol), np.max(off / tol)
