@@ -486,7 +486,7 @@ int ll_ops_set_wait_limit(uint64_t ns);
  * the activations with 16 bits or more (24 when x is fp32).  d_ids / d_probs [rows][top_k]
  * (NULL to skip) receive the picked experts, largest logit first, and their weights.  A NaN logit
  * ranks below every number.  A row with an infinity or NaN, or an expert with NaN weights, touches no
- * row but its own and those that picked it.  e4m3 experts take values of x and activations below 2^64,
+ * row but its own and those that picked it.  e4m3 experts take values of x and activations up to 2^63,
  * larger ones overflow; sums of 128 products (before the block's scale) below 2^-70 lose digits as
  * fp32's subnormal numbers do.  y may be x; otherwise no buffer overlaps another.
  * d_work: work_bytes >= ll_moe_workspace_bytes(desc, rows), 256-byte aligned device memory that no

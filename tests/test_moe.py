@@ -487,22 +487,14 @@ def test_rows_that_start_on_no_16_bytes_wait_for_no_barrier():
     layer.check()
 
 
-@pytest.mark.gpu
-@pytest.mark.timeout(300)
-@pytest.mark.parametrize("wtype", [ll.W_F8, ll.W_I8])
-@pytest.mark.parametrize("x_type", [ll.T_F32, ll.T_BF16])
-@pytest.mark.parametrize("rows", [1, 12])
-@pytest.mark.parametrize("scale,gated", [(1e-8, True), (2.0 ** -36, True), (2.0 ** -75, False), (2.0 ** 60, False)])
-def test_small_and_large_values_keep_their_digits(wtype, x_type, rows, scale, gated):
-    # one expert, so that the weight is 1; the bounds of the module's head, relative to the sums of magnitudes,
-    # without its absolute share: x of 1e-8 makes activations of 2^-54 through a gate and SiLU, of 2^-36 some 2^-72
-    h, f = 384, 256
-    act = ll.ACT_SILU if gated else ll.ACT_RELU
-    layer = Layer(ll.MoE(h, f, 1, 1, act, gated, wtype, x_type, ll.T_BF16), rows, seed=71)
-    layer.xv[:, :h] *= scale
-    layer.x = layer.xv[:, :h].double().cpu().numpy()
+def within_relative_bounds(layer):
+    """Run a layer of one expert (so that its weight is 1): the bounds of the module's head, relative to the sums of
+    magnitudes, without its absolute share."""
+    layer.x = layer.xv[:, :layer.m.hidden].double().cpu().numpy()
     layer.run()
     ll.ops_check()
+    m, rows, x_type, act = layer.m, layer.rows, layer.m.x_type, layer.m.act
+    h, f, gated = m.hidden, m.inter, m.gated
     ns, nsh = (3, 3) if x_type == ll.T_F32 else (1, 2)
     w = {n: layer.w[n][0] for n in layer.w}
     x = layer.x
@@ -520,3 +512,30 @@ def test_small_and_large_values_keep_their_digits(wtype, x_type, rows, scale, ga
     tol = tol * 1.01 + np.abs(y) * ROUND[x_type]
     off = np.abs(layer.y[:rows].double().cpu().numpy() - y)
     assert np.all(off <= tol), np.max(off / tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.timeout(300)
+@pytest.mark.parametrize("wtype", [ll.W_F8, ll.W_I8])
+@pytest.mark.parametrize("x_type", [ll.T_F32, ll.T_BF16])
+@pytest.mark.parametrize("rows", [1, 12])
+@pytest.mark.parametrize("scale,gated", [(1e-8, True), (2.0 ** -36, True), (2.0 ** -75, False), (2.0 ** 60, False)])
+def test_small_and_large_values_keep_their_digits(wtype, x_type, rows, scale, gated):
+    # x of 1e-8 makes activations of 2^-54 through a gate and SiLU, of 2^-36 some 2^-72
+    h, f = 384, 256
+    act = ll.ACT_SILU if gated else ll.ACT_RELU
+    layer = Layer(ll.MoE(h, f, 1, 1, act, gated, wtype, x_type, ll.T_BF16), rows, seed=71)
+    layer.xv[:, :h] *= scale
+    within_relative_bounds(layer)
+
+
+@pytest.mark.gpu
+@pytest.mark.timeout(300)
+@pytest.mark.parametrize("rows", [1, 9])
+def test_the_largest_fp32_values_are_finite(rows):
+    # above the largest bf16 number, which the first of their three terms must not exceed
+    layer = Layer(ll.MoE(128, 96, 1, 1, ll.ACT_RELU, False, ll.W_BF16, ll.T_F32, ll.T_BF16), rows, seed=81)
+    layer.xv.zero_()
+    for i in range(rows):
+        layer.xv[i, 7 * i] = 3.4e38 if i % 2 else -3.402e38
+    within_relative_bounds(layer)
