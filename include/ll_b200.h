@@ -439,17 +439,18 @@ int ll_batched_mlp_destroy(ll_batched_mlp *m);
  * fp32 (at least 2^-126; the power of two at or above that when pow2_scales = 1), q = e4m3 nearest
  * to x / s, ties to even.  A group of zeros has scale 0.  NaN stays in its place; a group that
  * holds an infinity gets an infinite scale and stands for NaN throughout.  Strides of 0 mean dim.
- * Bytes of a row of q from dim on are left as they are.
+ * Bytes of a row of q from dim on are left as they are.  The buffers do not overlap.
  */
 int ll_quantize_fp8(const void *d_x, int x_type, int rows, int dim, int64_t ldx, int pow2_scales, uint8_t *d_q,
                     int64_t ldq, float *d_s, void *stream);
 /* The same for a weight matrix on the host, W [m x k] row-major: q [m x k], s [ceil(m/128)][ceil(k/128)],
- * s = max|W| / 448 of the block (1 for a block of zeros), q nearest to W / s. */
+ * s = max|W| / 448 of the block (at least 2^-126; 1 for a block of zeros), q nearest to W / s. */
 void ll_quantize_fp8_blocks(const float *W, int m, int k, uint8_t *q, float *s);
 /*
  * ll_dense_fp8: y[r] = act(W x[r] + b) for `rows` rows on the tensor cores, W [M x K] e4m3 with
  * scales sw [ceil(M/128)][ceil(K/128)], x [rows x K] e4m3 with scales sx [rows][ceil(K/128)], b fp32
- * [M] or NULL.  Sums are fp32.  y_type: LL_T_F32, LL_T_BF16, LL_T_F16 (d_sy unused), or LL_T_F8: y as
+ * [M] or NULL.  Sums are fp32, and so is the product of a block's two scales (it loses digits below
+ * 2^-126).  y_type: LL_T_F32, LL_T_BF16, LL_T_F16 (d_sy unused), or LL_T_F8: y as
  * ll_quantize_fp8 would make it of the fp32 result (the next layer's input), its scales in
  * d_sy [rows][ceil(M/128)].  ldw, ldx (bytes) and ldy (elements): row strides, 0 = dense; the rows
  * of W and x start on 16 bytes, so ldw and ldx are multiples of 16.  What lies beyond column K of
@@ -482,8 +483,8 @@ int ll_ops_set_wait_limit(uint64_t ns);
  * down_scale [n_experts][hidden], as ll_quantize_int8_rows makes them); LL_W_F8 with scales per
  * 128 x 128 block of each expert's matrix (as ll_quantize_fp8_blocks makes them).  x and y are
  * [rows x hidden] in x_type (fp32, bf16, fp16), row strides ldx / ldy elements (0 = hidden);
- * rows <= LL_MOE_MAX_ROWS, 0 does nothing.  All sums are fp32; the weights are used exactly, x exactly,
- * the activations with 16 bits or more (24 when x is fp32).  d_ids / d_probs [rows][top_k]
+ * rows <= LL_MOE_MAX_ROWS, 0 does nothing.  All sums are fp32 (of int8 weights before their scale); the
+ * weights are used exactly, x exactly, the activations with 16 bits or more (24 when x is fp32).  d_ids / d_probs [rows][top_k]
  * (NULL to skip) receive the picked experts, largest logit first, and their weights.  A NaN logit
  * ranks below every number.  A row with an infinity or NaN, or an expert with NaN weights, touches no
  * row but its own and those that picked it.  e4m3 experts take values of x and activations up to 2^63,

@@ -124,23 +124,22 @@ __device__ __forceinline__ float2 unpack_bf16(uint32_t w)
     return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
 
-// Rounded towards zero.
-__device__ __forceinline__ uint32_t pack_bf16_rz(float lo, float hi)
+// The same, but at most the largest bf16 number: also for an infinity, whose second term is then infinite.
+__device__ __forceinline__ uint32_t pack_bf16_finite(float lo, float hi)
 {
     uint32_t w;
-    asm("cvt.rz.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));
+    asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));
     return w;
 }
 
-// (a, b) as NS packed bf16 terms each; an infinity or NaN keeps its first term alone.  Three terms are the 24 bits
-// of an fp32 value, cut into eights: rounded to nearest, the largest values would become infinite.  Two
-// are the nearest value of 16 bits.
+// (a, b) as NS packed bf16 terms each.  Three terms are an fp32 value exactly; two are the nearest value of 16
+// bits, and an infinity or NaN keeps its first term alone.
 template <int NS>
 __device__ __forceinline__ void split_pair(float a, float b, uint32_t (&w)[NS])
 {
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
-        w[s] = NS == 3 ? pack_bf16_rz(a, b) : pack_bf16(a, b);
+        w[s] = NS == 3 && s == 0 ? pack_bf16_finite(a, b) : pack_bf16(a, b);
         if (s + 1 < NS) {
             const float2 h = unpack_bf16(w[s]);
             a = fabsf(h.x) <= 3.4e38f ? a - h.x : 0.0f;

@@ -735,3 +735,15 @@ def test_quantize_ties_of_the_smallest_scales(x_type):
     want_q, want_s = quantize_rows(x)
     assert np.array_equal(s, want_s)
     assert np.array_equal(decode(q), decode(want_q))
+
+
+@pytest.mark.gpu
+@pytest.mark.timeout(300)
+@pytest.mark.parametrize("rows,M,K", [(17, 12300, 200), (32, 14336, 256), (100, 12288, 144)])
+@pytest.mark.parametrize("y_type", [ll.T_BF16, ll.T_F8])
+def test_dense_wide_layers_of_few_rows(rows, M, K, y_type):
+    # tiles of 128 rows of which most do not exist
+    c = DenseCase(rows, M, K, seed=91)
+    y, sy = c.run(ll.ACT_GELU, y_type, pad_y=4)
+    ll.ops_check()
+    c.check(ll.ACT_GELU, y_type, y, sy)

@@ -539,3 +539,21 @@ def test_the_largest_fp32_values_are_finite(rows):
     for i in range(rows):
         layer.xv[i, 7 * i] = 3.4e38 if i % 2 else -3.402e38
     within_relative_bounds(layer)
+
+
+@pytest.mark.gpu
+@pytest.mark.timeout(300)
+@pytest.mark.parametrize("wtype", [ll.W_BF16, ll.W_F8])
+@pytest.mark.parametrize("rows", [3, 12])
+def test_infinities_and_nan_of_fp32_rows_stay_in_their_rows(wtype, rows):
+    m = ll.MoE(256, 128, 8, 2, wtype=wtype, x_type=ll.T_F32)
+    clean, layer = Layer(m, rows), Layer(m, rows)
+    clean.run()
+    layer.xv[0, 7] = float("inf")
+    layer.xv[2, 9] = float("nan")
+    layer.run()
+    ll.ops_check()
+    y, want = layer.y.cpu().numpy()[:rows], clean.y.cpu().numpy()[:rows]
+    assert not np.isfinite(y[[0, 2]]).any()
+    keep = np.delete(np.arange(rows), [0, 2])
+    assert np.array_equal(y[keep], want[keep])
