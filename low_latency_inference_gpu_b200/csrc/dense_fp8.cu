@@ -128,8 +128,8 @@ __device__ __forceinline__ void store_y4(const DenseF8Params &p, long long row, 
 //     as their operands land and wait for nobody;
 //   * 4 stages of 18 KB at 16 rows, so that two CTAs fit an SM and the next launch's set-up
 //     (barriers, tensor memory, tensor maps) runs beside this one's end (programmatic dependent launch).
-// Back to back in a graph: 1 x 2048 x 2048 4.0 us, 32 x 4096 x 4096 with e4m3 output 7.2 (16.8 MB of weights, 2.4
-// TB/s), 256 x 2048 x 2048 8.2.
+// Back to back in a graph: 1 x 2048 x 2048 4.0 us, 32 x 4096 x 4096 with e4m3 output 6.7 (16.8 MB of weights, 2.5
+// TB/s), 256 x 2048 x 2048 7.8.
 //   warp 0     TMA producer (W box 16 KB + X box NT * 128 B per K block)
 //   warp 1     TMEM allocation; one lane issues the MMAs
 //   warps 2-5  lane = channel: TMEM -> registers, times the block's scales
@@ -431,8 +431,10 @@ __global__ void __launch_bounds__(kDsThreads, 1) ll_dense_fp8_kernel(const __gri
 // rows of x and half of the tile's channels; the 2-SM instruction reads the other half from the
 // peer, so an SM's shared memory takes in 32 KB and gives 32 KB per K block of 512 tensor cycles,
 // just its 128 bytes a cycle (a 128 x 256 tile of one SM wants 192).
-// 8192 x 4096 x 4096 with GELU and bf16 output: 156 us, 1758 TFLOP/s; without the store 125, and with the
-// instructions and loads alone 91, which twice the measured bf16 rate would do in 82.
+// 8192 x 4096 x 4096 with GELU, back to back in a graph: bf16 output 151 us, 1820 TFLOP/s (171 called in a row for
+// 70 ms, under the power cap), fp32 161, e4m3 320, whose group maxima and roundings of 128 values per thread spill.
+// Of a bf16 output at 156 us the loop without the store took 125, the instructions and loads alone 91, which
+// twice the measured bf16 rate would do in 82.
 // The loads from TMEM follow each other without a pause, across blocks too, each beside the multiply-adds of
 // the 32 columns before it (all of a block's loads and then its last sums: 167).
 // A K block's way out is 32 K values per CTA from TMEM and as many multiply-adds by the block's

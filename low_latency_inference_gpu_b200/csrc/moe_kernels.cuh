@@ -16,11 +16,12 @@
 // soon as a stage is read) and keeps the tile's sums in registers.  Nothing is handed from warp to
 // warp on the way, so the warps drift apart and cover each other's latencies.  For up to 8 rows two
 // warps share a tile, half of its columns each, as there are few tiles then.
-// Measured back to back in a graph, both kernels: 32 rows, 8 of 64 gated experts 2048 -> 1024 in bf16
-// (794 MB of weights) 224 us, 3.5 TB/s, where streaming them without the products takes 163: the
-// widths of a copy (256 bytes of a row) and the issue slots of copies and fragments hold it there.
-// One row, 8 of 64 e4m3 experts (50 MB) 31 us and 2 of 8 bf16 experts 1024 -> 512 15 us, of which
-// kernel 1 spends 7 to 10 on logits and choice before its first weight arrives: latency.
+// Measured back to back, both kernels: 32 rows, 8 of 64 gated experts 2048 -> 1024 in bf16 (794 MB of
+// weights) 185 us, 4.3 TB/s, with one layer again and again, and 260 us, 3.1 TB/s, with three layers in turn, in
+// a graph as in calls: short copies (256 bytes of a row) all over 2.4 GB.  The same with e4m3 experts 421 us
+// (three layers): x and the sums of four n-tiles beside the widened weights spill.  One row, 8 of 64 e4m3
+// experts (50 MB) 31 us and 2 of 8 bf16 experts 1024 -> 512 15 us, of which kernel 1 spends 7 to 10 on
+// logits and choice before its first weight arrives: latency.
 //
 // Precision: weights are exact in bf16 (int8 and e4m3 too; their scales multiply fp32 sums).  x
 // and the activations a are split into bf16 terms that add up to the value: x in bf16 one, fp16
