@@ -133,8 +133,8 @@ __device__ __forceinline__ uint32_t pack_bf16_finite(float lo, float hi)
     return w;
 }
 
-// (a, b) as NS packed bf16 terms each.  Three terms are an fp32 value exactly; two are the nearest value of 16
-// bits, and an infinity or NaN keeps its first term alone.
+// (a, b) as NS packed bf16 terms each.  Three terms are an fp32 value exactly (from 2^-110 on: bf16's numbers end
+// at 2^-133); two are the nearest value of 16 bits, and an infinity or NaN keeps its first term alone.
 template <int NS>
 __device__ __forceinline__ void split_pair(float a, float b, uint32_t (&w)[NS])
 {
