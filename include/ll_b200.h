@@ -485,8 +485,8 @@ int ll_ops_set_wait_limit(uint64_t ns);
  * [rows x hidden] in x_type (fp32, bf16, fp16), row strides ldx / ldy elements (0 = hidden);
  * rows <= LL_MOE_MAX_ROWS, 0 does nothing.  All sums are fp32 (of int8 weights before their scale); the
  * weights are used exactly, x exactly (fp32 values from 2^-110 on, below that to 2^-133), the activations
- * with 16 bits or more (24 when x is fp32).  d_ids / d_probs [rows][top_k] (NULL to skip) receive the picked experts, largest logit first, and their weights.  A NaN logit
- * ranks below every number.  A row with an infinity or NaN, or an expert with NaN weights, touches no
+ * with 16 bits or more (24 when x is fp32).  d_ids / d_probs [rows][top_k] (NULL to skip) receive the
+ * picked experts, largest logit first, and their weights.  A NaN logit ranks below every number.  A row with an infinity or NaN, or an expert with NaN weights, touches no
  * row but its own and those that picked it.  e4m3 experts take values of x and activations up to 2^63,
  * larger ones overflow; sums of 128 products (before the block's scale) below 2^-70 lose digits as
  * fp32's subnormal numbers do.  y may be x; otherwise no buffer overlaps another.
